@@ -61,6 +61,21 @@ class ConvDesc(C.Structure):
     ]
 
 
+class AttnDesc(C.Structure):
+    """Mirror of ``dc_attn_desc``: one masked attention call (forward, or backward with the gradients' fields)."""
+
+    _fields_ = [
+        ("type", i32), ("nb", i32), ("tq", i32), ("tk", i32), ("heads", i32), ("kv_heads", i32), ("d", i32),
+        ("q", vp), ("k", vp), ("v", vp), ("o", vp), ("lse", vp),
+        ("ldq", i32), ("ldk", i32), ("ldv", i32), ("ldo", i32),
+        ("scale", f32), ("softcap", f32), ("slopes", vp), ("causal", i32),
+        ("prefix", vp), ("kv_len", vp), ("doc_q", vp), ("doc_k", vp),
+        ("dout", vp), ("dq", vp), ("dk", vp), ("dv", vp),
+        ("lddo", i32), ("lddq", i32), ("lddk", i32), ("lddv", i32),
+        ("ws", vp), ("ws_bytes", i64),
+    ]
+
+
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 _SIGS = {
     "dc_abi_version": [],
@@ -80,6 +95,9 @@ _SIGS = {
     "dc_layernorm_bwd": [vp, i32, i64, i32, vp, vp, vp, i32, vp, i32, vp, i32, vp],
     "dc_attn_fwd": [vp, i32, i32, i32, i32, vp, i32, vp, vp, i64, vp],
     "dc_attn_bwd": [vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp],
+    "dc_attn_mask_ws_bytes": [C.POINTER(AttnDesc), i32],
+    "dc_attn_mask_fwd": [C.POINTER(AttnDesc), vp],
+    "dc_attn_mask_bwd": [C.POINTER(AttnDesc), vp],
     "dc_crossattn_tables_bytes": [i32, i32],
     "dc_crossattn_prepare": [vp, vp, i32, i32, vp, vp],
     "dc_crossattn_fwd": [vp, i32, i64, i32, i32, f32, vp, vp, vp, vp, vp, i32, vp, vp, vp, f32, vp],
@@ -150,7 +168,7 @@ _SIGS.update({
 })
 _RESTYPE = {"dc_session_error": C.c_char_p, "dc_sample_params_default": None,
             "dc_build_id": C.c_char_p, "dc_mask_rows_ws_bytes": i64, "dc_groupnorm_ws_bytes": i64, "dc_gn_acc_bytes": i64, "dc_dense_loss_ws_bytes": i64, "dc_depth_metrics_ws_bytes": i64,
-             "dc_ensemble_ws_bytes": i64, "dc_crossattn_tables_bytes": i64}
+             "dc_attn_mask_ws_bytes": i64, "dc_ensemble_ws_bytes": i64, "dc_crossattn_tables_bytes": i64}
 
 STATUS = {0: "ok", 1: "invalid argument / shape", 2: "kernel launch failed", 3: "alignment contract violated"}
 

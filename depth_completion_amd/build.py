@@ -17,11 +17,11 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libdcamd.so"
 OBJ_DIR = PKG / "build_obj"
 SOURCES = ["conv_gemm.hip", "conv_skinny9.hip", "conv_skinny1.hip", "conv_skinny9_gn.hip", "conv_skinny9_gnb.hip",
-           "conv_skinny1_gn.hip", "conv_skinny1_gnb.hip", "conv_gemm_gn.hip", "conv_gemm_gnb.hip", "conv_gemm_ln.hip", "norms.hip", "attention.hip", "crossattn.hip", "elementwise.hip", "guidance.hip", "metrics.hip", "vae_kl.hip",
+           "conv_skinny1_gn.hip", "conv_skinny1_gnb.hip", "conv_gemm_gn.hip", "conv_gemm_gnb.hip", "conv_gemm_ln.hip", "norms.hip", "attention.hip", "attn_mask_fwd.hip", "attn_mask_bwd.hip", "crossattn.hip", "elementwise.hip", "guidance.hip", "metrics.hip", "vae_kl.hip",
            "rowsets.hip", "ensemble.hip", "host_tables.cpp", "session.cpp", "version.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("DC_OFFLOAD_ARCH", "gfx950")
-HEADERS = [CSRC / h for h in ("common.h", "gn_acc.h", "conv_gemm_impl.h", "conv_skinny.h", "json_mini.h", "safetensors_mini.h")] + \
+HEADERS = [CSRC / h for h in ("common.h", "gn_acc.h", "attn_mask.h", "conv_gemm_impl.h", "conv_skinny.h", "json_mini.h", "safetensors_mini.h")] + \
     [PKG.parent / "include" / "dcamd.h"]
 # no packed fp32 instructions: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code, and some of their operand
 # forms have returned wrong values on these cards (the host pass's warning about the unknown feature is harmless)
@@ -30,7 +30,7 @@ FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wno-unused-re
 # per-file additions: the attention softmax's fp32 row sums must stay scalar v_add_f32 -- the SLP vectoriser pairs
 # them into v_pk_add_f32 behind register moves, which issue slower beside the partner wave's MFMAs
 # (MI355X_MICROARCH.md cycle constants, 'packed f32 VALU')
-FILE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"]}
+FILE_FLAGS = {f: ["-fno-slp-vectorize"] for f in ("attention.hip", "attn_mask_fwd.hip", "attn_mask_bwd.hip")}
 
 
 def source_files() -> list[Path]:

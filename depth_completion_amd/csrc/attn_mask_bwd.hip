@@ -1,0 +1,533 @@
+// Masked attention backward (gfx950): the gradients of q, k and v from the inputs, the output, its log-sum and its gradient.
+//
+//   P = exp(s - lse), dP = dO V^T, dS = P (dP - rowsum(dO o)) (1 - tanh^2), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO
+//
+// Two kernels, each holding one side in registers and sweeping the other through LDS, so every sum has one owner and a fixed
+// order: dq_kernel (128 query rows of a head; it also leaves the row constants), then dkv_kernel (128 keys of a key head, over all
+// query heads of its group).  Both compute S and dP again: 7 products for 5, for no exchange of dQ between blocks.
+//
+// fp16: dS is scaled by a power of two before it is rounded, by the row's (dQ) or the key head's (dK) largest |dO| so that this
+// lies in [2^-4, 2^-3): gradients far below 1 keep their digits, and dS stays in range while |v| < 2000.  P in dV is held 2^14 times
+// as large for the same reason.  Both factors are taken out of the fp32 sums again.
+#include "attn_mask.h"
+
+namespace dcm {
+namespace {
+
+struct Back {
+  float *nlse, *ndel;   // [nb heads][tq]: -lse log2 e (-inf: the row sees no key), -rowsum(dO o)
+  int2* rows32;         // [nb heads][n32]: of 32 rows, whether one sees no key, and the largest |dO| (its bits)
+  int n32;
+  int nk;               // splits of dkv_kernel's sweep
+  float* part;          // [nk][2][nb tk][kvh][DP]
+};
+
+template <typename T> constexpr bool is_half = __is_same(T, half);
+
+// power of two that brings a positive finite x into [2^-4, 2^-3)
+__device__ __forceinline__ float near_sixteenth(float x) {
+  if (!(x > 0.0f && x < INFINITY)) return 1.0f;
+  const int e = (int)(__float_as_uint(x) >> 23) - 127;
+  return ldexpf(1.0f, min(max(-4 - e, -100), 100));
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
+  typedef typename Vec<T>::v8 v8;
+  constexpr int TILE = 64 * DP;
+  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
+  __shared__ int ids[2][64];
+  __shared__ int range[4];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
+  const int nqb = (p.tq + 127) / 128, per_head = nqb * p.grp, total = p.nb * p.kvh * per_head;
+  int w = xcd_work(total);
+  if (w >= total) return;
+  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
+  w %= per_head;
+  const int h = kh * p.grp + w % p.grp, qb = nqb - 1 - w / p.grp;
+  const int len = length_of(p, b), q0 = qb * 128, qi = q0 + wid * 32 + (lane & 31);
+  const bool live = qi < p.tq;
+  const int pos = qi + len - p.tq;
+  const int pre = p.prefix ? p.prefix[b] : 0;
+  const long row = ((long)b * p.heads + h) * p.tq + (live ? qi : 0), trow = (long)b * p.tq + (live ? qi : 0);
+  const float lse = p.lse[row];
+  const bool sees = live && lse != -INFINITY;
+  v8 qf[DP / 16], df[DP / 16];
+  float del = 0.0f, most = 0.0f;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int c = 16 * s + 8 * hh;
+    const bool ok = sees && c < p.d;
+    qf[s] = load8_or_0((const T*)p.q + trow * p.ldq + h * p.d + c, ok);
+    df[s] = load8_or_0((const T*)p.dout + trow * p.lddo + h * p.d + c, ok);
+    const v8 of = load8_or_0((const T*)p.o + trow * p.ldo + h * p.d + c, ok);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      del = fmaf((float)df[s][j], (float)of[j], del);
+      most = fmaxf(most, fabsf((float)df[s][j]));
+    }
+  }
+  del = pair_sum(del);
+  most = pair_max(most);
+  const float nl = sees ? -lse * kLog2e : -INFINITY;
+  if (live && hh == 0) {
+    bk.nlse[row] = nl;
+    bk.ndel[row] = -del;
+  }
+  const float wave_most = wave_max(most);
+  const bool blind = __any(live && !sees);
+  if (lane == 0) bk.rows32[((long)b * p.heads + h) * bk.n32 + qb * 4 + wid] = make_int2(blind, __float_as_int(wave_most));
+  const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
+
+  int lim = p.causal ? min(len, max(pos + 1, pre)) : len;
+  const int mine = p.doc_q && live ? p.doc_q[(long)b * p.tq + qi] : 0;
+  if (!sees) lim = 0;
+  if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
+  __syncthreads();
+  atomicMax(&range[1], lim);
+  if (p.doc_q && sees) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
+  __syncthreads();
+  int t0 = 0, t1 = (range[1] + 63) / 64;
+  bool holes = false;
+  if (p.doc_q) {
+    const int nt = (p.tk + 63) / 64, least = range[2], largest = range[3];
+    const int4* sum = p.sum_k + (long)b * nt;
+    int first = 0x7fffffff, last = -1, none = 0;
+    for (int t = threadIdx.x; t < t1; t += 256) {
+      const int4 s = sum[t];
+      if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
+      none |= s.z;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) { range[1] = 0; range[2] = 0; }
+    __syncthreads();
+    if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
+    if (none) atomicOr(&range[2], 1);
+    __syncthreads();
+    t0 = min(range[0], range[1]);
+    t1 = range[1];
+    holes = range[2];
+  }
+
+  const T* kb = (const T*)p.k + (long)b * p.tk * p.ldk + kh * p.d;
+  const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
+  const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
+  Stage<T, DP, 64> ks, vs;
+  int id_next = -1;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int r0 = t * 64, last = len - 1 - r0;
+    ks.load(kb + (long)r0 * p.ldk, p.ldk, p.d, min(last, 63));
+    vs.load(vb + (long)r0 * p.ldv, p.ldv, p.d, min(last, 63));
+    if (kid && threadIdx.x < 64) id_next = kid[min(r0 + (int)threadIdx.x, len - 1)];
+  };
+  auto put = [&](int t, int buf) __attribute__((always_inline)) {
+    const int r0 = t * 64, last = len - 1 - r0;
+    if (last >= 63 && p.d == DP && !holes) {
+      ks.store(tiles[buf]);
+      vs.store(tiles[buf] + TILE);
+    } else {
+      auto keep = [&](int r) { return !holes || (r <= last && kid[r0 + r] >= 0); };
+      ks.store_some(tiles[buf], p.d, last, keep);
+      vs.store_some(tiles[buf] + TILE, p.d, last, keep);
+    }
+    if (kid && threadIdx.x < 64) ids[buf][threadIdx.x] = id_next;
+  };
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
+  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  int koff[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
+  TrAt ka[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) ka[n] = tr_at<DP>(32 * n, lane);
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) fetch(t + 1);
+    const T* kt = tiles[buf];
+    const T* vt = kt + TILE;
+    bool partial = __any(sees && lim < t * 64 + 64);
+    if (kid) partial |= __any(sees && ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        s = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s);
+        dp = mfma(*reinterpret_cast<const v8*>(vt + 32 * kb2 * DP + koff[c]), df[c], dp);
+      }
+      if (p.cap2 != 0.0f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float g;
+          s[r] = cap_score(p, s[r], &g);
+          dp[r] = (dp[r] - del) * g;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] -= del;
+      }
+      if (p.slopes) {
+        const float mul = p.cap2 != 0.0f ? 1.0f : p.scale * kLog2e;
+        const float dist = (float)(pos - t * 64 - 4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[r] * mul);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pw = exp2_raw(fmaf(s[r], p.mul, nl));
+        s[r] = (is_half<T> ? pw * f : pw) * dp[r];
+      }
+      if (partial) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int key = 32 * kb2 + 8 * g + 4 * hh;
+          int4 id = make_int4(0, 0, 0, 0);
+          if (kid) id = *reinterpret_cast<const int4*>(&ids[buf][key]);
+          const int id4[4] = {id.x, id.y, id.z, id.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t * 64 + key + e >= lim || (kid && id4[e] != mine)) s[4 * g + e] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const v8 sf = acc_frag<T>(s, c);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) dq[n] = mfma(tr_frag(kt + (32 * kb2 + 16 * c) * DP, ka[n]), sf, dq[n]);
+      }
+    }
+    if (t + 1 < t1) put(t + 1, buf ^ 1);
+    __syncthreads();
+  }
+  if (!live) return;
+  const float k = p.scale / f;
+  T* out = (T*)p.dq + ((long)b * p.tq + qi) * p.lddq + h * p.d;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * n + 8 * g + 4 * hh;
+      if (col >= p.d) continue;
+      typename Vec<T>::v4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)(sees ? dq[n][4 * g + e] * k : 0.0f);
+      *reinterpret_cast<typename Vec<T>::v4*>(out + col) = v;
+    }
+}
+
+// the factor of dS in dK for a key head: by the largest |dO| of its query heads, the same in every block that needs it
+__device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int b, int kh, float* scratch) {
+  const int2* r = bk.rows32 + ((long)b * p.heads + kh * p.grp) * bk.n32;
+  float most = 0.0f;
+  for (int i = threadIdx.x; i < p.grp * bk.n32; i += 256) most = fmaxf(most, __int_as_float(r[i].y));
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = most;
+  __syncthreads();
+  return near_sixteenth(fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3])));
+}
+
+constexpr float kPShift = 14.0f;   // fp16: P in dV is 2^14 times as large
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back bk) {
+  typedef typename Vec<T>::v8 v8;
+  constexpr int TILE = 64 * DP;
+  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
+  __shared__ __attribute__((aligned(16))) float cn[2][64], cd[2][64];
+  __shared__ __attribute__((aligned(16))) int ids[2][64];
+  __shared__ int range[4];
+  __shared__ float scratch[4];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
+  const int nkb = (p.tk + 127) / 128, per_head = nkb * bk.nk, total = p.nb * p.kvh * per_head;
+  int w = xcd_work(total);
+  if (w >= total) return;
+  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
+  w %= per_head;
+  const int part = w % bk.nk, k0 = w / bk.nk * 128;   // the first keys of a causal call have the longest columns
+  const int len = length_of(p, b), pre = p.prefix ? p.prefix[b] : 0, shift = len - p.tq;
+  const int key = k0 + wid * 32 + (lane & 31);
+  const int mine = p.doc_q ? (key < len ? p.doc_k[(long)b * p.tk + key] : -1) : 0;
+  const bool ok = key < len && mine >= 0;
+  v8 kf[DP / 16], vf[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int c = 16 * s + 8 * hh;
+    kf[s] = load8_or_0((const T*)p.k + ((long)b * p.tk + key) * p.ldk + kh * p.d + c, ok && c < p.d);
+    vf[s] = load8_or_0((const T*)p.v + ((long)b * p.tk + key) * p.ldv + kh * p.d + c, ok && c < p.d);
+  }
+  const float f = is_half<T> ? head_factor(p, bk, b, kh, scratch) : 1.0f;
+  // the lane's key is seen from position `from` on
+  const int from = !ok ? 0x7fffffff : p.causal && key >= pre ? key : -0x7fffffff;
+  int t0 = 0, t1 = (p.tq + 63) / 64;
+  if (p.causal && k0 >= pre) t0 = max(0, k0 - shift) / 64;
+  if (k0 >= len) t1 = 0;
+  if (p.doc_q) {
+    const int nt = (p.tq + 63) / 64;
+    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
+    __syncthreads();
+    if (ok) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
+    __syncthreads();
+    const int least = range[2], largest = range[3];
+    int first = 0x7fffffff, last = -1;
+    for (int t = t0 + threadIdx.x; t < t1; t += 256) {
+      const int4 s = p.sum_q[(long)b * nt + t];
+      if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
+    }
+    if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
+    __syncthreads();
+    t0 = range[0];
+    t1 = range[1];
+  }
+  const int nt = max(0, t1 - t0), steps = nt * p.grp;
+  const int each = (steps + bk.nk - 1) / bk.nk, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
+
+  Stage<T, DP, 64> qs, ds;
+  float cn_next = 0.0f, cd_next = 0.0f;
+  int id_next = -1, blind = 0;
+  int hg_next = nt ? i0 / nt : 0, t_next = nt ? t0 + i0 % nt : 0, put_row0 = 0;
+  long put_at = 0;
+  auto fetch = [&]() __attribute__((always_inline)) {   // the next (query head, tile) of the sweep
+    const int h = kh * p.grp + hg_next, r0 = t_next * 64, last = min(63, p.tq - 1 - r0);
+    const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h;
+    qs.load((const T*)p.q + trow * p.ldq + h * p.d, p.ldq, p.d, last);
+    ds.load((const T*)p.dout + trow * p.lddo + h * p.d, p.lddo, p.d, last);
+    put_row0 = r0;
+    put_at = head * p.tq + r0;
+    if (threadIdx.x < 64) {
+      const int r = min((int)threadIdx.x, last);
+      cn_next = bk.nlse[put_at + r];
+      cd_next = bk.ndel[put_at + r];
+      if (p.doc_q) id_next = p.doc_q[trow + r];
+    }
+    const int2* fl = bk.rows32 + head * bk.n32 + r0 / 32;
+    blind = fl[0].x | (r0 + 32 < p.tq ? fl[1].x : 0);
+    if (++t_next == t1) { t_next = t0; ++hg_next; }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    const int last = p.tq - 1 - put_row0;
+    if (last >= 63 && p.d == DP && !blind) {
+      qs.store(tiles[buf]);
+      ds.store(tiles[buf] + TILE);
+    } else {
+      auto keep = [&](int r) { return !blind || (r <= last && bk.nlse[put_at + r] != -INFINITY); };
+      qs.store_some(tiles[buf], p.d, last, keep);
+      ds.store_some(tiles[buf] + TILE, p.d, last, keep);
+    }
+    if (threadIdx.x < 64) {
+      const bool in = (int)threadIdx.x <= last;
+      cn[buf][threadIdx.x] = in ? cn_next : -INFINITY;
+      cd[buf][threadIdx.x] = in ? cd_next : 0.0f;
+      ids[buf][threadIdx.x] = id_next;
+    }
+  };
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) { dk[n] = f32x16{}; dv[n] = f32x16{}; }
+  int qoff[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) qoff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
+  TrAt ta[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) ta[n] = tr_at<DP>(32 * n, lane);
+  if (i0 < i1) {
+    fetch();
+    put(0);
+  }
+  __syncthreads();
+  int hg = nt ? i0 / nt : 0, t = nt ? t0 + i0 % nt : 0;
+  for (int i = i0; i < i1; ++i) {
+    const int buf = (i - i0) & 1;
+    if (i + 1 < i1) fetch();
+    const T* qt = tiles[buf];
+    const T* dt = qt + TILE;
+    const int pos0 = t * 64 + shift;   // position of the tile's first row
+    bool partial = __any(from > pos0);
+    if (p.doc_q) partial |= __any(ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
+    const float slope = p.slopes ? p.slopes[kh * p.grp + hg] * kLog2e : 0.0f;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      f32x16 s = {}, dp;
+      f32x4 nl[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int r = 32 * qb + 8 * g + 4 * hh;
+        nl[g] = *reinterpret_cast<const f32x4*>(&cn[buf][r]);
+        const f32x4 nd = *reinterpret_cast<const f32x4*>(&cd[buf][r]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] = nd[e];
+      }
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        s = mfma(*reinterpret_cast<const v8*>(qt + 32 * qb * DP + qoff[c]), kf[c], s);
+        dp = mfma(*reinterpret_cast<const v8*>(dt + 32 * qb * DP + qoff[c]), vf[c], dp);
+      }
+      if (p.cap2 != 0.0f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float g;
+          s[r] = cap_score(p, s[r], &g);
+          dp[r] *= g;
+        }
+      }
+      if (p.slopes) {
+        const float mul = p.cap2 != 0.0f ? 1.0f : p.scale * kLog2e;
+        const float dist = (float)(pos0 + 4 * hh - key);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = fmaf(-slope, fabsf(dist + (float)(32 * qb + (r & 3) + 8 * (r >> 2))), s[r] * mul);
+      }
+      const float fs = is_half<T> ? f * 6.103515625e-05f : 1.0f;   // 2^-14
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float up = is_half<T> ? kPShift : 0.0f;
+        s[r] = exp2_raw(fmaf(s[r], p.mul, nl[r >> 2][r & 3] + up));
+        dp[r] *= is_half<T> ? s[r] * fs : s[r];
+      }
+      if (partial) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int r = 32 * qb + 8 * g + 4 * hh;
+          int4 id = make_int4(0, 0, 0, 0);
+          if (p.doc_q) id = *reinterpret_cast<const int4*>(&ids[buf][r]);
+          const int id4[4] = {id.x, id.y, id.z, id.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (pos0 + r + e < from || (p.doc_q && id4[e] != mine)) {
+              s[4 * g + e] = 0.0f;
+              dp[4 * g + e] = 0.0f;
+            }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const v8 pf = acc_frag<T>(s, c), sf = acc_frag<T>(dp, c);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) {
+          dv[n] = mfma(tr_frag(dt + (32 * qb + 16 * c) * DP, ta[n]), pf, dv[n]);
+          dk[n] = mfma(tr_frag(qt + (32 * qb + 16 * c) * DP, ta[n]), sf, dk[n]);
+        }
+      }
+    }
+    if (i + 1 < i1) put(buf ^ 1);
+    if (++t == t1) { t = t0; ++hg; }
+    __syncthreads();
+  }
+  if (key >= p.tk) return;
+  const float kk = p.scale / f, kv = is_half<T> ? 6.103515625e-05f : 1.0f;
+  const long krow = (long)b * p.tk + key;
+  float* pk = nullptr;
+  if (bk.nk > 1) pk = bk.part + (((long)part * 2 * p.nb * p.tk + krow) * p.kvh + kh) * DP;
+  const long other = (long)p.nb * p.tk * p.kvh * DP;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * n + 8 * g + 4 * hh;
+      if (col >= p.d) continue;
+      f32x4 a, c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = ok ? dk[n][4 * g + e] * kk : 0.0f;
+        c[e] = ok ? dv[n][4 * g + e] * kv : 0.0f;
+      }
+      if (pk) {
+        *reinterpret_cast<f32x4*>(pk + col) = a;
+        *reinterpret_cast<f32x4*>(pk + other + col) = c;
+      } else {
+        typename Vec<T>::v4 ta4, tc4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { ta4[e] = (T)a[e]; tc4[e] = (T)c[e]; }
+        *reinterpret_cast<typename Vec<T>::v4*>((T*)p.dk + krow * p.lddk + kh * p.d + col) = ta4;
+        *reinterpret_cast<typename Vec<T>::v4*>((T*)p.dv + krow * p.lddv + kh * p.d + col) = tc4;
+      }
+    }
+}
+
+// dK and dV of a split sweep: the parts added in their order, four columns to a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void dkv_join_kernel(Call p, Back bk) {
+  const long rows = (long)p.nb * p.tk * p.kvh, i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long rk = i / (DP / 4);
+  const int col = (int)(i % (DP / 4)) * 4;
+  if (rk >= 2 * rows || col >= p.d) return;
+  const bool v = rk >= rows;
+  const float* src = bk.part + rk * DP + col;
+  f32x4 a = {};
+  for (int s = 0; s < bk.nk; ++s) a += *reinterpret_cast<const f32x4*>(src + 2L * s * rows * DP);
+  const long r = v ? rk - rows : rk, krow = r / p.kvh;
+  T* out = (v ? (T*)p.dv + krow * p.lddv : (T*)p.dk + krow * p.lddk) + r % p.kvh * p.d + col;
+  typename Vec<T>::v4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (T)a[e];
+  *reinterpret_cast<typename Vec<T>::v4*>(out) = x;
+}
+
+// Splits of dkv_kernel's sweep: where its blocks are fewer than two to a CU, up to 8 and no shorter than 8 tiles each.
+int dkv_splits(const dc_attn_desc* d) {
+  const long blocks = (long)d->nb * d->kv_heads * ((d->tk + 127L) / 128);
+  const long steps = (long)(d->heads / d->kv_heads) * ((d->tq + 63L) / 64);
+  if (blocks >= 512) return 1;
+  return (int)max(1L, min(min((1024 + blocks - 1) / blocks, steps / 8), 8L));
+}
+long pad16(long bytes) { return (bytes + 15) / 16 * 16; }
+
+long rows_bytes(const dc_attn_desc* d) { return pad16(4L * d->nb * d->heads * d->tq); }
+long rows32_bytes(const dc_attn_desc* d) { return pad16(8L * d->nb * d->heads * ((d->tq + 127L) / 128 * 4)); }
+long part_bytes(const dc_attn_desc* d) {
+  const int n = dkv_splits(d);
+  return n > 1 ? 8L * n * d->nb * d->tk * d->kv_heads * (d->d > 64 ? 128 : 64) : 0;
+}
+long bwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d); }
+
+template <typename T, int DP>
+void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
+  hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(xcd_grid((long)c.nb * c.heads * ((c.tq + 127) / 128))), dim3(256), 0, st, c, bk);
+  hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(xcd_grid((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)), dim3(256), 0, st, c,
+                     bk);
+  if (bk.nk > 1) {
+    const long n = 2L * c.nb * c.tk * c.kvh * (DP / 4);
+    hipLaunchKernelGGL((dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, c, bk);
+  }
+}
+
+}  // namespace
+
+long long fwd_ws_bytes(const dc_attn_desc* d);
+
+}  // namespace dcm
+
+using namespace dcm;
+
+extern "C" long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward) {
+  if (!d || d->nb <= 0 || d->tq <= 0 || d->tk <= 0 || d->heads <= 0 || d->kv_heads <= 0) return 0;
+  return backward ? bwd_ws_bytes(d) : fwd_ws_bytes(d);
+}
+
+extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream) {
+  Call c;
+  if (const int rc = make_call(d, c, true)) return rc;
+  if (!d->ws || bwd_ws_bytes(d) > d->ws_bytes) return DC_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = reinterpret_cast<char*>(d->ws);
+  launch_summaries(d, c, ws, st);
+  ws += summary_bytes(d);
+  Back bk;
+  bk.nlse = reinterpret_cast<float*>(ws);
+  bk.ndel = reinterpret_cast<float*>(ws + rows_bytes(d));
+  bk.rows32 = reinterpret_cast<int2*>(ws + 2 * rows_bytes(d));
+  bk.n32 = (d->tq + 127) / 128 * 4;
+  bk.nk = dkv_splits(d);
+  bk.part = reinterpret_cast<float*>(ws + 2 * rows_bytes(d) + rows32_bytes(d));
+  if (d->type == 0) d->d > 64 ? launch_bwd<bf16, 128>(c, bk, st) : launch_bwd<bf16, 64>(c, bk, st);
+  else d->d > 64 ? launch_bwd<half, 128>(c, bk, st) : launch_bwd<half, 64>(c, bk, st);
+  DC_CHECK_LAUNCH();
+  return DC_OK;
+}

@@ -1,0 +1,585 @@
+// Masked attention forward (gfx950): grouped heads, documents, causal with a prefix, filled key lengths, tanh-capped scores and a
+// bias that falls with distance; head dims to 128, bf16 and fp16, 32x32x16 MFMA.
+//
+// Scores are held transposed (S^T = K Q^T, a query to a lane), so the running maximum and sum of a row stay in the lane and
+// P feeds O^T += V^T P^T straight from the accumulator.  Two kernels share that product:
+//   fwd_kernel    128 query rows of one head to a block; the keys' tiles pass through LDS, the next one on its way to registers.
+//   token_kernel  few query rows: all rows of a key head's query heads (up to 32) to a wave, each wave its own 32 keys at a time,
+//                 keys read straight into fragments.  It reads every key and value once, whatever the group.
+// Where rows are few the keys are split over blocks; each writes (m, l, O) in 32 bits and join_kernel adds them in split order.
+#include "attn_mask.h"
+
+namespace dcm {
+namespace {
+
+// least and largest document of 64 rows (rows in none left out), and whether a row is in none
+__global__ __launch_bounds__(256) void summary_kernel(const int* doc, int t, int nt, int total, int4* out) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= total) return;
+  const int b = i / nt, r = (i % nt) * 64 + lane;
+  const int id = r < t ? doc[(long)b * t + r] : -1;
+  const int lo = wave_min_i(id >= 0 ? id : 0x7fffffff), hi = wave_max_i(id);
+  const bool none = __any(r < t && id < 0);
+  if (lane == 0) out[i] = make_int4(lo, hi, none, 0);
+}
+
+// Running softmax of one lane's query over tiles of scores.  m is the reference of the weights 2^(x - m); it follows the row's
+// maximum only when that has grown by more than 8 log2 e, so that most tiles leave O alone.  A row that has seen no key keeps
+// m = -inf and weights of zero.  fp16 weights are held 2^4 times as large: with the slack they reach 2^15.6, and one key among
+// many may weigh 2^-28 before it is rounded away.
+template <typename T, int DP>
+struct Row {
+  static constexpr int NO = DP / 32;
+  static constexpr float SHIFT = sizeof(Vec<T>) && __is_same(T, half) ? 4.0f : 0.0f;
+  float m, l;
+  f32x16 o[NO];
+  __device__ __forceinline__ void init() {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+  }
+  // weights of NB blocks of scores, in place; mul turns a score into an exponent of 2
+  template <int NB>
+  __device__ __forceinline__ void weigh(f32x16 (&s)[NB], float mul) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = pair_max(mx) * mul;
+    if (__any(mx > m + 8.0f * kLog2e)) {
+      const float up = fmaxf(m, mx);
+      const float k = up > m ? exp2_raw(m - up) : 1.0f;
+#pragma unroll
+      for (int n = 0; n < NO; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] *= k;
+      l *= k;
+      m = up;
+    }
+    const float ref = (m == -INFINITY ? 0.0f : m) - SHIFT;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = exp2_raw(fmaf(s[b][r], mul, -ref));
+        sum[r & 3] += s[b][r];
+      }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+  __device__ __forceinline__ void merge(float m2, float l2, const float* o2, int stride) {
+    const float up = fmaxf(m, m2);
+    const float a = up > m ? exp2_raw(m - up) : 1.0f, b = up > m2 ? exp2_raw(m2 - up) : 1.0f;
+    l = l * a + l2 * b;
+#pragma unroll
+    for (int n = 0; n < NO; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[n][r] = o[n][r] * a + o2[(16 * n + r) * stride] * b;
+    m = up;
+  }
+};
+
+struct Split {
+  int n;        // splits of the keys
+  int tiles;    // token_kernel: 32-key steps of a split
+  float* o;     // [row][n][DP]
+  float* ml;    // [row][n][2], row = (sequence, head, query)
+};
+
+// O and the log-sum of a finished row; hh: which half of each eight columns the lane holds
+template <typename T, int DP>
+__device__ __forceinline__ void put_row(const Call& p, const Row<T, DP>& s, float l, long row, long orow, int h, int hh) {
+  const float inv = 1.0f / l;
+  const bool none = l == 0.0f;
+  T* o = (T*)p.o + orow * p.ldo + h * p.d;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * n + 8 * g + 4 * hh;
+      if (col >= p.d) continue;
+      typename Vec<T>::v4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : s.o[n][4 * g + e] * inv);
+      *reinterpret_cast<typename Vec<T>::v4*>(o + col) = v;
+    }
+  if (hh == 0) p.lse[row] = none ? -INFINITY : (s.m + (__builtin_amdgcn_logf(l) - s.SHIFT)) * kLn2;
+}
+template <typename T, int DP>
+__device__ __forceinline__ void put_part(const Split& sp, const Row<T, DP>& s, float l, long row, int part, int hh) {
+  float* o = sp.o + (row * sp.n + part) * DP;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = s.o[n][4 * g + e];
+      *reinterpret_cast<f32x4*>(o + 32 * n + 8 * g + 4 * hh) = v;
+    }
+  if (hh == 0) *reinterpret_cast<float2*>(sp.ml + (row * sp.n + part) * 2) = make_float2(s.m, l);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void fwd_kernel(Call p, Split sp) {
+  typedef typename Vec<T>::v8 v8;
+  constexpr int TILE = 64 * DP;
+  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
+  __shared__ int ids[2][64];
+  __shared__ int range[4];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
+  const int nqb = (p.tq + 127) / 128, per_head = nqb * p.grp * sp.n, total = p.nb * p.kvh * per_head;
+  int w = xcd_work(total);
+  if (w >= total) return;
+  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
+  w %= per_head;
+  const int h = kh * p.grp + w % p.grp;
+  w /= p.grp;
+  const int part = w % sp.n, qb = nqb - 1 - w / sp.n;   // the longest rows of a causal call first
+
+  const int len = length_of(p, b), q0 = qb * 128, qi = q0 + wid * 32 + (lane & 31);
+  const bool live = qi < p.tq;
+  const int pos = qi + len - p.tq;
+  const int pre = p.prefix ? p.prefix[b] : 0;
+  const T* qrow = (const T*)p.q + ((long)b * p.tq + qi) * p.ldq + h * p.d;
+  v8 qf[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, live && 16 * s + 8 * hh < p.d);
+  // the lane's query sees the keys below lim (of its document)
+  int lim = p.causal ? min(len, max(pos + 1, pre)) : len;
+  const int mine = p.doc_q ? (live ? p.doc_q[(long)b * p.tq + qi] : -1) : 0;
+  if (mine < 0) lim = 0;
+  // tiles that some query of the block sees, in a range
+  if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
+  __syncthreads();
+  atomicMax(&range[1], live ? lim : 0);
+  if (p.doc_q && live && mine >= 0) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
+  __syncthreads();
+  int t0 = 0, t1 = (range[1] + 63) / 64;
+  bool holes = false;
+  if (p.doc_q) {
+    const int nt = (p.tk + 63) / 64, least = range[2], most = range[3];
+    const int4* sum = p.sum_k + (long)b * nt;
+    int first = 0x7fffffff, last = -1, none = 0;
+    for (int t = threadIdx.x; t < t1; t += 256) {
+      const int4 s = sum[t];
+      if (s.y >= least && s.x <= most) { first = min(first, t); last = t; }
+      none |= s.z;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) { range[1] = 0; range[2] = 0; }
+    __syncthreads();
+    if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
+    if (none) atomicOr(&range[2], 1);
+    __syncthreads();
+    t0 = min(range[0], range[1]);
+    t1 = range[1];
+    holes = range[2];
+  }
+  if (sp.n > 1) {
+    const int each = (t1 - t0 + sp.n - 1) / sp.n;
+    t0 = min(t1, t0 + part * each);
+    t1 = min(t1, t0 + each);
+  }
+
+  const T* kb = (const T*)p.k + (long)b * p.tk * p.ldk + kh * p.d;
+  const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
+  const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
+  Stage<T, DP, 64> ks, vs;
+  int id_next = -1;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int r0 = t * 64, last = len - 1 - r0;
+    ks.load(kb + (long)r0 * p.ldk, p.ldk, p.d, min(last, 63));
+    vs.load(vb + (long)r0 * p.ldv, p.ldv, p.d, min(last, 63));
+    if (kid && threadIdx.x < 64) id_next = kid[min(r0 + (int)threadIdx.x, len - 1)];
+  };
+  auto put = [&](int t, int buf) __attribute__((always_inline)) {
+    const int r0 = t * 64, last = len - 1 - r0;
+    if (last >= 63 && p.d == DP && !holes) {
+      ks.store(tiles[buf]);
+      vs.store(tiles[buf] + TILE);
+    } else {
+      auto keep = [&](int r) { return !holes || (r <= last && kid[r0 + r] >= 0); };
+      ks.store_some(tiles[buf], p.d, last, keep);
+      vs.store_some(tiles[buf] + TILE, p.d, last, keep);
+    }
+    if (kid && threadIdx.x < 64) ids[buf][threadIdx.x] = id_next;
+  };
+
+  Row<T, DP> st;
+  st.init();
+  const bool shaped = p.cap2 != 0.0f || p.slopes;
+  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  int koff[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
+  TrAt va[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
+
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, 0);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) fetch(t + 1);
+    const T* kt = tiles[buf];
+    const T* vt = kt + TILE;
+    f32x16 s[2];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      s[kb2] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c)
+        s[kb2] = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s[kb2]);
+    }
+    if (shaped) {
+      if (p.cap2 != 0.0f) {
+#pragma unroll
+        for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb2][r] = cap_score(p, s[kb2][r], nullptr);
+      } else {
+#pragma unroll
+        for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb2][r] *= p.scale * kLog2e;
+      }
+      if (p.slopes) {
+        const float dist = (float)(pos - t * 64 - 4 * hh);
+#pragma unroll
+        for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[kb2][r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[kb2][r]);
+      }
+    }
+    bool partial = __any(live && lim < t * 64 + 64);
+    if (kid) partial |= __any(live && ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
+    if (partial) {
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int key = 32 * kb2 + 8 * g + 4 * hh;
+          int4 id = make_int4(0, 0, 0, 0);
+          if (kid) id = *reinterpret_cast<const int4*>(&ids[buf][key]);
+          const int id4[4] = {id.x, id.y, id.z, id.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t * 64 + key + e >= lim || (kid && id4[e] != mine)) s[kb2][4 * g + e] = -INFINITY;
+        }
+    }
+    st.weigh(s, p.mul);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const v8 pf = acc_frag<T>(s[c >> 1], c & 1);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) st.o[n] = mfma(tr_frag(vt + 16 * c * DP, va[n]), pf, st.o[n]);
+    }
+    if (t + 1 < t1) put(t + 1, buf ^ 1);
+    __syncthreads();
+  }
+  const float l = pair_sum(st.l);
+  if (!live) return;
+  const long row = ((long)b * p.heads + h) * p.tq + qi;
+  if (sp.n > 1) put_part<T, DP>(sp, st, l, row, part, hh);
+  else put_row<T, DP>(p, st, l, row, (long)b * p.tq + qi, h, hh);
+}
+
+// One block: up to 32 of the rows (query, head of the group) of one key head, `sp.tiles` steps of 4 x 32 keys.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
+  typedef typename Vec<T>::v8 v8;
+  constexpr int SUB = 32 * DP, NV = SUB / 8 / 64, CH = DP / 8, RED = (2 + DP / 2) * 64;
+  constexpr int BYTES = 4 * SUB * 2 > 3 * RED * 4 ? 4 * SUB * 2 : 3 * RED * 4;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
+  const int rows = p.tq * p.grp, nrb = (rows + 31) / 32, per_head = nrb * sp.n, total = p.nb * p.kvh * per_head;
+  int w = xcd_work(total);
+  if (w >= total) return;
+  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
+  w %= per_head;
+  const int rb = w % nrb, part = w / nrb;
+  const int r = rb * 32 + (lane & 31);
+  const bool live = r < rows;
+  const int qi = live ? r / p.grp : 0, h = kh * p.grp + (live ? r % p.grp : 0);
+  const int len = length_of(p, b), pos = qi + len - p.tq, pre = p.prefix ? p.prefix[b] : 0;
+  int lim = p.causal ? min(len, max(pos + 1, pre)) : len;
+  const int mine = p.doc_q ? p.doc_q[(long)b * p.tq + qi] : 0;
+  if (mine < 0 || !live) lim = 0;
+  const int end = wave_max_i(lim);   // the same in the four waves
+  const T* qrow = (const T*)p.q + ((long)b * p.tq + qi) * p.ldq + h * p.d;
+  v8 qf[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, live && 16 * s + 8 * hh < p.d);
+  const T* kb = (const T*)p.k + (long)b * p.tk * p.ldk + kh * p.d;
+  const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
+  const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
+  T* vt = reinterpret_cast<T*>(smem) + wid * SUB;
+  const bool shaped = p.cap2 != 0.0f || p.slopes;
+  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  TrAt va[DP / 32];
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
+
+  Row<T, DP> st;
+  st.init();
+  v8 kf[DP / 16];
+  uint4 vr[NV];
+  const int steps = (end + 31) / 32, u1 = min(steps, (part + 1) * sp.tiles * 4);
+  // keys from `end` on, and columns from d on, read a place that is valid; their weights, or their columns, are zeroed
+  auto fetch = [&](int u) __attribute__((always_inline)) {
+    const long key = min(u * 32 + (lane & 31), end - 1);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int c = 16 * s + 8 * hh;
+      kf[s] = *reinterpret_cast<const v8*>(kb + key * p.ldk + (c < p.d ? c : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int piece = lane + 64 * i, c = piece % CH * 8;
+      vr[i] = *reinterpret_cast<const uint4*>(vb + (long)min(u * 32 + piece / CH, end - 1) * p.ldv + (c < p.d ? c : 0));
+    }
+  };
+  int u = part * sp.tiles * 4 + wid;
+  if (u < u1) fetch(u);
+  for (; u < u1; u += 4) {
+    int my_key_id = 0;
+    if (kid) {   // a key in no document: its row may hold anything
+      my_key_id = kid[min(u * 32 + (lane & 31), end - 1)];
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+        if (my_key_id < 0) kf[s] = v8{};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (__shfl(my_key_id, (lane + 64 * i) / CH, 64) < 0) vr[i] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int piece = lane + 64 * i;
+      *reinterpret_cast<uint4*>(vt + tile_at<DP>(piece / CH, piece % CH)) = vr[i];
+    }
+    f32x16 s[1] = {f32x16{}};
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) s[0] = mfma(kf[c], qf[c], s[0]);   // qf is zero where the columns end
+    if (u + 4 < u1) fetch(u + 4);
+    if (shaped) {
+      if (p.cap2 != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] = cap_score(p, s[0][e], nullptr);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] *= p.scale * kLog2e;
+      }
+      if (p.slopes) {
+        const float dist = (float)(pos - u * 32 - 4 * hh);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] = fmaf(-slope, fabsf(dist - (float)((e & 3) + 8 * (e >> 2))), s[0][e]);
+      }
+    }
+    if (kid || __any(lim < u * 32 + 32)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = 8 * (e >> 2) + 4 * hh + (e & 3);
+        const bool other = kid && __shfl(my_key_id, key, 64) != mine;
+        if (u * 32 + key >= lim || other) s[0][e] = -INFINITY;
+      }
+    }
+    st.weigh(s, p.mul);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const v8 pf = acc_frag<T>(s[0], c);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) st.o[n] = mfma(tr_frag(vt + 16 * c * DP, va[n]), pf, st.o[n]);
+    }
+  }
+  float l = pair_sum(st.l);
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);
+  if (wid > 0) {
+    float* dst = red + (wid - 1) * RED + lane;
+    dst[0] = st.m;
+    dst[64] = l;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dst[(2 + 16 * n + e) * 64] = st.o[n][e];
+  }
+  __syncthreads();
+  if (wid > 0) return;
+  st.l = l;
+#pragma unroll
+  for (int o = 0; o < 3; ++o) {
+    const float* src = red + o * RED + lane;
+    st.merge(src[0], src[64], src + 128, 64);
+  }
+  if (!live) return;
+  const long row = ((long)b * p.heads + h) * p.tq + qi;
+  if (sp.n > 1) put_part<T, DP>(sp, st, st.l, row, part, hh);
+  else put_row<T, DP>(p, st, st.l, row, (long)b * p.tq + qi, h, hh);
+}
+
+// One wave: one row's splits, joined in their order.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) {
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (lane < sp.n) ml = *reinterpret_cast<const float2*>(sp.ml + (row * sp.n + lane) * 2);
+  const float top = wave_max(ml.x);
+  const float f = ml.x == -INFINITY ? 0.0f : exp2_raw(ml.x - top);
+  // (a split that saw NaN scores alone has m = -inf and l = NaN: it has to reach the result)
+  const float l = wave_sum(ml.y * (ml.y != ml.y ? 1.0f : f));
+  constexpr int E = DP / 64;
+  float o[E] = {};
+  const float* src = sp.o + row * sp.n * DP + lane * E;
+  for (int i = 0; i < sp.n; ++i) {
+    const float k = __shfl(f, i, 64);
+    if (k == 0.0f) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(src[(long)i * DP + e], k, o[e]);
+  }
+  const long bh = row / p.tq, q = row % p.tq, b = bh / p.heads;
+  const int h = (int)(bh % p.heads);
+  const bool none = l == 0.0f;
+  const float inv = 1.0f / l;
+  if (lane * E < p.d) {
+    T* dst = (T*)p.o + (b * p.tq + q) * p.ldo + h * p.d + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = (T)(none ? 0.0f : o[e] * inv);
+  }
+  if (lane == 0) p.lse[row] = none ? -INFINITY : (top + (__builtin_amdgcn_logf(l) - Row<T, DP>::SHIFT)) * kLn2;
+}
+
+constexpr int kMaxSplit = 64;
+
+// Few query rows (at most 32 in a sequence, a quarter of fwd_kernel's block): token_kernel.
+bool few_rows(int tq) { return tq <= 32; }
+
+// How the keys are split.  Enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or more for
+// few rows (the steps a block has cover its start and its merge) and 8 tiles of 64 for many.
+Split split_of(const dc_attn_desc* d) {
+  Split s{1, 0, nullptr, nullptr};
+  const long grp = d->heads / d->kv_heads;
+  if (few_rows(d->tq)) {
+    const long blocks = (long)d->nb * d->kv_heads * ((d->tq * grp + 31) / 32), steps = (d->tk + 127L) / 128;
+    long n = (1024 + blocks - 1) / blocks;
+    n = min(min(n, (steps + 3) / 4), (long)kMaxSplit);
+    s.tiles = (int)((steps + n - 1) / n);
+    s.n = (int)((steps + s.tiles - 1) / s.tiles);
+  } else {
+    const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
+    if (blocks < 256) s.n = (int)min(min((512 + blocks - 1) / blocks, max(tiles / 8, 1L)), (long)kMaxSplit);
+  }
+  return s;
+}
+
+long part_floats(const dc_attn_desc* d, const Split& s) {
+  if (s.n <= 1) return 0;
+  return (long)d->nb * d->heads * d->tq * s.n * ((d->d > 64 ? 128 : 64) + 2);
+}
+
+template <typename T, int DP>
+void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
+  if (few_rows(d->tq)) {
+    const long blocks = (long)c.nb * c.kvh * ((c.tq * c.grp + 31) / 32) * s.n;
+    hipLaunchKernelGGL((token_kernel<T, DP>), dim3(xcd_grid(blocks)), dim3(256), 0, st, c, s);
+  } else {
+    const long blocks = (long)c.nb * c.heads * ((c.tq + 127) / 128) * s.n;
+    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(xcd_grid(blocks)), dim3(256), 0, st, c, s);
+  }
+  const long rows = (long)c.nb * c.heads * c.tq;
+  if (s.n > 1) hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, c, s, rows);
+}
+
+}  // namespace
+
+long long summary_bytes(const dc_attn_desc* d) {
+  if (!d->doc_q) return 0;
+  return 16LL * d->nb * ((d->tq + 63L) / 64 + (d->tk + 63L) / 64);
+}
+
+void launch_summaries(const dc_attn_desc* d, Call& c, char* ws, hipStream_t st) {
+  if (!d->doc_q) return;
+  const int nk = (d->tk + 63) / 64, nq = (d->tq + 63) / 64;
+  int4* k = reinterpret_cast<int4*>(ws);
+  int4* q = k + (long)d->nb * nk;
+  c.sum_k = k;
+  c.sum_q = q;
+  hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * nk + 3) / 4)), dim3(256), 0, st, d->doc_k, d->tk, nk,
+                     d->nb * nk, k);
+  hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * nq + 3) / 4)), dim3(256), 0, st, d->doc_q, d->tq, nq,
+                     d->nb * nq, q);
+}
+
+int make_call(const dc_attn_desc* d, Call& c, bool backward) {
+  if (!d || !d->q || !d->k || !d->v || !d->o || !d->lse || d->type < 0 || d->type > 1) return DC_ERR_ARG;
+  if (d->nb <= 0 || d->tq <= 0 || d->tk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return DC_ERR_ARG;
+  if (d->d <= 0 || d->d > 128 || d->d % 8 || !(d->scale > 0.0f) || !(d->softcap >= 0.0f)) return DC_ERR_ARG;
+  if (!(d->scale <= 1e30f) || !(d->softcap <= 1e30f) || (d->softcap > 0.0f && !(d->scale / d->softcap <= 1e30f))) return DC_ERR_ARG;
+  if (d->prefix && !d->causal) return DC_ERR_ARG;
+  if (!d->doc_q != !d->doc_k) return DC_ERR_ARG;
+  // row and block counts stay within 31 bits
+  const long long rows = (long long)d->nb * d->heads * d->tq;
+  if (rows >= (1LL << 31) || (long long)d->nb * d->tk * d->kv_heads >= (1LL << 31) || d->tq > (1 << 30) || d->tk > (1 << 30))
+    return DC_ERR_ARG;
+  const int hq = d->heads * d->d, hk = d->kv_heads * d->d;
+  if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
+  if (d->ldq % 8 || d->ldk % 8 || d->ldv % 8 || d->ldo % 8) return DC_ERR_ALIGN;
+  const uintptr_t at = (uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o | (uintptr_t)d->ws;
+  if (at & 15) return DC_ERR_ALIGN;
+  if (backward) {
+    if (!d->dout || !d->dq || !d->dk || !d->dv) return DC_ERR_ARG;
+    if (d->lddo < hq || d->lddq < hq || d->lddk < hk || d->lddv < hk) return DC_ERR_ARG;
+    if (d->lddo % 8 || d->lddq % 8 || d->lddk % 8 || d->lddv % 8) return DC_ERR_ALIGN;
+    if (((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) & 15) return DC_ERR_ALIGN;
+  }
+  c = Call{};
+  c.q = d->q; c.k = d->k; c.v = d->v; c.o = d->o; c.lse = d->lse;
+  c.dout = d->dout; c.dq = d->dq; c.dk = d->dk; c.dv = d->dv;
+  c.ldq = d->ldq; c.ldk = d->ldk; c.ldv = d->ldv; c.ldo = d->ldo;
+  c.lddo = d->lddo; c.lddq = d->lddq; c.lddk = d->lddk; c.lddv = d->lddv;
+  c.nb = d->nb; c.tq = d->tq; c.tk = d->tk; c.heads = d->heads; c.kvh = d->kv_heads; c.grp = d->heads / d->kv_heads; c.d = d->d;
+  c.scale = d->scale;
+  c.mul = d->softcap > 0.0f || d->slopes ? 1.0f : d->scale * kLog2e;
+  if (d->softcap > 0.0f) {
+    c.cap2 = d->softcap * kLog2e;
+    c.icap = 2.0f * kLog2e * d->scale / d->softcap;
+  }
+  c.slopes = d->slopes;
+  c.causal = d->causal;
+  c.prefix = d->prefix; c.kv_len = d->kv_len; c.doc_q = d->doc_q; c.doc_k = d->doc_k;
+  return DC_OK;
+}
+
+long long fwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 4LL * part_floats(d, split_of(d)); }
+
+}  // namespace dcm
+
+using namespace dcm;
+
+extern "C" int dc_attn_mask_fwd(const dc_attn_desc* d, void* stream) {
+  Call c;
+  if (const int rc = make_call(d, c, false)) return rc;
+  if (fwd_ws_bytes(d) > (d->ws ? d->ws_bytes : 0)) return DC_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = reinterpret_cast<char*>(d->ws);
+  launch_summaries(d, c, ws, st);
+  Split s = split_of(d);
+  if (s.n > 1) {
+    s.o = reinterpret_cast<float*>(ws + summary_bytes(d));
+    s.ml = s.o + (long)d->nb * d->heads * d->tq * s.n * (d->d > 64 ? 128 : 64);
+  }
+  if (d->type == 0) d->d > 64 ? launch_fwd<bf16, 128>(c, d, s, st) : launch_fwd<bf16, 64>(c, d, s, st);
+  else d->d > 64 ? launch_fwd<half, 128>(c, d, s, st) : launch_fwd<half, 64>(c, d, s, st);
+  DC_CHECK_LAUNCH();
+  return DC_OK;
+}

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch
 
 from . import _lib
-from ._lib import ConvDesc, GnFuse, LnFuse, call
+from ._lib import AttnDesc, ConvDesc, GnFuse, LnFuse, call
 
 BF16 = torch.bfloat16
 
@@ -432,6 +432,114 @@ def attn_bwd(ctx: Ctx, qkv, o, dout, lse, nb, t, heads, delta, dqkv):
     call("dc_attn_bwd", P(qkv), LD(qkv), P(o), LD(o), P(dout), LD(dout), lse.data_ptr(), nb, t, heads,
          delta.data_ptr(), P(dqkv), LD(dqkv), ctx.ws.data_ptr(), ctx.ws_bytes, ctx.stream)
     return dqkv
+
+
+# Operators of a transformer block (masked attention): their operands are checked here, since their lengths, types and masks vary
+# per call; rows may be strided views or Slices whose columns are contiguous.
+TYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _row_view(name: str, t, rows: int, cols: int, dtype, dev: int) -> tuple:
+    """(pointer, row stride) of a 2-D operand that holds ``rows`` x ``cols`` of ``dtype`` on device ``dev``."""
+    col = 0
+    if isinstance(t, Slice):
+        t, col = t.t, t.col
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: {t.dtype}, expected {dtype}")
+    if t.dim() != 2 or t.shape[0] < rows or col < 0 or t.shape[1] - col < cols or (t.stride(1) != 1 and cols > 1):
+        raise ValueError(f"{name}: needs {rows} rows of {cols} contiguous columns, got {tuple(t.shape)} from column {col}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, the context is on device {dev}")
+    return t.data_ptr() + col * t.element_size(), t.stride(0) if t.shape[0] > 1 else -(-cols // 8) * 8
+
+
+def _flat(name: str, t, n: int, dtype, dev: int) -> int | None:
+    """Pointer of a contiguous operand of at least ``n`` values of ``dtype`` on device ``dev`` (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: needs {n} contiguous {dtype} on device {dev}, got {t.numel()} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _launch(dev: int, name: str, *args):
+    """call() with ``dev`` as the current device, where a kernel launch has to find its stream."""
+    if torch.cuda.current_device() == dev:
+        call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args)
+
+
+def _device_of(ctx: Ctx) -> int:
+    if ctx.device.type != "cuda":
+        raise ValueError(f"needs a GPU context, got one on {ctx.device}")
+    return ctx.device.index if ctx.device.index is not None else torch.cuda.current_device()
+
+
+def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, scale, softcap, slopes, causal, prefix, kv_len,
+               doc_q, doc_k):
+    if min(nb, tq, tk, heads, kv_heads, d) <= 0 or heads % kv_heads or d % 8 or d > 128:
+        raise ValueError(f"attn_mask: nb {nb}, tq {tq}, tk {tk}, {heads} heads over {kv_heads}, d {d} "
+                         "(positive; whole groups of heads; d a multiple of 8 up to 128)")
+    base = q.t if isinstance(q, Slice) else q
+    dt = base.dtype
+    if TYPE_IDS.get(dt, 2) > 1:
+        raise ValueError(f"attn_mask: {dt} (bfloat16 or float16)")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30 or not 0.0 <= softcap <= 1e30 or softcap and scale > 1e30 * softcap:
+        raise ValueError(f"attn_mask: scale {scale}, softcap {softcap} (scale above 0, softcap 0 for none, both and scale / softcap at most 1e30)")
+    if prefix is not None and not causal:
+        raise ValueError("attn_mask: a prefix opens a causal mask; without causal every key is seen already")
+    if (doc_q is None) != (doc_k is None):
+        raise ValueError("attn_mask: documents are given for queries and keys, or for neither")
+    dev, hq, hk, nq, nk = _device_of(ctx), heads * d, kv_heads * d, nb * tq, nb * tk
+    pq, ldq = _row_view("q", q, nq, hq, dt, dev)
+    pk, ldk = _row_view("k", k, nk, hk, dt, dev)
+    pv, ldv = _row_view("v", v, nk, hk, dt, dev)
+    po, ldo = _row_view("o", o, nq, hq, dt, dev)
+    i4 = torch.int32
+    desc = AttnDesc(TYPE_IDS[dt], nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po,
+                    _flat("lse", lse, nb * heads * tq, torch.float32, dev), ldq, ldk, ldv, ldo, scale, softcap,
+                    _flat("slopes", slopes, heads, torch.float32, dev), bool(causal), _flat("prefix", prefix, nb, i4, dev),
+                    _flat("kv_len", kv_len, nb, i4, dev), _flat("doc_q", doc_q, nq, i4, dev),
+                    _flat("doc_k", doc_k, nk, i4, dev))
+    if back is not None:
+        desc.dout, desc.lddo = _row_view("dout", back[0], nq, hq, dt, dev)
+        desc.dq, desc.lddq = _row_view("dq", back[1], nq, hq, dt, dev)
+        desc.dk, desc.lddk = _row_view("dk", back[2], nk, hk, dt, dev)
+        desc.dv, desc.lddv = _row_view("dv", back[3], nk, hk, dt, dev)
+    # scratch of the call's own (the allocator hands it on in stream order, a capture takes it from the graph's pool), so calls on
+    # other streams and graphs that replay beside each other share nothing
+    need = _lib.load().dc_attn_mask_ws_bytes(desc, int(back is not None))
+    ws = None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=ctx.device)
+        desc.ws, desc.ws_bytes = ws.data_ptr(), need
+    _launch(dev, "dc_attn_mask_fwd" if back is None else "dc_attn_mask_bwd", desc, ctx.stream)
+
+
+def attn_mask_fwd(ctx: Ctx, q, k, v, o, lse, *, nb: int, tq: int, tk: int, heads: int, kv_heads: int, d: int,
+                  scale: float | None = None, softcap: float = 0.0, slopes=None, causal: bool = False, prefix=None,
+                  kv_len=None, doc_q=None, doc_k=None):
+    """o = softmax(mask(shape(scale q k^T))) v and lse [nb][heads][tq] (include/dcamd.h dc_attn_desc).
+
+    q, o [nb tq][heads d], k, v [nb tk][kv_heads d] in bf16 or fp16; scale 1 / sqrt(d) unless given.  kv_len int32 [nb]: filled
+    keys, of which the query rows are the last; causal, and prefix int32 [nb]: the keys that every row sees all the same;
+    doc_q / doc_k int32 [nb][tq] / [nb][tk]: rows see their own document, below 0 none; slopes fp32 [heads]; softcap: cap c of
+    c tanh(s / c).  A row that sees no key gets o = 0, lse = -inf."""
+    _attn_mask(ctx, None, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, scale, softcap, slopes, causal, prefix, kv_len,
+               doc_q, doc_k)
+    return o
+
+
+def attn_mask_bwd(ctx: Ctx, q, k, v, o, lse, dout, dq, dk, dv, *, nb: int, tq: int, tk: int, heads: int, kv_heads: int, d: int,
+                  scale: float | None = None, softcap: float = 0.0, slopes=None, causal: bool = False, prefix=None,
+                  kv_len=None, doc_q=None, doc_k=None):
+    """Gradients of attn_mask_fwd's q, k and v from its o, lse and dout; every row of dq, dk and dv is written."""
+    _attn_mask(ctx, (dout, dq, dk, dv), q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, scale, softcap, slopes, causal, prefix,
+               kv_len, doc_q, doc_k)
+    return dq, dk, dv
 
 
 def crossattn_tables(ctx: Ctx, U, D, heads, c) -> torch.Tensor:

@@ -450,6 +450,40 @@ int dc_complete(dc_session* s, const void* imgs_u8, const float* sparses, int n,
                 int noise_n, const void* prev, const dc_sample_params* p, float* dense_out, void* latents_out,
                 void* stream);
 
+/* ---------------------------------------------------------------- masked attention (grouped heads, head dim <= 128)
+ * Beside dc_attn_*: query and key rows of their own lengths, types and strides, `heads` query heads over `kv_heads` key heads
+ * (head h reads key head h kv_heads / heads), a mask, and scores that are capped or fall with distance.  Row i of sequence b
+ * stands at pos(i) = i + L - tq, L = kv_len[b] (clamped to 0 .. tk) or tk: the query rows are the last of the filled keys.
+ *   s = scale q_i . k_j;  softcap c > 0: s = c tanh(s / c);  slopes: s -= slopes[h] |pos(i) - j|
+ *   key j counts where j < L, doc_q[i] == doc_k[j] >= 0 (documents given), and j <= pos(i) or j < prefix[b] (causal)
+ *   o = softmax(s) v;  lse = log sum exp(s).  A row that sees no key: o = 0, lse = -inf, and its gradients are 0.
+ * Rows of q / k / v / dout that no pair reaches (keys from L on, documents below 0, rows that see no key) may hold anything.
+ * A visible key that is not finite may also reach other rows of its tile of 64 keys.  Sums and softmax statistics are fp32, the
+ * weights P and dS are rounded to the type for the matrix units (dS of fp16 scaled by a power of two so that small gradients
+ * keep their digits).  Gradients of shared key heads are summed over their query heads in a fixed order; no atomics.
+ * type: 0 bf16, 1 fp16.  d: a multiple of 8.  Pointers 16-byte aligned, ld* multiples of 8.  Inputs and outputs may not overlap. */
+typedef struct dc_attn_desc {
+  int type, nb, tq, tk, heads, kv_heads, d;
+  const void *q, *k, *v;        /* [nb tq][ldq] head h at column h d; [nb tk][ldk], [nb tk][ldv] */
+  void* o;                      /* [nb tq][ldo]; read by the backward */
+  float* lse;                   /* [nb][heads][tq] natural log; read by the backward */
+  int ldq, ldk, ldv, ldo;
+  float scale, softcap;         /* scale > 0; softcap 0: none */
+  const float* slopes;          /* [heads] or NULL; constants, no gradient */
+  int causal;
+  const int* prefix;            /* [nb] or NULL; with causal only */
+  const int* kv_len;            /* [nb] or NULL */
+  const int *doc_q, *doc_k;     /* [nb][tq], [nb][tk], both or NULL */
+  const void* dout;             /* backward: [nb tq][lddo] */
+  void *dq, *dk, *dv;
+  int lddo, lddq, lddk, lddv;
+  float* ws;                    /* scratch of dc_attn_mask_ws_bytes, private to the call until it has run */
+  long long ws_bytes;
+} dc_attn_desc;
+long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward);
+int dc_attn_mask_fwd(const dc_attn_desc* d, void* stream);
+int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

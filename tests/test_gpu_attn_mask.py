@@ -1,0 +1,360 @@
+"""Masked attention (dc_attn_mask_*) against the definition in 64 bits, forward and gradients (GPU).
+
+Tolerances, relative to the 2-norm of the result, u = half a step of the type (bf16 2^-8, fp16 2^-11): the output carries one
+rounding of itself and one of the weights P; the gradients carry one of themselves, one of P or dS and, through rowsum(dO o), one
+of o.  Each is at most u in the norm, so o is held to 2 u and the gradients to 4 u.  Where a row sees one key alone dP and
+rowsum(dO o) cancel: what fp32 sums of d products leave, 2^-18 of the gradients' sum without signs, is allowed beside that.  The
+log-sum is computed in fp32 from exact products: 2e-6 of max(1, |lse|), 1e-5 where scores pass tanh, whose fp32 form is off by
+2e-7 of the cap.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+dev = torch.device("cuda:0")
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from depth_completion_amd.ops import Ctx
+    return Ctx(dev, ws_mb=1)
+
+
+def definition(q, k, v, c, dout=None):
+    """o, lse and gradients in 64 bits on the CPU, a head at a time."""
+    nb, tq, tk, h, g, d = (c[x] for x in ("nb", "tq", "tk", "heads", "kv_heads", "d"))
+    q, k, v = (x.double().cpu().reshape(nb, -1, n, d) for x, n in ((q, h), (k, g), (v, g)))
+    do = None if dout is None else dout.double().cpu().reshape(nb, tq, h, d)
+    scale = c.get("scale") or d ** -0.5
+    cap, slopes = c.get("softcap", 0.0), c.get("slopes")
+    o, lse = torch.zeros(nb, tq, h, d, dtype=torch.float64), torch.zeros(nb, h, tq, dtype=torch.float64)
+    dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    size = {"dq": 0.0, "dk": 0.0, "dv": 0.0}
+    for b in range(nb):
+        n = tk if c.get("kv_len") is None else min(max(int(c["kv_len"][b]), 0), tk)
+        pos, key = torch.arange(tq) + n - tq, torch.arange(tk)
+        see = (key < n)[None].expand(tq, tk)
+        if c.get("causal"):
+            pre = int(c["prefix"][b]) if c.get("prefix") is not None else 0
+            see = see & ((key[None] <= pos[:, None]) | (key[None] < pre))
+        if c.get("doc_q") is not None:
+            iq, ik = c["doc_q"].cpu().view(nb, tq)[b], c["doc_k"].cpu().view(nb, tk)[b]
+            see = see & (iq[:, None] == ik[None]) & (iq[:, None] >= 0)
+        for i in range(h):
+            j = i * g // h
+            # what no pair reaches counts as zero
+            kk, vv = (torch.where(see.any(0)[:, None], x[b, :, j], 0.0) for x in (k, v))
+            qq = torch.where(see.any(1)[:, None], q[b, :, i], 0.0)
+            s = qq @ kk.T * scale
+            slope = 1.0
+            if cap:
+                t = torch.tanh(s / cap)
+                s, slope = t * cap, 1 - t * t
+            if slopes is not None:
+                s = s - float(slopes[i]) * (pos[:, None] - key[None]).abs()
+            s = s.masked_fill(~see, -math.inf)
+            lse[b, i] = torch.logsumexp(s, 1)
+            p = torch.where(see, torch.exp(s - torch.where(see.any(1), lse[b, i], 0.0)[:, None]), 0.0)
+            o[b, :, i] = p @ vv
+            if do is not None:
+                dd = torch.where(see.any(1)[:, None], do[b, :, i], 0.0)
+                dp = dd @ vv.T
+                ds = p * (dp - (p * dp).sum(1, keepdim=True)) * slope * scale
+                dq[b, :, i] = ds @ kk
+                whole = p * (dp.abs() + (p * dp).sum(1, keepdim=True).abs()) * scale
+                size["dq"] += float((whole @ kk.abs()).norm())
+                size["dk"] += float((whole.T @ qq.abs()).norm())
+                dk[b, :, j] += ds.T @ qq
+                dv[b, :, j] += p.T @ dd
+    flat = lambda x: x.reshape(x.shape[0] * x.shape[1], -1)  # noqa: E731
+    return flat(o), lse, flat(dq), flat(dk), flat(dv), size
+
+
+def inputs(c, dtype, seed=0, qscale=1.0, fused=False):
+    g = torch.Generator().manual_seed(seed)
+    nb, tq, tk, h, kv, d = (c[x] for x in ("nb", "tq", "tk", "heads", "kv_heads", "d"))
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v, do = r(nb * tq, h * d) * qscale, r(nb * tk, kv * d), r(nb * tk, kv * d), r(nb * tq, h * d)
+    if fused:   # one row holds q | k | v and a margin
+        row = torch.cat([q, k, v, torch.full((nb * tq, 24), float("nan"))], 1).to(dtype).to(dev)
+        a, b = h * d, kv * d
+        return row[:, :a], row[:, a:a + b], row[:, a + b:a + 2 * b], do.to(dtype).to(dev)
+    return tuple(x.to(dtype).to(dev) for x in (q, k, v, do))
+
+
+def rel(a, b):
+    return float((a.double().cpu() - b).norm() / b.norm().clamp_min(1e-30))
+
+
+def check(ctx, c, dtype, train=True, seed=0, qscale=1.0, fused=False, tensors=None):
+    from depth_completion_amd import ops
+    q, k, v, do = tensors or inputs(c, dtype, seed, qscale, fused)
+    nq, nk = c["nb"] * c["tq"], c["nb"] * c["tk"]
+    hq, hk = c["heads"] * c["d"], c["kv_heads"] * c["d"]
+    pad = 16   # columns behind the last head stay as they were
+    o = torch.full((nq + 1, hq + pad), 7.0, dtype=dtype, device=dev)
+    lse = torch.full((c["nb"], c["heads"], c["tq"]), 7.0, device=dev)
+    kw = {x: y for x, y in c.items()}
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **kw)
+    ro, rl, rq, rk, rv, size = definition(q, k, v, c, do if train else None)
+    u = U[dtype]
+    assert torch.equal(torch.isinf(lse.cpu()), torch.isinf(rl))
+    seen = torch.isfinite(rl)
+    tol = 1e-5 if c.get("softcap") else 2e-6
+    if seen.any():
+        assert float(((lse.cpu().double() - rl)[seen].abs() / rl[seen].abs().clamp_min(1.0)).max()) < tol
+    assert rel(o[:nq, :hq], ro) < 2 * u
+    assert (o[:nq, hq:] == 7).all() and (o[nq:] == 7).all()
+    empty = (~seen).permute(0, 2, 1).reshape(nq, c["heads"], 1).expand(-1, -1, c["d"]).reshape(nq, hq)
+    assert (o[:nq, :hq].cpu()[empty] == 0).all()
+    if not train:
+        return
+    dq, dk, dv = (torch.full((n + 1, w + pad), 7.0, dtype=dtype, device=dev) for n, w in ((nq, hq), (nk, hk), (nk, hk)))
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **kw)
+    for name, x, r, n, w in (("dq", dq, rq, nq, hq), ("dk", dk, rk, nk, hk), ("dv", dv, rv, nk, hk)):
+        assert torch.isfinite(x[:n, :w]).all(), name
+        off = float((x[:n, :w].double().cpu() - r).norm())
+        assert off <= max(4 * u * float(r.norm()), 2.0 ** -18 * size[name]), (name, off, float(r.norm()), size[name])
+        assert (x[:n, w:] == 7).all() and (x[n:] == 7).all(), name
+
+
+def shape(nb, tq, tk, heads, kv_heads, d, **kw):
+    return dict(nb=nb, tq=tq, tk=tk, heads=heads, kv_heads=kv_heads, d=d, **kw)
+
+
+TYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
+@TYPES
+@pytest.mark.parametrize("nb,tq,tk,heads,kv_heads,d", [
+    (1, 1, 1, 1, 1, 64), (1, 1, 432, 20, 20, 64), (3, 1, 700, 8, 2, 128), (2, 5, 1031, 7, 1, 64), (1, 32, 33, 4, 4, 40),
+    (1, 33, 1, 2, 2, 8), (2, 64, 64, 4, 2, 64), (1, 129, 257, 3, 1, 128), (1, 300, 1500, 6, 2, 72), (2, 511, 130, 4, 4, 128)])
+def test_lengths_and_heads(ctx, nb, tq, tk, heads, kv_heads, d, dtype):
+    check(ctx, shape(nb, tq, tk, heads, kv_heads, d), dtype)
+
+
+@TYPES
+@pytest.mark.parametrize("tq,tk,d", [(1, 300, 128), (200, 200, 64), (70, 333, 64), (333, 70, 128), (20, 7, 64)])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_causal_and_prefix(ctx, tq, tk, d, prefix, dtype):
+    c = shape(3, tq, tk, 4, 2, d, causal=True)
+    if prefix:
+        c["prefix"] = torch.tensor([0, tk // 3, tk + 5], dtype=torch.int32, device=dev)
+    check(ctx, c, dtype)
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tq,causal", [(1, True), (4, True), (4, False), (100, True)])
+def test_filled_lengths(ctx, tq, causal, d, dtype):
+    """Keys behind the filled length may hold anything; no length at all leaves rows empty."""
+    lens = [0, 1, 64, 333, 4000, -3]
+    c = shape(6, tq, 400, 6, 2, d, causal=causal, kv_len=torch.tensor(lens, dtype=torch.int32, device=dev))
+    q, k, v, do = inputs(c, dtype, 3)
+    for x in (k, v):
+        for b, n in enumerate(lens):
+            x.view(6, 400, -1)[b, max(n, 0):] = float("nan")
+    check(ctx, c, dtype, tensors=(q, k, v, do))
+
+
+def documents(kind, t, nb=1):
+    g = torch.Generator().manual_seed(t)
+    if kind == "packed":      # ragged, the last one ends inside a tile, padding behind it
+        cuts = [0, t // 3, t // 3 + 1, t // 2, t - t // 7]
+        ids = torch.full((t,), -1)
+        for n in range(4):
+            ids[cuts[n]:cuts[n + 1]] = n + 5
+    elif kind == "mixed":     # any order
+        ids = torch.randint(-1, 4, (t,), generator=g)
+    elif kind == "one":
+        ids = torch.zeros(t, dtype=torch.long)
+    else:                     # nothing belongs anywhere
+        ids = torch.full((t,), -1)
+    return ids.to(torch.int32).repeat(nb).to(dev)
+
+
+@TYPES
+@pytest.mark.parametrize("kind", ["packed", "mixed", "one", "none"])
+@pytest.mark.parametrize("t,d", [(20, 64), (300, 64), (517, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_documents(ctx, kind, t, d, causal, dtype):
+    """Rows in no document hold NaN and infinities in every operand; they reach nothing."""
+    ids = documents(kind, t, 2)
+    c = shape(2, t, t, 4, 2, d, doc_q=ids, doc_k=ids, causal=causal)
+    q, k, v, do = inputs(c, dtype, 5)
+    for n, x in enumerate((q, k, v, do)):
+        x[ids < 0] = float("nan") if n % 2 else float("inf")
+    check(ctx, c, dtype, tensors=(q, k, v, do))
+
+
+def test_documents_across(ctx):
+    """Queries and keys of different counts; a query document without keys and a key document without queries."""
+    iq = torch.tensor([0] * 40 + [3] * 30 + [1] * 31, dtype=torch.int32, device=dev)
+    ik = torch.tensor([1] * 100 + [0] * 90 + [2] * 60 + [-1] * 5, dtype=torch.int32, device=dev)
+    c = shape(1, 101, 255, 2, 1, 64, doc_q=iq, doc_k=ik)
+    check(ctx, c, torch.bfloat16)
+    # the gradients of rows that see nothing may hold anything
+    q, k, v, do = inputs(c, torch.bfloat16, 9)
+    do[40:70] = float("nan")
+    q[40:70] = float("inf")
+    check(ctx, c, torch.bfloat16, tensors=(q, k, v, do))
+
+
+@TYPES
+@pytest.mark.parametrize("tq,tk,d", [(1, 500, 128), (3, 100, 64), (190, 190, 64), (140, 300, 128)])
+@pytest.mark.parametrize("cap,bias", [(20.0, False), (0.0, True), (30.0, True)])
+def test_shaped_scores(ctx, tq, tk, d, cap, bias, dtype):
+    slopes = 2.0 ** -torch.arange(1.0, 7.0, device=dev) if bias else None
+    check(ctx, shape(2, tq, tk, 6, 3, d, softcap=cap, slopes=slopes), dtype, qscale=4.0)
+    check(ctx, shape(2, tq, tk, 6, 3, d, softcap=cap, slopes=slopes, causal=True, scale=0.3), dtype)
+
+
+@TYPES
+def test_scores_far_apart(ctx, dtype):
+    """Scores that rise and fall by hundreds along the keys: the running maximum moves late, early and not at all."""
+    c = shape(1, 96, 640, 2, 1, 64, scale=1.0)
+    q, k, v, do = inputs(c, dtype, 1)
+    ramp = torch.linspace(-6, 6, 640, device=dev)
+    for order in (ramp, ramp.flip(0), ramp.abs()):
+        kk = (k.float() * 0.1 + order[:, None] * q.float()[0, :64].sign()[None]).to(dtype)
+        check(ctx, c, dtype, train=False, tensors=(q, kk, v, do))
+
+
+def test_views_and_slices(ctx):
+    """q | k | v in one row with a margin of NaN, and column slices of row buffers."""
+    from depth_completion_amd import ops
+    c = shape(2, 150, 150, 4, 2, 64, causal=True)
+    check(ctx, c, torch.bfloat16, fused=True)
+    q, k, v, _ = inputs(c, torch.bfloat16, 4)
+    buf = torch.cat([torch.full((300, 8), float("nan"), device=dev), q.float(), k.float(), v.float()], 1).bfloat16()
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    lse = torch.empty(2, 4, 150, device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, a, lse, **c)
+    ops.attn_mask_fwd(ctx, ops.S(buf, 8), ops.S(buf, 264), ops.S(buf, 392), b, lse, **c)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", ["dq", "dk"])
+def test_small_output_gradients_keep_their_digits(ctx, name):
+    """fp16 with dout at the border of its subnormals: dS alone would be a few units of 2^-24.  The other factor is scaled up so
+    that the gradient itself has its digits in the type."""
+    from depth_completion_amd import ops
+    c = shape(1, 300, 300, 2, 1, 64)
+    q, k, v, do = inputs(c, torch.float16, 2)
+    up = 64.0 if name == "dq" else 1 / 64.0
+    q, k, do = (q.float() / up).half(), (k.float() * up).half(), (do.float() * 2.0 ** -14).half()
+    o, lse = torch.empty_like(q), torch.empty(1, 2, 300, device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+    got = dict(zip(("dq", "dk", "dv"), (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))))
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, *got.values(), **c)
+    want = dict(zip(("dq", "dk"), definition(q, k, v, c, do)[2:4]))
+    assert rel(got[name], want[name]) < 4 * U[torch.float16]
+
+
+def test_gradients_by_differences(ctx):
+    """sum(o w) falls as the gradients say when q, k and v move along a direction (fp32 sum of the forward's fp16 output)."""
+    from depth_completion_amd import ops
+    c = shape(1, 80, 80, 4, 2, 64, causal=True, softcap=10.0)
+    q, k, v, w = inputs(c, torch.float16, 6, qscale=0.5)
+    o, lse = torch.empty_like(q), torch.empty(1, 4, 80, device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, w, dq, dk, dv, **c)
+    for x, g in ((q, dq), (k, dk), (v, dv)):
+        step = 2.0 ** -5 * g.float().sign()   # along the gradient's signs: the sum moves by |g|_1 a step
+        vals = []
+        for sign in (1, -1):
+            old = x.clone()
+            x += (sign * step).to(x.dtype)
+            ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+            vals.append((o.double() * w.double()).sum().item())
+            x.copy_(old)
+        want = 2 * 2.0 ** -5 * g.double().abs().sum().item()
+        # third differences of a step of 2^-5 and the rounding of x: below 3 %
+        assert abs(vals[0] - vals[1] - want) < 0.03 * want
+
+
+def test_far_keys(ctx):
+    """A cache whose last rows lie beyond 2^31 elements: the addresses are 64 bits wide."""
+    from depth_completion_amd import ops
+    tk, g, d, ld = 70000, 1, 64, 32768   # 2.3e9 elements, 4.6 GB each
+    k, v = (torch.zeros(tk, ld, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    gen = torch.Generator(device=dev).manual_seed(1)
+    kk, vv = (torch.randn(tk, d, generator=gen, device=dev).bfloat16() for _ in range(2))
+    k[:, :d], v[:, :d] = kk, vv
+    for tq in (1, 40):
+        q = torch.randn(tq, 2 * d, generator=gen, device=dev).bfloat16()
+        c = shape(1, tq, tk, 2, g, d, causal=True)
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        la, lb = (torch.empty(1, 2, tq, device=dev) for _ in range(2))
+        ops.attn_mask_fwd(ctx, q, k, v, a, la, **c)
+        ops.attn_mask_fwd(ctx, q, kk, vv, b, lb, **c)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+        check(ctx, c, torch.bfloat16, train=False, tensors=(q, kk, vv, q))
+
+
+def test_same_bits_every_time(ctx):
+    """No atomics on values: two passes give the same bits, split keys and split sweeps included."""
+    from depth_completion_amd import ops
+    for c in (shape(1, 1, 5000, 8, 2, 128), shape(1, 200, 1500, 8, 1, 64, causal=True)):
+        q, k, v, do = inputs(c, torch.bfloat16, 8)
+        got = []
+        for _ in range(2):
+            o, lse = torch.empty_like(q), torch.empty(1, 8, c["tq"], device=dev)
+            ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+            got.append((o, lse, dq, dk, dv))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_two_graphs_and_a_stream(ctx):
+    """Two captured graphs and an eager call on a third stream run beside each other: each has its own scratch."""
+    from depth_completion_amd import ops
+    cs = [shape(1, 1, 6000, 8, 2, 128, causal=True), shape(1, 260, 260, 4, 2, 64, doc_q=documents("packed", 260),
+                                                            doc_k=documents("packed", 260))]
+    graphs, outs, want = [], [], []
+    side = torch.cuda.Stream()
+    for c in cs:
+        q, k, v, do = inputs(c, torch.bfloat16, 8)
+        bufs = [torch.empty_like(q), torch.empty(1, c["heads"], c["tq"], device=dev), torch.empty_like(q),
+                torch.empty_like(k), torch.empty_like(v)]
+
+        def step(c=c, q=q, k=k, v=v, do=do, bufs=bufs):
+            o, lse, dq, dk, dv = bufs
+            ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+            ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+
+        step()
+        torch.cuda.synchronize()
+        want.append([b.clone() for b in bufs])
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            step()
+        graphs.append((gr, step))
+        outs.append(bufs)
+    other = inputs(cs[0], torch.bfloat16, 8)
+    o3, l3 = torch.empty_like(other[0]), torch.empty(1, 8, 1, device=dev)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(4):
+        for bufs in outs:
+            for b in bufs:
+                b.fill_(3.0)
+        o3.fill_(3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            graphs[0][0].replay()
+        with torch.cuda.stream(s2):
+            graphs[1][0].replay()
+        with torch.cuda.stream(side):
+            ops.attn_mask_fwd(ctx, *other[:3], o3, l3, **cs[0])
+        torch.cuda.synchronize()
+        for bufs, ref in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(bufs, ref))
+        assert torch.equal(o3, want[0][0])
