@@ -98,6 +98,8 @@ _SIGS = {
     "dc_attn_mask_ws_bytes": [C.POINTER(AttnDesc), i32],
     "dc_attn_mask_fwd": [C.POINTER(AttnDesc), vp],
     "dc_attn_mask_bwd": [C.POINTER(AttnDesc), vp],
+    "dc_rotary": [vp, i64, vp, i64, i32, i64, i32, i32, i32, i32, vp, vp, i32, i32, f32, i32, i32, vp],
+    "dc_rotary_freqs": [i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, fp],
     "dc_crossattn_tables_bytes": [i32, i32],
     "dc_crossattn_prepare": [vp, vp, i32, i32, vp, vp],
     "dc_crossattn_fwd": [vp, i32, i64, i32, i32, f32, vp, vp, vp, vp, vp, i32, vp, vp, vp, f32, vp],

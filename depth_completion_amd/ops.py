@@ -434,7 +434,7 @@ def attn_bwd(ctx: Ctx, qkv, o, dout, lse, nb, t, heads, delta, dqkv):
     return dqkv
 
 
-# Operators of a transformer block (masked attention): their operands are checked here, since their lengths, types and masks vary
+# Operators of a transformer block (masked attention, rotary positions): their operands are checked here, since their lengths, types and masks vary
 # per call; rows may be strided views or Slices whose columns are contiguous.
 TYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -540,6 +540,46 @@ def attn_mask_bwd(ctx: Ctx, q, k, v, o, lse, dout, dq, dk, dv, *, nb: int, tq: i
     _attn_mask(ctx, (dout, dq, dk, dv), q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, scale, softcap, slopes, causal, prefix,
                kv_len, doc_q, doc_k)
     return dq, dk, dv
+
+
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def rotary_freqs(rot: int, *, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained: float = 0.0,
+                 fast: float = 32.0, slow: float = 1.0, device=None) -> tuple:
+    """(freqs float64 [rot / 2] on ``device``, mag) of rotary() for heads whose ``rot`` columns turn (include/dcamd.h
+    dc_rotary_freqs: linear, base and parts reach ``factor`` times further; parts goes by the turns over the ``trained`` length)."""
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"rotary_freqs: scaling {scaling!r} (one of {', '.join(ROTARY_SCALINGS)})")
+    if rot <= 0 or rot % 2:
+        raise ValueError(f"rotary_freqs: rot {rot} (even, above 0)")
+    freqs, mag = torch.empty(rot // 2, dtype=torch.float64), C.c_float()
+    call("dc_rotary_freqs", rot, theta, ROTARY_SCALINGS[scaling], factor, trained, fast, slow, freqs.data_ptr(), C.byref(mag))
+    return freqs if device is None else freqs.to(device), mag.value
+
+
+def rotary(ctx: Ctx, x, rows: int, heads: int, d: int, freqs, y=None, *, pos=None, t: int = 0, pos0: int = 0, off: int = 0,
+           interleaved: bool = False, inverse: bool = False, mag: float = 1.0):
+    """Turn the columns [off, off + 2 len(freqs)) of each head of x [rows][heads d] by its position (include/dcamd.h dc_rotary);
+    returns y, or x where it is turned in place.  pos int32 [rows], or rows of sequences of t from pos0 on; q and k that lie side
+    by side are one call over heads + kv_heads.  inverse: the gradient, dL/dx from dL/dy."""
+    rot = 2 * freqs.numel()
+    if rows <= 0 or heads <= 0 or d <= 0 or rot <= 0 or off < 0 or off + rot > d:
+        raise ValueError(f"rotary: {rows} rows of {heads} heads of {d}, {rot} columns from {off}")
+    if pos is None and t <= 0:
+        raise ValueError("rotary: needs the rows' positions, or the length t of the sequences that they form")
+    if not abs(mag) <= 1e30:
+        raise ValueError(f"rotary: mag {mag}")
+    dt = (x.t if isinstance(x, Slice) else x).dtype
+    if dt not in TYPE_IDS:
+        raise ValueError(f"rotary: {dt} (bfloat16, float16 or float32)")
+    dev = _device_of(ctx)
+    px, ldx = _row_view("x", x, rows, heads * d, dt, dev)
+    py, ldy = (px, ldx) if y is None else _row_view("y", y, rows, heads * d, dt, dev)
+    _launch(dev, "dc_rotary", px, ldx, py, ldy, TYPE_IDS[dt], rows, heads, d, off, rot,
+            _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), pos0, t, mag,
+            interleaved, inverse, ctx.stream)
+    return x if y is None else y
 
 
 def crossattn_tables(ctx: Ctx, U, D, heads, c) -> torch.Tensor:

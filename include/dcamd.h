@@ -484,6 +484,20 @@ long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward);
 int dc_attn_mask_fwd(const dc_attn_desc* d, void* stream);
 int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream);
 
+/* ---------------------------------------------------------------- rotary positions
+ * y = x with the columns [off, off + rot) of each of `heads` heads (head h at column h d) turned by angles pos * freqs[i],
+ * i < rot / 2, and multiplied by mag: pairs (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; inverse turns back, which is the
+ * gradient (dL/dx from dL/dy).  y may be x (same ldx); else the other columns are copied.  Angles are formed in 64 bits.
+ * type: 0 bf16, 1 fp16, 2 fp32.  pos: int [rows], or NULL: row r stands at pos0 + r % t.  freqs: [rot / 2] in device memory.
+ * Any d, off and even rot; 16-byte accesses where base, ld, d and off allow them and rot is whole packs. */
+int dc_rotary(const void* x, long long ldx, void* y, long long ldy, int type, long long rows, int heads, int d, int off, int rot,
+              const double* freqs, const int* pos, int pos0, int t, float mag, int interleaved, int inverse, void* stream);
+/* host: freqs[i] = theta^(-2 i / rot) and mag, scaled to reach `factor` times further: 0 not; 1 every frequency / factor; 2 a base
+ * of theta factor^(rot / (rot - 2)) (rot >= 4: the fastest stays, the slowest is divided by factor); 3 by turns over the `trained`
+ * length: fast or more stay, slow or fewer are divided by factor, between them in proportion, and mag = 1 + 0.1 ln factor. */
+int dc_rotary_freqs(int rot, double theta, int scaling, double factor, double trained, double fast, double slow, double* freqs,
+                    float* mag);
+
 #ifdef __cplusplus
 }
 #endif
