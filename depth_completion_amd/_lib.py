@@ -76,6 +76,21 @@ class AttnDesc(C.Structure):
     ]
 
 
+class ResnormDesc(C.Structure):
+    """Mirror of ``dc_resnorm_desc``: the norms around a block with gate and residual scale."""
+
+    _fields_ = [
+        ("type", i32), ("c", i32), ("first", i32), ("second", i32), ("rows", i64), ("gates", i64),
+        ("x", vp), ("y", vp), ("gate", vp), ("w1", vp), ("b1", vp), ("w2", vp), ("b2", vp),
+        ("ldx", i32), ("ldy", i32), ("ldg", i32), ("ldr", i32), ("ldh", i32),
+        ("a", f32), ("s", f32), ("eps", f32), ("r", vp), ("h", vp), ("stats", vp),
+        ("dr", vp), ("dh", vp), ("dx", vp), ("dy", vp), ("dgate", vp),
+        ("dw1", vp), ("db1", vp), ("dw2", vp), ("db2", vp),
+        ("lddr", i32), ("lddh", i32), ("lddx", i32), ("lddy", i32), ("lddg", i32),
+        ("ws", vp), ("ws_bytes", i64),
+    ]
+
+
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 _SIGS = {
     "dc_abi_version": [],
@@ -93,6 +108,9 @@ _SIGS = {
                              vp, i32, vp],
     "dc_layernorm_fwd": [vp, i32, i64, i32, f32, vp, vp, vp, i32, vp, vp],
     "dc_layernorm_bwd": [vp, i32, i64, i32, vp, vp, vp, i32, vp, i32, vp, i32, vp],
+    "dc_resnorm_fwd": [C.POINTER(ResnormDesc), vp],
+    "dc_resnorm_ws_bytes": [C.POINTER(ResnormDesc)],
+    "dc_resnorm_bwd": [C.POINTER(ResnormDesc), vp],
     "dc_attn_fwd": [vp, i32, i32, i32, i32, vp, i32, vp, vp, i64, vp],
     "dc_attn_bwd": [vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp],
     "dc_attn_mask_ws_bytes": [C.POINTER(AttnDesc), i32],
@@ -170,7 +188,7 @@ _SIGS.update({
 })
 _RESTYPE = {"dc_session_error": C.c_char_p, "dc_sample_params_default": None,
             "dc_build_id": C.c_char_p, "dc_mask_rows_ws_bytes": i64, "dc_groupnorm_ws_bytes": i64, "dc_gn_acc_bytes": i64, "dc_dense_loss_ws_bytes": i64, "dc_depth_metrics_ws_bytes": i64,
-             "dc_attn_mask_ws_bytes": i64, "dc_ensemble_ws_bytes": i64, "dc_crossattn_tables_bytes": i64}
+             "dc_attn_mask_ws_bytes": i64, "dc_resnorm_ws_bytes": i64, "dc_ensemble_ws_bytes": i64, "dc_crossattn_tables_bytes": i64}
 
 STATUS = {0: "ok", 1: "invalid argument / shape", 2: "kernel launch failed", 3: "alignment contract violated"}
 

@@ -16,7 +16,7 @@ from pathlib import Path
 import torch
 
 from . import _lib
-from ._lib import AttnDesc, ConvDesc, GnFuse, LnFuse, call
+from ._lib import AttnDesc, ConvDesc, GnFuse, LnFuse, ResnormDesc, call
 
 BF16 = torch.bfloat16
 
@@ -434,7 +434,7 @@ def attn_bwd(ctx: Ctx, qkv, o, dout, lse, nb, t, heads, delta, dqkv):
     return dqkv
 
 
-# Operators of a transformer block (masked attention, rotary positions): their operands are checked here, since their lengths, types and masks vary
+# Operators of a transformer block (masked attention, rotary positions, the norms around it): their operands are checked here, since their lengths, types and masks vary
 # per call; rows may be strided views or Slices whose columns are contiguous.
 TYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -580,6 +580,85 @@ def rotary(ctx: Ctx, x, rows: int, heads: int, d: int, freqs, y=None, *, pos=Non
             _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), pos0, t, mag,
             interleaved, inverse, ctx.stream)
     return x if y is None else y
+
+
+NORMS = {"none": 0, "layer": 1, "rms": 2}
+
+
+def _resnorm(ctx: Ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats):
+    if rows <= 0 or c <= 0 or c % 8 or c > 8192:
+        raise ValueError(f"resnorm: {rows} rows of {c} (a multiple of 8 up to 8192)")
+    if first not in NORMS or second not in NORMS:
+        raise ValueError(f"resnorm: norms {first!r}, {second!r} (of {', '.join(NORMS)})")
+    if first == "none" and (w1 is not None or b1 is not None) or second == "none" and (w2 is not None or b2 is not None):
+        raise ValueError("resnorm: weights of a norm that is none")
+    if not 0.0 <= eps <= 1e30 or not abs(a) <= 1e30 or not abs(s) <= 1e30:
+        raise ValueError(f"resnorm: a {a}, s {s}, eps {eps}")
+    dt = (x.t if isinstance(x, Slice) else x).dtype
+    if dt not in TYPE_IDS:
+        raise ValueError(f"resnorm: {dt} (bfloat16, float16 or float32)")
+    gates = 0
+    if gate is not None:
+        gates = (gate.t if isinstance(gate, Slice) else gate).shape[0]
+        if gates == 0 or rows % gates:
+            raise ValueError(f"resnorm: {gates} gate rows for {rows} rows (one for each of equal runs of rows)")
+    dev = _device_of(ctx)
+    d = ResnormDesc(TYPE_IDS[dt], c, NORMS[first], NORMS[second], rows, gates)
+    d.x, d.ldx = _row_view("x", x, rows, c, dt, dev)
+    d.y, d.ldy = _row_view("y", y, rows, c, dt, dev)
+    if gates:
+        d.gate, d.ldg = _row_view("gate", gate, gates, c, dt, dev)
+    f4 = torch.float32
+    d.w1, d.b1, d.w2, d.b2 = (_flat(n, v, c, f4, dev) for n, v in (("w1", w1), ("b1", b1), ("w2", w2), ("b2", b2)))
+    d.a, d.s, d.eps = a, s, eps
+    d.stats = _flat("stats", stats, 4 * rows, f4, dev)
+    return d, dt, dev
+
+
+def resnorm_fwd(ctx: Ctx, x, y, rows: int, c: int, r, h, stats, *, first: str = "none", second: str = "layer", w1=None, b1=None,
+                w2=None, b2=None, gate=None, a: float = 1.0, s: float = 1.0, eps: float = 1e-5):
+    """r = a x + s gate N1(y) and h = N2(r) in one pass (include/dcamd.h dc_resnorm_desc): x the residual stream, y a block's
+    output.  Norms "none", "layer" or "rms" with fp32 weights (None: 1) and offsets (None: 0); gate [gates][c] in the rows' type,
+    each for rows / gates rows in turn; h None where second is "none"; stats fp32 [rows][4] for the backward.  Returns r, h."""
+    d, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
+    if (second == "none") != (h is None):
+        raise ValueError("resnorm: h goes with a second norm")
+    d.r, d.ldr = _row_view("r", r, rows, c, dt, dev)
+    if h is not None:
+        d.h, d.ldh = _row_view("h", h, rows, c, dt, dev)
+    _launch(dev, "dc_resnorm_fwd", d, ctx.stream)
+    return r, h
+
+
+def resnorm_bwd(ctx: Ctx, x, y, rows: int, c: int, stats, dr, dh, dx, dy, *, first: str = "none", second: str = "layer", w1=None,
+                b1=None, w2=None, b2=None, gate=None, a: float = 1.0, s: float = 1.0, eps: float = 1e-5, dgate=None, dw1=None,
+                db1=None, dw2=None, db2=None):
+    """Gradients of resnorm_fwd from its x, y, weights and stats: dx, dy, and those of dgate (like gate), dw1, db1, dw2, db2 (fp32
+    [c]) that are given.  dr is the gradient of r from elsewhere (None: none), dh that of h (None where second is "none")."""
+    d, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
+    if (second == "none") != (dh is None):
+        raise ValueError("resnorm: dh goes with a second norm")
+    if dr is None and dh is None:
+        raise ValueError("resnorm: no gradient is given")
+    if dgate is not None and gate is None or first == "none" and (dw1 is not None or db1 is not None) \
+            or second == "none" and (dw2 is not None or db2 is not None):
+        raise ValueError("resnorm: a gradient of what the forward does not have")
+    for n, v in (("dr", dr), ("dh", dh), ("dx", dx), ("dy", dy)):
+        if v is not None:
+            p, ld = _row_view(n, v, rows, c, dt, dev)
+            setattr(d, n, p)
+            setattr(d, "ld" + n, ld)
+    if dgate is not None:
+        d.dgate, d.lddg = _row_view("dgate", dgate, d.gates, c, dt, dev)
+    for n, v in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2)):
+        setattr(d, n, _flat(n, v, c, torch.float32, dev))
+    need = _lib.load().dc_resnorm_ws_bytes(d)
+    ws = None
+    if need:   # the call's own, as the attention's
+        ws = torch.empty(need, dtype=torch.uint8, device=ctx.device)
+        d.ws, d.ws_bytes = ws.data_ptr(), need
+    _launch(dev, "dc_resnorm_bwd", d, ctx.stream)
+    return dx, dy
 
 
 def crossattn_tables(ctx: Ctx, U, D, heads, c) -> torch.Tensor:

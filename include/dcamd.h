@@ -498,6 +498,34 @@ int dc_rotary(const void* x, long long ldx, void* y, long long ldy, int type, lo
 int dc_rotary_freqs(int rot, double theta, int scaling, double factor, double trained, double fast, double slow, double* freqs,
                     float* mag);
 
+/* ---------------------------------------------------------------- norms around a block, with gate and residual scale
+ *   u = N1(y), r = a x + s gate u, h = N2(r): x the residual stream, y the block's output, r the stream behind it, h what the next
+ *   block reads (N2 of r before r is rounded).  N: layer (v - mean) rstd w + b, rms v rstd w + b, or none; NULL w: 1, NULL b: 0.
+ * gate: [gates][ldg] in the rows' type, row i under gate row i / (rows / gates): one for all, one a frame, one a row; 0: none.
+ * Forward leaves stats [rows][4] (mean1, rstd1, mean2, rstd2).  Backward takes the forward's x, y, weights and stats and dr, dh (dr
+ * may be NULL) to dx, dy and, where given, dgate (rows' type), dw1, db1, dw2, db2 (fp32 [c]); column sums in a fixed order.
+ * r may be x (where no backward follows) and dx may be dr.  type: 0 bf16, 1 fp16, 2 fp32; c a multiple of 8 up to 8192; pointers of
+ * rows, gate, stats and ws 16-byte aligned, ld* multiples of 8. */
+typedef struct dc_resnorm_desc {
+  int type, c, first, second;   /* norms: 0 none, 1 layer, 2 rms */
+  long long rows, gates;
+  const void *x, *y, *gate;
+  const float *w1, *b1, *w2, *b2;
+  int ldx, ldy, ldg, ldr, ldh;
+  float a, s, eps;
+  void *r, *h;
+  float* stats;
+  const void *dr, *dh;
+  void *dx, *dy, *dgate;
+  float *dw1, *db1, *dw2, *db2;
+  int lddr, lddh, lddx, lddy, lddg;
+  float* ws;                    /* backward: scratch of dc_resnorm_ws_bytes, private to the call until it has run */
+  long long ws_bytes;
+} dc_resnorm_desc;
+int dc_resnorm_fwd(const dc_resnorm_desc* d, void* stream);
+long long dc_resnorm_ws_bytes(const dc_resnorm_desc* d);
+int dc_resnorm_bwd(const dc_resnorm_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
