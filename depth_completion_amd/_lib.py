@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 # DC_LIB overrides the in-tree library (A/B experiments between builds); there is still no fallback
@@ -72,7 +73,16 @@ class AttnDesc(C.Structure):
         ("prefix", vp), ("kv_len", vp), ("doc_q", vp), ("doc_k", vp),
         ("dout", vp), ("dq", vp), ("dk", vp), ("dv", vp),
         ("lddo", i32), ("lddq", i32), ("lddk", i32), ("lddv", i32),
-        ("ws", vp), ("ws_bytes", i64),
+    ]
+
+
+class RotaryDesc(C.Structure):
+    """Mirror of ``dc_rotary_desc``."""
+
+    _fields_ = [
+        ("x", vp), ("y", vp), ("freqs", vp), ("pos", vp), ("ldx", i64), ("ldy", i64), ("rows", i64),
+        ("type", i32), ("heads", i32), ("d", i32), ("off", i32), ("rot", i32), ("pos0", i32), ("t", i32), ("interleaved", i32),
+        ("inverse", i32), ("mag", f32),
     ]
 
 
@@ -87,8 +97,19 @@ class ResnormDesc(C.Structure):
         ("dr", vp), ("dh", vp), ("dx", vp), ("dy", vp), ("dgate", vp),
         ("dw1", vp), ("db1", vp), ("dw2", vp), ("db2", vp),
         ("lddr", i32), ("lddh", i32), ("lddx", i32), ("lddy", i32), ("lddg", i32),
-        ("ws", vp), ("ws_bytes", i64),
     ]
+
+
+def _packer(desc) -> struct.Struct:
+    """The layout of a descriptor as a struct.Struct: pack() of all its fields in order gives the bytes that an entry point reads,
+    in a third of the time that filling the Structure takes (0 for None)."""
+    code = {vp: "P", i32: "i", i64: "q", f32: "f"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in desc._fields_))
+    # C pads a structure to its alignment, struct does not
+    return s if s.size == C.sizeof(desc) else struct.Struct(s.format + f"{C.sizeof(desc) - s.size}x")
+
+
+PACK_ATTN, PACK_ROTARY, PACK_RESNORM = (_packer(d) for d in (AttnDesc, RotaryDesc, ResnormDesc))
 
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
@@ -108,15 +129,16 @@ _SIGS = {
                              vp, i32, vp],
     "dc_layernorm_fwd": [vp, i32, i64, i32, f32, vp, vp, vp, i32, vp, vp],
     "dc_layernorm_bwd": [vp, i32, i64, i32, vp, vp, vp, i32, vp, i32, vp, i32, vp],
-    "dc_resnorm_fwd": [C.POINTER(ResnormDesc), vp],
-    "dc_resnorm_ws_bytes": [C.POINTER(ResnormDesc)],
-    "dc_resnorm_bwd": [C.POINTER(ResnormDesc), vp],
+    "dc_resnorm_fwd": [vp, vp],
+    "dc_resnorm_ws_bytes": [vp],
+    "dc_resnorm_bwd": [vp, vp, i64, vp],
     "dc_attn_fwd": [vp, i32, i32, i32, i32, vp, i32, vp, vp, i64, vp],
     "dc_attn_bwd": [vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, vp, vp, i32, vp, i64, vp],
-    "dc_attn_mask_ws_bytes": [C.POINTER(AttnDesc), i32],
-    "dc_attn_mask_fwd": [C.POINTER(AttnDesc), vp],
-    "dc_attn_mask_bwd": [C.POINTER(AttnDesc), vp],
-    "dc_rotary": [vp, i64, vp, i64, i32, i64, i32, i32, i32, i32, vp, vp, i32, i32, f32, i32, i32, vp],
+    # (descriptors of these: byref of the Structure, or the bytes of its packer)
+    "dc_attn_mask_ws_bytes": [vp, i32],
+    "dc_attn_mask_fwd": [vp, vp, i64, vp],
+    "dc_attn_mask_bwd": [vp, vp, i64, vp],
+    "dc_rotary": [vp, vp],
     "dc_rotary_freqs": [i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp, fp],
     "dc_crossattn_tables_bytes": [i32, i32],
     "dc_crossattn_prepare": [vp, vp, i32, i32, vp, vp],

@@ -511,12 +511,13 @@ extern "C" long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward) 
   return backward ? bwd_ws_bytes(d) : fwd_ws_bytes(d);
 }
 
-extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream) {
+extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* scratch, long long ws_bytes, void* stream) {
   Call c;
   if (const int rc = make_call(d, c, true)) return rc;
-  if (!d->ws || bwd_ws_bytes(d) > d->ws_bytes) return DC_ERR_ARG;
+  if (!scratch || bwd_ws_bytes(d) > ws_bytes) return DC_ERR_ARG;
+  if ((uintptr_t)scratch & 15) return DC_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
-  char* ws = reinterpret_cast<char*>(d->ws);
+  char* ws = static_cast<char*>(scratch);
   launch_summaries(d, c, ws, st);
   ws += summary_bytes(d);
   Back bk;

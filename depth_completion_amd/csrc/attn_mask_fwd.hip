@@ -534,7 +534,7 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   const int hq = d->heads * d->d, hk = d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
   if (d->ldq % 8 || d->ldk % 8 || d->ldv % 8 || d->ldo % 8) return DC_ERR_ALIGN;
-  const uintptr_t at = (uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o | (uintptr_t)d->ws;
+  const uintptr_t at = (uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o;
   if (at & 15) return DC_ERR_ALIGN;
   if (backward) {
     if (!d->dout || !d->dq || !d->dk || !d->dv) return DC_ERR_ARG;
@@ -566,12 +566,13 @@ long long fwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 4LL * 
 
 using namespace dcm;
 
-extern "C" int dc_attn_mask_fwd(const dc_attn_desc* d, void* stream) {
+extern "C" int dc_attn_mask_fwd(const dc_attn_desc* d, void* scratch, long long ws_bytes, void* stream) {
   Call c;
   if (const int rc = make_call(d, c, false)) return rc;
-  if (fwd_ws_bytes(d) > (d->ws ? d->ws_bytes : 0)) return DC_ERR_ARG;
+  if (fwd_ws_bytes(d) > (scratch ? ws_bytes : 0)) return DC_ERR_ARG;
+  if ((uintptr_t)scratch & 15) return DC_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
-  char* ws = reinterpret_cast<char*>(d->ws);
+  char* ws = static_cast<char*>(scratch);
   launch_summaries(d, c, ws, st);
   Split s = split_of(d);
   if (s.n > 1) {

@@ -11,6 +11,7 @@
 // kept in registers over a block's rows, left as one row of partial sums a block, and added by a second kernel in block order.
 #include "common.h"
 #include "../../include/dcamd.h"
+#include <type_traits>
 
 namespace {
 
@@ -29,10 +30,14 @@ struct Desc {
   float *part, *gpart;   // [blocks][4][c] of dw1, db1, dw2, db2; [blocks][c] of dgate where chunks > 1
 };
 
+// Rows are read at a place that is valid in every lane (`at` of lanes behind the row's end is 0), so that no load waits behind a
+// branch, and become zeros there when they are widened.
 template <typename T>
-__device__ __forceinline__ void get8(const T* p, bool ok, float* f) {
-  Row8<T> v;
-  if (ok) v = *reinterpret_cast<const Row8<T>*>(p);
+__device__ __forceinline__ Row8<T> raw8(const void* p, long row, int ld, int at) {
+  return *reinterpret_cast<const Row8<T>*>((const T*)p + row * ld + at);
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Row8<T>& v, bool ok, float* f) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = ok ? (float)v.v[i] : 0.0f;
 }
@@ -43,18 +48,39 @@ __device__ __forceinline__ void put8(T* p, bool ok, const float* f) {
   for (int i = 0; i < 8; ++i) v.v[i] = (T)f[i];
   if (ok) *reinterpret_cast<Row8<T>*>(p) = v;
 }
-__device__ __forceinline__ void get_w(const float* w, int at, bool ok, float none, float* f) {
+// a lane's eight weights (`from`: a place that is valid in every lane)
+__device__ __forceinline__ void get_w(const float* w, int from, float none, float* f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = w && ok ? w[at + i] : none;
+  for (int i = 0; i < 8; ++i) f[i] = none;
+  if (w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = w[from + i];
+  }
 }
 __device__ __forceinline__ float sum8(const float* f) {
   return ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
 }
 
+// Sum over a wave, in every lane, by cross-lane moves (wave_sum's shuffles pass through LDS: six round trips a
+// sum).
+__device__ __forceinline__ float lanes_sum(float v) {
+  auto moved = [](float x, auto ctrl) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v += moved(v, std::integral_constant<int, 0xb1>{});    // lane ^ 1
+  v += moved(v, std::integral_constant<int, 0x4e>{});    // lane ^ 2
+  v += moved(v, std::integral_constant<int, 0x141>{});   // the other four of eight
+  v += moved(v, std::integral_constant<int, 0x140>{});   // the other eight of sixteen
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Sum over the waves of a row; `red` has a slot of WPR floats for each of two calls in turn, so that one barrier a call is enough.
 template <int WPR>
 __device__ __forceinline__ float row_sum(float v, float (*red)[16], int& turn) {
-  v = wave_sum(v);
+  v = lanes_sum(v);
   if constexpr (WPR == 1) return v;
   else {
     if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
@@ -83,25 +109,32 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void fwd_kernel(Desc p) 
   constexpr int RP = WPR == 1 ? 4 : 1;   // rows at a time
   __shared__ float red[2][16];
   const dc_resnorm_desc& d = p.d;
-  const int slot = WPR == 1 ? threadIdx.x >> 6 : 0, at = (WPR == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
+  const int slot = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, at = (WPR == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
   const bool in = at < d.c;
+  const int from = in ? at : 0;
   const float inv_c = 1.0f / d.c;
   float w1[8], b1[8], w2[8], b2[8], g[8];
-  get_w(d.w1, at, in, 1.0f, w1);
-  get_w(d.b1, at, in, 0.0f, b1);
-  get_w(d.w2, at, in, 1.0f, w2);
-  get_w(d.b2, at, in, 0.0f, b2);
+  get_w(d.w1, from, 1.0f, w1);
+  get_w(d.b1, from, 0.0f, b1);
+  get_w(d.w2, from, 1.0f, w2);
+  get_w(d.b2, from, 0.0f, b2);
   int turn = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) g[i] = 1.0f;
   long have = -1;
-  for (long row = (long)blockIdx.x * RP + slot; row < d.rows; row += (long)gridDim.x * RP) {
+  long row = (long)blockIdx.x * RP + slot;
+  if (row >= d.rows) return;   // (a row's waves together)
+  Row8<T> xr = raw8<T>(d.x, row, d.ldx, from), yr = raw8<T>(d.y, row, d.ldy, from);
+  for (; row < d.rows; row += (long)gridDim.x * RP) {
     float x[8], y[8];
-    get8((const T*)d.x + row * d.ldx + at, in, x);
-    get8((const T*)d.y + row * d.ldy + at, in, y);
+    widen(xr, in, x);
+    widen(yr, in, y);
+    const long next = min(row + (long)gridDim.x * RP, d.rows - 1);   // on its way while this row is computed
+    xr = raw8<T>(d.x, next, d.ldx, from);
+    yr = raw8<T>(d.y, next, d.ldy, from);
     if (p.per_gate && row / p.per_gate != have) {
       have = row / p.per_gate;
-      get8((const T*)d.gate + have * d.ldg + at, in, g);
+      widen(raw8<T>(d.gate, have, d.ldg, from), in, g);
     }
     float m1 = 0.0f, k1 = 1.0f, m2 = 0.0f, k2 = 1.0f;
     if (d.first != NONE) stats_of<WPR>(y, in, d.first, inv_c, d.eps, red, turn, m1, k1);
@@ -140,81 +173,107 @@ __device__ __forceinline__ void leave(const float* f, int at, int slot, bool in,
   put8(out + at, in, v);
 }
 
-template <typename T, int WPR>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void bwd_kernel(Desc p) {
+// OFFS: there is an offset b1, or a gradient of an offset is wanted (24 registers of sums that a call without them does not carry).
+template <typename T, int WPR, bool OFFS>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR, WPR == 16 ? 4 : WPR == 8 ? 2 : 3) void bwd_kernel(Desc p) {
   constexpr int RP = WPR == 1 ? 4 : 1;
   __shared__ float red[2][16];
   __shared__ float cols[RP == 1 ? 1 : RP * 512];
   const dc_resnorm_desc& d = p.d;
-  const int slot = WPR == 1 ? threadIdx.x >> 6 : 0, at = (WPR == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
+  const int slot = WPR == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, at = (WPR == 1 ? threadIdx.x & 63 : threadIdx.x) * 8;
   const bool in = at < d.c;
+  const int from = in ? at : 0;
   const float inv_c = 1.0f / d.c;
+  // the 16 waves of the widest rows have 128 registers each: their weights wait in LDS, each lane's own
+  constexpr bool LDS_W = WPR == 16;
+  __shared__ __attribute__((aligned(16))) float lds_w[LDS_W ? 3 * 8192 : 1];
   float w1[8], b1[8], w2[8], g[8];
-  get_w(d.w1, at, in, 1.0f, w1);
-  get_w(d.b1, at, in, 0.0f, b1);
-  get_w(d.w2, at, in, 1.0f, w2);
+  get_w(d.w1, from, 1.0f, w1);
+  get_w(OFFS ? d.b1 : nullptr, from, 0.0f, b1);
+  get_w(d.w2, from, 1.0f, w2);
+  if constexpr (LDS_W)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lds_w[at + i] = w1[i];
+      lds_w[8192 + at + i] = w2[i];
+      if (OFFS) lds_w[16384 + at + i] = b1[i];
+    }
+  auto w1_of = [&](int i) __attribute__((always_inline)) { return LDS_W ? lds_w[at + i] : w1[i]; };
+  auto w2_of = [&](int i) __attribute__((always_inline)) { return LDS_W ? lds_w[8192 + at + i] : w2[i]; };
+  auto b1_of = [&](int i) __attribute__((always_inline)) { return !OFFS ? 0.0f : LDS_W ? lds_w[16384 + at + i] : b1[i]; };
   int turn = 0;
   float s1[8] = {}, t1[8] = {}, s2[8] = {}, t2[8] = {}, sg[8] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) g[i] = 1.0f;
+  Row8<T> xr, yr, rr = {}, hr = {};
+  float4 str;
+  auto fetch = [&](long row) __attribute__((always_inline)) {
+    xr = raw8<T>(d.x, row, d.ldx, from);
+    yr = raw8<T>(d.y, row, d.ldy, from);
+    str = *reinterpret_cast<const float4*>(d.stats + row * 4);
+    if (d.dr) rr = raw8<T>(d.dr, row, d.lddr, from);
+    if (d.second != NONE) hr = raw8<T>(d.dh, row, d.lddh, from);
+  };
   // chunks > 0: rows row0 .. of one gate row, dealt to the block's slots; else whole gate rows to a slot
   const long gate0 = p.chunks ? blockIdx.x / p.chunks : (long)blockIdx.x * p.gates + slot;
   const long gate1 = p.chunks ? gate0 + 1 : min((long)(blockIdx.x + 1) * p.gates, p.per_gate ? d.rows / p.per_gate : 1L);
   const long per = p.per_gate ? p.per_gate : d.rows;
   for (long gi = gate0; gi < gate1; gi += p.chunks ? 1 : RP) {
-    if (p.per_gate) get8((const T*)d.gate + gi * d.ldg + at, in, g);
+    if (p.per_gate) widen(raw8<T>(d.gate, gi, d.ldg, from), in, g);
     const long row0 = gi * per + (p.chunks ? blockIdx.x % p.chunks * p.chunk + slot : 0);
     const long row1 = min((gi + 1) * per, p.chunks ? gi * per + (blockIdx.x % p.chunks + 1) * p.chunk : d.rows);
+    if (row0 < row1) fetch(row0);
     for (long row = row0; row < row1; row += p.chunks ? RP : 1) {
-      float x[8], y[8], n1[8], n2[8], gr[8], gh[8];
-      get8((const T*)d.x + row * d.ldx + at, in, x);
-      get8((const T*)d.y + row * d.ldy + at, in, y);
-      const float4 st = *reinterpret_cast<const float4*>(d.stats + row * 4);
-      if (d.dr) get8((const T*)d.dr + row * d.lddr + at, in, gr);
-      else
+      if constexpr (LDS_W) asm volatile("" ::: "memory");   // read them anew for each row
+      // u = n1 w1 + b1 is formed where it is used (a norm that is none: n1 = y, 1 and 0)
+      float x[8], n1[8], gr[8];
+      const float4 st = str;
+      widen(xr, in, x);
+      widen(yr, in, n1);
+      widen(rr, in && d.dr, gr);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) gr[i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n1[i] = in ? (y[i] - st.x) * st.y : 0.0f;
-        y[i] = d.first != NONE ? n1[i] * w1[i] + b1[i] : y[i];   // u
-      }
+      for (int i = 0; i < 8; ++i) n1[i] = in ? (n1[i] - st.x) * st.y : 0.0f;
       if (d.second != NONE) {
-        get8((const T*)d.dh + row * d.lddh + at, in, gh);
-        float c1 = 0.0f, q[8];
+        float gh[8];
+        widen(hr, in, gh);
+        fetch(min(row + (p.chunks ? RP : 1), row1 - 1));   // on its way while this row is computed
+        float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          n2[i] = in ? (d.a * x[i] + d.s * (g[i] * y[i]) - st.z) * st.w : 0.0f;
-          s2[i] += gh[i] * n2[i];
-          t2[i] += gh[i];
-          gh[i] *= w2[i];
-          q[i] = gh[i] * n2[i];
+          x[i] = in ? (d.a * x[i] + d.s * (g[i] * (n1[i] * w1_of(i) + b1_of(i))) - st.z) * st.w : 0.0f;   // n2
+          s2[i] += gh[i] * x[i];
+          if constexpr (OFFS) t2[i] += gh[i];
+          gh[i] *= w2_of(i);
+          c1 += gh[i];
+          c2 += gh[i] * x[i];
         }
-        const float c2 = row_sum<WPR>(sum8(q), red, turn) * inv_c;
-        if (d.second == LAYER) c1 = row_sum<WPR>(sum8(gh), red, turn) * inv_c;
+        c2 = row_sum<WPR>(c2, red, turn) * inv_c;
+        c1 = d.second == LAYER ? row_sum<WPR>(c1, red, turn) * inv_c : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) gr[i] += st.w * (gh[i] - c1 - n2[i] * c2);
+        for (int i = 0; i < 8; ++i) gr[i] += st.w * (gh[i] - c1 - x[i] * c2);
+      } else {
+        fetch(min(row + (p.chunks ? RP : 1), row1 - 1));
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = d.a * gr[i];
       put8((T*)d.dx + row * d.lddx + at, in, x);
+      float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         gr[i] *= d.s;
-        sg[i] += gr[i] * y[i];
+        sg[i] += gr[i] * (n1[i] * w1_of(i) + b1_of(i));
         gr[i] *= g[i];
         s1[i] += gr[i] * n1[i];
-        t1[i] += gr[i];
+        if constexpr (OFFS) t1[i] += gr[i];
+        if (d.first != NONE) {
+          gr[i] = in ? gr[i] * w1_of(i) : 0.0f;
+          c1 += gr[i];
+          c2 += gr[i] * n1[i];
+        }
       }
       if (d.first != NONE) {
-        float c1 = 0.0f, q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          gr[i] = in ? gr[i] * w1[i] : 0.0f;
-          q[i] = gr[i] * n1[i];
-        }
-        const float c2 = row_sum<WPR>(sum8(q), red, turn) * inv_c;
-        if (d.first == LAYER) c1 = row_sum<WPR>(sum8(gr), red, turn) * inv_c;
+        c2 = row_sum<WPR>(c2, red, turn) * inv_c;
+        c1 = d.first == LAYER ? row_sum<WPR>(c1, red, turn) * inv_c : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) gr[i] = st.y * (gr[i] - c1 - n1[i] * c2);
       }
@@ -228,67 +287,71 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void bwd_kernel(Desc p) 
   }
   float* part = p.part + (long)blockIdx.x * 4 * d.c;
   if (d.dw1) leave<RP>(s1, at, slot, in, cols, part);
-  if (d.db1) leave<RP>(t1, at, slot, in, cols, part + d.c);
+  if (OFFS && d.db1) leave<RP>(t1, at, slot, in, cols, part + d.c);
   if (d.dw2) leave<RP>(s2, at, slot, in, cols, part + 2 * d.c);
-  if (d.db2) leave<RP>(t2, at, slot, in, cols, part + 3 * d.c);
+  if (OFFS && d.db2) leave<RP>(t2, at, slot, in, cols, part + 3 * d.c);
   if (p.chunks && d.dgate) {
     if (p.chunks == 1) leave<RP>(sg, at, slot, in, cols, (T*)d.dgate + gate0 * d.lddg);
     else leave<RP>(sg, at, slot, in, cols, p.gpart + (long)blockIdx.x * d.c);
   }
 }
 
-// 64 columns of one sum to a block: 4 waves take a quarter of the partial rows each, in order.
+// 64 columns of one sum to a block: its 16 waves take a run of the partial rows each, and are added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void fold_kernel(Desc p) {
-  __shared__ float red[4][64];
+__global__ __launch_bounds__(1024) void fold_kernel(Desc p) {
+  __shared__ float red[16][64];
   const dc_resnorm_desc& d = p.d;
   const int which = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int col = blockIdx.x * 64 + lane;
-  float* const outs[4] = {d.dw1, d.db1, d.dw2, d.db2};
-  const float* src;
+  float* const out = which == 0 ? d.dw1 : which == 1 ? d.db1 : which == 2 ? d.dw2 : d.db2;
+  const float* src = p.part + (long)which * d.c;
   int n = p.blocks;
   long stride = 4L * d.c;
-  if (which < 4) {
-    if (!outs[which]) return;
-    src = p.part + (long)which * d.c;
-  } else {   // a gate row's chunks
+  if (which >= 4) {   // a gate row's chunks
     n = p.chunks;
     stride = d.c;
     src = p.gpart + (long)(which - 4) * n * d.c;
+  } else if (!out) {
+    return;
   }
-  const int each = (n + 3) / 4, i0 = w * each, i1 = min(n, i0 + each);
-  float s[4] = {};
+  const int each = (n + 15) / 16, i0 = w * each, i1 = min(n, i0 + each);
+  float s[8] = {};
   if (col < d.c) {
+    src += col;
     int i = i0;
-    for (; i + 4 <= i1; i += 4)
+    for (; i + 8 <= i1; i += 8)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] += src[(i + k) * stride + col];
-    for (; i < i1; ++i) s[0] += src[i * stride + col];
+      for (int k = 0; k < 8; ++k) s[k] += src[(i + k) * stride];
+    for (; i < i1; ++i) s[0] += src[i * stride];
   }
-  red[w][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+  red[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   if (w > 0 || col >= d.c) return;
-  const float v = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-  if (which < 4) outs[which][col] = v;
+  float v = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v += red[k][lane];
+  if (which < 4) out[col] = v;
   else ((T*)d.dgate)[(long)(which - 4) * d.lddg + col] = (T)v;
 }
 
-constexpr int kBlocks = 512;   // backward blocks that leave partial sums: two of the largest to a CU
+// Backward blocks that leave partial sums: as many as the card holds at once (12 waves to a CU, of the 16-wave blocks one).
+int most_blocks(int c) { return c <= 512 ? 768 : c <= 1024 ? 1536 : c <= 2048 ? 768 : 256; }
 
 void plan(const dc_resnorm_desc* d, Desc& p) {
   p.d = *d;
   p.per_gate = d->gates > 0 ? d->rows / d->gates : 0;
   const long gates = d->gates > 0 ? d->gates : 1, per = d->rows / gates;
   const int rp = d->c <= 512 ? 4 : 1;
+  const int most = most_blocks(d->c);
   p.gates = 0;
   p.chunks = 0;
-  if (gates <= kBlocks) {
-    p.chunks = (int)max(1L, min(kBlocks / gates, (per + rp - 1) / rp));
+  if (gates <= most) {
+    p.chunks = (int)max(1L, min(most / gates, (per + rp - 1) / rp));
     p.chunk = (per + p.chunks - 1) / p.chunks;
     p.chunks = (int)((per + p.chunk - 1) / p.chunk);
     p.blocks = (int)(gates * p.chunks);
   } else {
-    p.gates = (int)((gates + kBlocks - 1) / kBlocks);
+    p.gates = (int)((gates + most - 1) / most);
     p.gates = (p.gates + rp - 1) / rp * rp;
     p.blocks = (int)((gates + p.gates - 1) / p.gates);
   }
@@ -309,7 +372,7 @@ int check(const dc_resnorm_desc* d, bool backward) {
   if (!(d->eps >= 0.0f)) return DC_ERR_ARG;
   const int c = d->c;
   if (d->ldx < c || d->ldy < c || (d->gate && d->ldg < c)) return DC_ERR_ARG;
-  uintptr_t at = (uintptr_t)d->x | (uintptr_t)d->y | (uintptr_t)d->gate | (uintptr_t)d->stats | (uintptr_t)d->ws;
+  uintptr_t at = (uintptr_t)d->x | (uintptr_t)d->y | (uintptr_t)d->gate | (uintptr_t)d->stats;
   int ld = d->ldx | d->ldy | (d->gate ? d->ldg : 0);
   const uintptr_t words = (uintptr_t)d->w1 | (uintptr_t)d->b1 | (uintptr_t)d->w2 | (uintptr_t)d->b2 | (uintptr_t)d->dw1 |
                           (uintptr_t)d->db1 | (uintptr_t)d->dw2 | (uintptr_t)d->db2;
@@ -336,7 +399,9 @@ void forward(const Desc& p, hipStream_t st) {
 }
 template <typename T, int W>
 void backward(const Desc& p, hipStream_t st) {
-  hipLaunchKernelGGL((bwd_kernel<T, W>), dim3((unsigned)p.blocks), dim3(W == 1 ? 256 : 64 * W), 0, st, p);
+  const dim3 grid((unsigned)p.blocks), block(W == 1 ? 256 : 64 * W);
+  if (p.d.b1 || p.d.db1 || p.d.db2) hipLaunchKernelGGL((bwd_kernel<T, W, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((bwd_kernel<T, W, false>), grid, block, 0, st, p);
 }
 
 // 8 columns to a lane: a row takes as many waves as that needs
@@ -350,8 +415,8 @@ void launch(const Desc& p, bool back, hipStream_t st) {
   else back ? backward<T, 16>(p, st) : forward<T, 16>(p, st);
   const bool gate = p.d.dgate && p.chunks > 1;
   if (back && (part_floats(p) || gate))
-    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)((c + 63) / 64), (unsigned)(4 + (gate ? p.d.gates : 0))), dim3(256), 0, st,
-                       p);
+    hipLaunchKernelGGL((fold_kernel<T>), dim3((unsigned)((c + 63) / 64), (unsigned)(4 + (gate ? p.d.gates : 0))), dim3(1024), 0,
+                       st, p);
 }
 void launch(const Desc& p, bool back, hipStream_t st) {
   if (p.d.type == 0) launch<bf16>(p, back, st);
@@ -378,13 +443,14 @@ extern "C" long long dc_resnorm_ws_bytes(const dc_resnorm_desc* d) {
   return ws_of(p);
 }
 
-extern "C" int dc_resnorm_bwd(const dc_resnorm_desc* d, void* stream) {
+extern "C" int dc_resnorm_bwd(const dc_resnorm_desc* d, void* ws, long long ws_bytes, void* stream) {
   if (const int rc = check(d, true)) return rc;
   Desc p{};
   plan(d, p);
-  if (ws_of(p) > (d->ws ? d->ws_bytes : 0)) return DC_ERR_ARG;
-  p.part = d->ws;
-  p.gpart = d->ws + part_floats(p);
+  if (ws_of(p) > (ws ? ws_bytes : 0)) return DC_ERR_ARG;
+  if ((uintptr_t)ws & 15) return DC_ERR_ALIGN;
+  p.part = static_cast<float*>(ws);
+  p.gpart = p.part + part_floats(p);
   hipStream_t st = (hipStream_t)stream;
   launch(p, true, st);
   DC_CHECK_LAUNCH();

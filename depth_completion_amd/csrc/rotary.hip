@@ -40,7 +40,8 @@ struct Rotary {
   int inverse, hpt, nturn, units;   // heads to a thread; of a head's units, those that turn
 };
 
-// A unit: V pairs (two packs of V columns), or two packs of V columns that are copied.
+// A unit: V pairs (two packs of V columns), or two packs that are copied (the last of an odd count twice).  Both run the same loads
+// and stores, the copied ones keep their bits by a select, so a wave whose lanes lie over a whole head stays together.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(Rotary p) {
   typedef Pack<T, V> P;
@@ -49,58 +50,69 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotary p) {
   const int u = (int)(i - row * p.units);
   const int h0 = blockIdx.y * p.hpt, h1 = min(p.heads, h0 + p.hpt);
   if (row >= p.rows) return;
-  const T* x = (const T*)p.x + row * p.ldx;
-  T* y = (T*)p.y + row * p.ldy;
-  if (u >= p.nturn) {
+  const bool turns = u < p.nturn;
+  int at[2];
+  float s[V], c[V];
+  if (turns) {
+    at[0] = INTER ? p.off + u * 2 * V : p.off + u * V;
+    at[1] = INTER ? at[0] + V : at[0] + p.rot / 2;
+    const double pos = p.pos ? (double)p.pos[row] : (double)p.pos0 + (double)(row % p.t);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      sin_cos<T>(pos, p.freqs[u * V + k], s[k], c[k]);
+      s[k] *= p.inverse ? -p.mag : p.mag;
+      c[k] *= p.mag;
+    }
+  } else {
     const int rest = (p.d - p.rot) / V;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int j = 2 * (u - p.nturn) + k;
-      if (j >= rest) break;
-      const int at = j * V < p.off ? j * V : j * V + p.rot;
-      for (int h = h0; h < h1; ++h) *reinterpret_cast<P*>(y + h * p.d + at) = *reinterpret_cast<const P*>(x + h * p.d + at);
+      const int j = min(2 * (u - p.nturn) + k, rest - 1) * V;
+      at[k] = j < p.off ? j : j + p.rot;
     }
-    return;
-  }
-  const double pos = p.pos ? (double)p.pos[row] : (double)p.pos0 + (double)(row % p.t);
-  const int a0 = INTER ? p.off + u * 2 * V : p.off + u * V, b0 = INTER ? a0 + V : a0 + p.rot / 2;
-  float s[V], c[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    sin_cos<T>(pos, p.freqs[u * V + k], s[k], c[k]);
-    s[k] *= p.inverse ? -p.mag : p.mag;
-    c[k] *= p.mag;
+    for (int k = 0; k < V; ++k) s[k] = c[k] = 0.0f;
   }
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    const P a = *reinterpret_cast<const P*>(x + h * p.d + a0), b = *reinterpret_cast<const P*>(x + h * p.d + b0);
-    P ya, yb;
+  const T* x = (const T*)p.x + row * p.ldx + (long)h0 * p.d;
+  T* y = (T*)p.y + row * p.ldy + (long)h0 * p.d;
+  auto turn = [&](const P& a, const P& b, T* to) __attribute__((always_inline)) {
+    P r[2] = {a, b};
+    if (turns) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      // element 2 k and 2 k + 1 of the 2 V columns, or k of either half
-      const float e = (float)(!INTER ? a.v[k] : 2 * k < V ? a.v[2 * k % V] : b.v[2 * k % V]);
-      const float f = (float)(!INTER ? b.v[k] : 2 * k + 1 < V ? a.v[(2 * k + 1) % V] : b.v[(2 * k + 1) % V]);
-      const T r0 = (T)(e * c[k] - f * s[k]), r1 = (T)(e * s[k] + f * c[k]);
-      if constexpr (!INTER) {
-        ya.v[k] = r0;
-        yb.v[k] = r1;
-      } else {
-        (2 * k < V ? ya.v[2 * k % V] : yb.v[2 * k % V]) = r0;
-        (2 * k + 1 < V ? ya.v[(2 * k + 1) % V] : yb.v[(2 * k + 1) % V]) = r1;
+      for (int k = 0; k < V; ++k) {
+        // elements 2 k and 2 k + 1 of the 2 V columns, or k of either half
+        const int n0 = INTER ? 2 * k / V : 0, n1 = INTER ? (2 * k + 1) / V : 1;
+        const int e0 = INTER ? 2 * k % V : k, e1 = INTER ? (2 * k + 1) % V : k;
+        const float e = (float)(n0 ? b : a).v[e0], f = (float)(n1 ? b : a).v[e1];
+        r[n0].v[e0] = (T)(e * c[k] - f * s[k]);
+        r[n1].v[e1] = (T)(e * s[k] + f * c[k]);
       }
     }
-    *reinterpret_cast<P*>(y + h * p.d + a0) = ya;
-    *reinterpret_cast<P*>(y + h * p.d + b0) = yb;
+    *reinterpret_cast<P*>(to + at[0]) = r[0];
+    *reinterpret_cast<P*>(to + at[1]) = r[1];
+  };
+  int h = h0;
+  for (; h + 4 <= h1; h += 4, x += 4 * p.d, y += 4 * p.d) {   // four heads' reads before the first is used
+    P a[4], b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = *reinterpret_cast<const P*>(x + k * p.d + at[0]);
+      b[k] = *reinterpret_cast<const P*>(x + k * p.d + at[1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) turn(a[k], b[k], y + k * p.d);
   }
+  for (; h < h1; ++h, x += p.d, y += p.d)
+    turn(*reinterpret_cast<const P*>(x + at[0]), *reinterpret_cast<const P*>(x + at[1]), y);
 }
 
 template <typename T, int V>
 void launch(Rotary p, int interleaved, hipStream_t st) {
   p.nturn = p.rot / (2 * V);
   p.units = p.nturn + (p.x == p.y ? 0 : ((p.d - p.rot) / V + 1) / 2);
-  // as many heads to a thread as leave 2^18 threads, four to a lane of the card
+  // enough threads to fill the card (2^19) come before heads that share their sines; past 8 heads these cost nothing
   const long all = p.rows * p.units * p.heads;
-  p.hpt = (int)min((long)p.heads, max(1L, all >> 18));
+  p.hpt = (int)min((long)min(p.heads, 8), max(1L, all >> 19));
   const dim3 grid((unsigned)((p.rows * p.units + 255) / 256), (unsigned)((p.heads + p.hpt - 1) / p.hpt));
   if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, V, true>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((rotary_kernel<T, V, false>), grid, dim3(256), 0, st, p);
@@ -118,21 +130,21 @@ void launch_type(const Rotary& p, int interleaved, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int dc_rotary(const void* x, long long ldx, void* y, long long ldy, int type, long long rows, int heads, int d, int off,
-                         int rot, const double* freqs, const int* pos, int pos0, int t, float mag, int interleaved, int inverse,
-                         void* stream) {
-  if (!x || !y || !freqs || type < 0 || type > 2 || rows <= 0 || heads <= 0 || d <= 0) return DC_ERR_ARG;
-  if (rot <= 0 || rot % 2 || off < 0 || off > d || rot > d - off || d > 65536 || heads > 65535) return DC_ERR_ARG;
-  if ((long long)heads * d >= (1LL << 31) || (x == y && ldx != ldy)) return DC_ERR_ARG;
-  if (ldx < (long long)heads * d || ldy < (long long)heads * d || (!pos && t <= 0) || rows > (1LL << 40) / d) return DC_ERR_ARG;
-  const uintptr_t size = type == 2 ? 4 : 2;
-  if ((((uintptr_t)x | (uintptr_t)y) & (size - 1)) || ((uintptr_t)freqs & 7) || ((uintptr_t)pos & 3)) return DC_ERR_ALIGN;
-  if ((rows * d + 255) / 256 >= (1LL << 31)) return DC_ERR_ARG;
-  Rotary p{x, y, (long)ldx, (long)ldy, (long)rows, heads, d, off, rot, freqs, pos, pos0, t, mag, inverse, 0, 0, 0};
+extern "C" int dc_rotary(const dc_rotary_desc* r, void* stream) {
+  if (!r || !r->x || !r->y || !r->freqs || r->type < 0 || r->type > 2 || r->rows <= 0 || r->heads <= 0 || r->d <= 0) return DC_ERR_ARG;
+  const int d = r->d, heads = r->heads;
+  if (r->rot <= 0 || r->rot % 2 || r->off < 0 || r->off > d || r->rot > d - r->off || d > 65536 || heads > 65535) return DC_ERR_ARG;
+  if ((long long)heads * d >= (1LL << 31) || (r->x == r->y && r->ldx != r->ldy)) return DC_ERR_ARG;
+  if (r->ldx < (long long)heads * d || r->ldy < (long long)heads * d || (!r->pos && r->t <= 0)) return DC_ERR_ARG;
+  if (r->rows > (1LL << 38) / d) return DC_ERR_ARG;   // the grid's blocks of 256 units
+  const uintptr_t size = r->type == 2 ? 4 : 2;
+  if ((((uintptr_t)r->x | (uintptr_t)r->y) & (size - 1)) || ((uintptr_t)r->freqs & 7) || ((uintptr_t)r->pos & 3)) return DC_ERR_ALIGN;
+  Rotary p{r->x, r->y, (long)r->ldx, (long)r->ldy, (long)r->rows, heads, d, r->off, r->rot, r->freqs, r->pos, r->pos0, r->t, r->mag,
+           r->inverse, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
-  if (type == 0) launch_type<bf16>(p, interleaved, st);
-  else if (type == 1) launch_type<half>(p, interleaved, st);
-  else launch_type<float>(p, interleaved, st);
+  if (r->type == 0) launch_type<bf16>(p, r->interleaved, st);
+  else if (r->type == 1) launch_type<half>(p, r->interleaved, st);
+  else launch_type<float>(p, r->interleaved, st);
   DC_CHECK_LAUNCH();
   return DC_OK;
 }

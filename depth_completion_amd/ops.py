@@ -16,7 +16,7 @@ from pathlib import Path
 import torch
 
 from . import _lib
-from ._lib import AttnDesc, ConvDesc, GnFuse, LnFuse, ResnormDesc, call
+from ._lib import PACK_ATTN, PACK_RESNORM, PACK_ROTARY, ConvDesc, GnFuse, LnFuse, call
 
 BF16 = torch.bfloat16
 
@@ -444,31 +444,41 @@ def _row_view(name: str, t, rows: int, cols: int, dtype, dev: int) -> tuple:
     col = 0
     if isinstance(t, Slice):
         t, col = t.t, t.col
-    if t.dtype is not dtype:
-        raise ValueError(f"{name}: {t.dtype}, expected {dtype}")
-    if t.dim() != 2 or t.shape[0] < rows or col < 0 or t.shape[1] - col < cols or (t.stride(1) != 1 and cols > 1):
-        raise ValueError(f"{name}: needs {rows} rows of {cols} contiguous columns, got {tuple(t.shape)} from column {col}")
-    if t.get_device() != dev:
-        raise ValueError(f"{name}: on {t.device}, the context is on device {dev}")
-    return t.data_ptr() + col * t.element_size(), t.stride(0) if t.shape[0] > 1 else -(-cols // 8) * 8
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or len(shape) != 2 or shape[0] < rows or col < 0 or shape[1] - col < cols \
+            or (stride[1] != 1 and cols > 1) or t.get_device() != dev:
+        raise ValueError(f"{name}: needs {rows} rows of {cols} contiguous columns of {dtype} on device {dev}, "
+                         f"got {tuple(shape)} from column {col} of {t.dtype} on {t.device}")
+    return t.data_ptr() + col * t.element_size(), stride[0] if shape[0] > 1 else -(-cols // 8) * 8
 
 
-def _flat(name: str, t, n: int, dtype, dev: int) -> int | None:
-    """Pointer of a contiguous operand of at least ``n`` values of ``dtype`` on device ``dev`` (None stays None)."""
+def _flat(name: str, t, n: int, dtype, dev: int) -> int:
+    """Pointer of a contiguous operand of at least ``n`` values of ``dtype`` on device ``dev`` (0 for None)."""
     if t is None:
-        return None
+        return 0
     if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
         raise ValueError(f"{name}: needs {n} contiguous {dtype} on device {dev}, got {t.numel()} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
 def _launch(dev: int, name: str, *args):
-    """call() with ``dev`` as the current device, where a kernel launch has to find its stream."""
+    """An entry point on the current stream of ``dev``, which has to be the current device while a kernel is launched."""
+    f = getattr(_lib.load(), name)
     if torch.cuda.current_device() == dev:
-        call(name, *args)
+        status = f(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args)
+            status = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    _lib.check(status, name)
+
+
+def _scratch(need: int, dev: int) -> tuple:
+    """(tensor, pointer) of a call's own scratch.  The allocator hands it on in stream order and a capture takes it from the
+    graph's pool, so calls on other streams and graphs that replay beside each other share nothing."""
+    if not need:
+        return None, 0
+    t = torch.empty(need, dtype=torch.uint8, device=dev)
+    return t, t.data_ptr()
 
 
 def _device_of(ctx: Ctx) -> int:
@@ -477,18 +487,22 @@ def _device_of(ctx: Ctx) -> int:
     return ctx.device.index if ctx.device.index is not None else torch.cuda.current_device()
 
 
+NO_GRADIENTS = (0,) * 8
+
+
 def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, scale, softcap, slopes, causal, prefix, kv_len,
                doc_q, doc_k):
     if min(nb, tq, tk, heads, kv_heads, d) <= 0 or heads % kv_heads or d % 8 or d > 128:
         raise ValueError(f"attn_mask: nb {nb}, tq {tq}, tk {tk}, {heads} heads over {kv_heads}, d {d} "
                          "(positive; whole groups of heads; d a multiple of 8 up to 128)")
-    base = q.t if isinstance(q, Slice) else q
-    dt = base.dtype
-    if TYPE_IDS.get(dt, 2) > 1:
+    dt = (q.t if isinstance(q, Slice) else q).dtype
+    kind = TYPE_IDS.get(dt, 2)
+    if kind > 1:
         raise ValueError(f"attn_mask: {dt} (bfloat16 or float16)")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 1e30 or not 0.0 <= softcap <= 1e30 or softcap and scale > 1e30 * softcap:
-        raise ValueError(f"attn_mask: scale {scale}, softcap {softcap} (scale above 0, softcap 0 for none, both and scale / softcap at most 1e30)")
+        raise ValueError(f"attn_mask: scale {scale}, softcap {softcap} "
+                         "(scale above 0, softcap 0 for none, both and scale / softcap at most 1e30)")
     if prefix is not None and not causal:
         raise ValueError("attn_mask: a prefix opens a causal mask; without causal every key is seen already")
     if (doc_q is None) != (doc_k is None):
@@ -498,25 +512,19 @@ def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, 
     pk, ldk = _row_view("k", k, nk, hk, dt, dev)
     pv, ldv = _row_view("v", v, nk, hk, dt, dev)
     po, ldo = _row_view("o", o, nq, hq, dt, dev)
-    i4 = torch.int32
-    desc = AttnDesc(TYPE_IDS[dt], nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po,
-                    _flat("lse", lse, nb * heads * tq, torch.float32, dev), ldq, ldk, ldv, ldo, scale, softcap,
-                    _flat("slopes", slopes, heads, torch.float32, dev), bool(causal), _flat("prefix", prefix, nb, i4, dev),
-                    _flat("kv_len", kv_len, nb, i4, dev), _flat("doc_q", doc_q, nq, i4, dev),
-                    _flat("doc_k", doc_k, nk, i4, dev))
+    i4, f4 = torch.int32, torch.float32
+    grads = NO_GRADIENTS
     if back is not None:
-        desc.dout, desc.lddo = _row_view("dout", back[0], nq, hq, dt, dev)
-        desc.dq, desc.lddq = _row_view("dq", back[1], nq, hq, dt, dev)
-        desc.dk, desc.lddk = _row_view("dk", back[2], nk, hk, dt, dev)
-        desc.dv, desc.lddv = _row_view("dv", back[3], nk, hk, dt, dev)
-    # scratch of the call's own (the allocator hands it on in stream order, a capture takes it from the graph's pool), so calls on
-    # other streams and graphs that replay beside each other share nothing
-    need = _lib.load().dc_attn_mask_ws_bytes(desc, int(back is not None))
-    ws = None
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=ctx.device)
-        desc.ws, desc.ws_bytes = ws.data_ptr(), need
-    _launch(dev, "dc_attn_mask_fwd" if back is None else "dc_attn_mask_bwd", desc, ctx.stream)
+        p, ld = zip(*(_row_view(n, t, rows, cols, dt, dev) for n, t, rows, cols in
+                      (("dout", back[0], nq, hq), ("dq", back[1], nq, hq), ("dk", back[2], nk, hk), ("dv", back[3], nk, hk))))
+        grads = p + ld
+    desc = PACK_ATTN.pack(
+        kind, nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po, _flat("lse", lse, nb * heads * tq, f4, dev), ldq, ldk, ldv, ldo,
+        scale, softcap, _flat("slopes", slopes, heads, f4, dev), bool(causal), _flat("prefix", prefix, nb, i4, dev),
+        _flat("kv_len", kv_len, nb, i4, dev), _flat("doc_q", doc_q, nq, i4, dev), _flat("doc_k", doc_k, nk, i4, dev), *grads)
+    need = _lib.load().dc_attn_mask_ws_bytes(desc, back is not None)
+    keep, ws = _scratch(need, dev)
+    _launch(dev, "dc_attn_mask_fwd" if back is None else "dc_attn_mask_bwd", desc, ws, need)
 
 
 def attn_mask_fwd(ctx: Ctx, q, k, v, o, lse, *, nb: int, tq: int, tk: int, heads: int, kv_heads: int, d: int,
@@ -576,13 +584,14 @@ def rotary(ctx: Ctx, x, rows: int, heads: int, d: int, freqs, y=None, *, pos=Non
     dev = _device_of(ctx)
     px, ldx = _row_view("x", x, rows, heads * d, dt, dev)
     py, ldy = (px, ldx) if y is None else _row_view("y", y, rows, heads * d, dt, dev)
-    _launch(dev, "dc_rotary", px, ldx, py, ldy, TYPE_IDS[dt], rows, heads, d, off, rot,
-            _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), pos0, t, mag,
-            interleaved, inverse, ctx.stream)
+    _launch(dev, "dc_rotary", PACK_ROTARY.pack(
+        px, py, _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), ldx, ldy, rows,
+        TYPE_IDS[dt], heads, d, off, rot, pos0, t, bool(interleaved), bool(inverse), mag))
     return x if y is None else y
 
 
 NORMS = {"none": 0, "layer": 1, "rms": 2}
+NO_SUMS = (0,) * 14   # the backward's fields of a forward call
 
 
 def _resnorm(ctx: Ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats):
@@ -602,17 +611,13 @@ def _resnorm(ctx: Ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s,
         gates = (gate.t if isinstance(gate, Slice) else gate).shape[0]
         if gates == 0 or rows % gates:
             raise ValueError(f"resnorm: {gates} gate rows for {rows} rows (one for each of equal runs of rows)")
-    dev = _device_of(ctx)
-    d = ResnormDesc(TYPE_IDS[dt], c, NORMS[first], NORMS[second], rows, gates)
-    d.x, d.ldx = _row_view("x", x, rows, c, dt, dev)
-    d.y, d.ldy = _row_view("y", y, rows, c, dt, dev)
-    if gates:
-        d.gate, d.ldg = _row_view("gate", gate, gates, c, dt, dev)
-    f4 = torch.float32
-    d.w1, d.b1, d.w2, d.b2 = (_flat(n, v, c, f4, dev) for n, v in (("w1", w1), ("b1", b1), ("w2", w2), ("b2", b2)))
-    d.a, d.s, d.eps = a, s, eps
-    d.stats = _flat("stats", stats, 4 * rows, f4, dev)
-    return d, dt, dev
+    dev, f4 = _device_of(ctx), torch.float32
+    px, ldx = _row_view("x", x, rows, c, dt, dev)
+    py, ldy = _row_view("y", y, rows, c, dt, dev)
+    pg, ldg = _row_view("gate", gate, gates, c, dt, dev) if gates else (0, 0)
+    common = (TYPE_IDS[dt], c, NORMS[first], NORMS[second], rows, gates, px, py, pg, _flat("w1", w1, c, f4, dev),
+              _flat("b1", b1, c, f4, dev), _flat("w2", w2, c, f4, dev), _flat("b2", b2, c, f4, dev), ldx, ldy, ldg)
+    return common, _flat("stats", stats, 4 * rows, f4, dev), gates, dt, dev
 
 
 def resnorm_fwd(ctx: Ctx, x, y, rows: int, c: int, r, h, stats, *, first: str = "none", second: str = "layer", w1=None, b1=None,
@@ -620,13 +625,12 @@ def resnorm_fwd(ctx: Ctx, x, y, rows: int, c: int, r, h, stats, *, first: str = 
     """r = a x + s gate N1(y) and h = N2(r) in one pass (include/dcamd.h dc_resnorm_desc): x the residual stream, y a block's
     output.  Norms "none", "layer" or "rms" with fp32 weights (None: 1) and offsets (None: 0); gate [gates][c] in the rows' type,
     each for rows / gates rows in turn; h None where second is "none"; stats fp32 [rows][4] for the backward.  Returns r, h."""
-    d, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
+    common, pst, _, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
     if (second == "none") != (h is None):
         raise ValueError("resnorm: h goes with a second norm")
-    d.r, d.ldr = _row_view("r", r, rows, c, dt, dev)
-    if h is not None:
-        d.h, d.ldh = _row_view("h", h, rows, c, dt, dev)
-    _launch(dev, "dc_resnorm_fwd", d, ctx.stream)
+    pr, ldr = _row_view("r", r, rows, c, dt, dev)
+    ph, ldh = (0, 0) if h is None else _row_view("h", h, rows, c, dt, dev)
+    _launch(dev, "dc_resnorm_fwd", PACK_RESNORM.pack(*common, ldr, ldh, a, s, eps, pr, ph, pst, *NO_SUMS))
     return r, h
 
 
@@ -635,7 +639,7 @@ def resnorm_bwd(ctx: Ctx, x, y, rows: int, c: int, stats, dr, dh, dx, dy, *, fir
                 db1=None, dw2=None, db2=None):
     """Gradients of resnorm_fwd from its x, y, weights and stats: dx, dy, and those of dgate (like gate), dw1, db1, dw2, db2 (fp32
     [c]) that are given.  dr is the gradient of r from elsewhere (None: none), dh that of h (None where second is "none")."""
-    d, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
+    common, pst, gates, dt, dev = _resnorm(ctx, x, y, rows, c, first, second, w1, b1, w2, b2, gate, a, s, eps, stats)
     if (second == "none") != (dh is None):
         raise ValueError("resnorm: dh goes with a second norm")
     if dr is None and dh is None:
@@ -643,21 +647,14 @@ def resnorm_bwd(ctx: Ctx, x, y, rows: int, c: int, stats, dr, dh, dx, dy, *, fir
     if dgate is not None and gate is None or first == "none" and (dw1 is not None or db1 is not None) \
             or second == "none" and (dw2 is not None or db2 is not None):
         raise ValueError("resnorm: a gradient of what the forward does not have")
-    for n, v in (("dr", dr), ("dh", dh), ("dx", dx), ("dy", dy)):
-        if v is not None:
-            p, ld = _row_view(n, v, rows, c, dt, dev)
-            setattr(d, n, p)
-            setattr(d, "ld" + n, ld)
-    if dgate is not None:
-        d.dgate, d.lddg = _row_view("dgate", dgate, d.gates, c, dt, dev)
-    for n, v in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2)):
-        setattr(d, n, _flat(n, v, c, torch.float32, dev))
-    need = _lib.load().dc_resnorm_ws_bytes(d)
-    ws = None
-    if need:   # the call's own, as the attention's
-        ws = torch.empty(need, dtype=torch.uint8, device=ctx.device)
-        d.ws, d.ws_bytes = ws.data_ptr(), need
-    _launch(dev, "dc_resnorm_bwd", d, ctx.stream)
+    (pdr, lddr), (pdh, lddh), (pdx, lddx), (pdy, lddy), (pdg, lddg) = (
+        (0, 0) if v is None else _row_view(n, v, m, c, dt, dev)
+        for n, v, m in (("dr", dr, rows), ("dh", dh, rows), ("dx", dx, rows), ("dy", dy, rows), ("dgate", dgate, gates)))
+    sums = (_flat(n, v, c, torch.float32, dev) for n, v in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2)))
+    desc = PACK_RESNORM.pack(*common, 0, 0, a, s, eps, 0, 0, pst, pdr, pdh, pdx, pdy, pdg, *sums, lddr, lddh, lddx, lddy, lddg)
+    need = _lib.load().dc_resnorm_ws_bytes(desc)
+    keep, ws = _scratch(need, dev)
+    _launch(dev, "dc_resnorm_bwd", desc, ws, need)
     return dx, dy
 
 

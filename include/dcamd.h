@@ -477,12 +477,11 @@ typedef struct dc_attn_desc {
   const void* dout;             /* backward: [nb tq][lddo] */
   void *dq, *dk, *dv;
   int lddo, lddq, lddk, lddv;
-  float* ws;                    /* scratch of dc_attn_mask_ws_bytes, private to the call until it has run */
-  long long ws_bytes;
 } dc_attn_desc;
+/* ws: scratch of dc_attn_mask_ws_bytes (0: NULL will do), private to the call until it has run */
 long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward);
-int dc_attn_mask_fwd(const dc_attn_desc* d, void* stream);
-int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream);
+int dc_attn_mask_fwd(const dc_attn_desc* d, void* ws, long long ws_bytes, void* stream);
+int dc_attn_mask_bwd(const dc_attn_desc* d, void* ws, long long ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------- rotary positions
  * y = x with the columns [off, off + rot) of each of `heads` heads (head h at column h d) turned by angles pos * freqs[i],
@@ -490,8 +489,16 @@ int dc_attn_mask_bwd(const dc_attn_desc* d, void* stream);
  * gradient (dL/dx from dL/dy).  y may be x (same ldx); else the other columns are copied.  Angles are formed in 64 bits.
  * type: 0 bf16, 1 fp16, 2 fp32.  pos: int [rows], or NULL: row r stands at pos0 + r % t.  freqs: [rot / 2] in device memory.
  * Any d, off and even rot; 16-byte accesses where base, ld, d and off allow them and rot is whole packs. */
-int dc_rotary(const void* x, long long ldx, void* y, long long ldy, int type, long long rows, int heads, int d, int off, int rot,
-              const double* freqs, const int* pos, int pos0, int t, float mag, int interleaved, int inverse, void* stream);
+typedef struct dc_rotary_desc {
+  const void* x;
+  void* y;
+  const double* freqs;
+  const int* pos;
+  long long ldx, ldy, rows;
+  int type, heads, d, off, rot, pos0, t, interleaved, inverse;
+  float mag;
+} dc_rotary_desc;
+int dc_rotary(const dc_rotary_desc* r, void* stream);
 /* host: freqs[i] = theta^(-2 i / rot) and mag, scaled to reach `factor` times further: 0 not; 1 every frequency / factor; 2 a base
  * of theta factor^(rot / (rot - 2)) (rot >= 4: the fastest stays, the slowest is divided by factor); 3 by turns over the `trained`
  * length: fast or more stay, slow or fewer are divided by factor, between them in proportion, and mag = 1 + 0.1 ln factor. */
@@ -519,12 +526,11 @@ typedef struct dc_resnorm_desc {
   void *dx, *dy, *dgate;
   float *dw1, *db1, *dw2, *db2;
   int lddr, lddh, lddx, lddy, lddg;
-  float* ws;                    /* backward: scratch of dc_resnorm_ws_bytes, private to the call until it has run */
-  long long ws_bytes;
 } dc_resnorm_desc;
 int dc_resnorm_fwd(const dc_resnorm_desc* d, void* stream);
+/* ws: scratch of dc_resnorm_ws_bytes (0: NULL will do), private to the call until it has run */
 long long dc_resnorm_ws_bytes(const dc_resnorm_desc* d);
-int dc_resnorm_bwd(const dc_resnorm_desc* d, void* stream);
+int dc_resnorm_bwd(const dc_resnorm_desc* d, void* ws, long long ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -47,7 +47,7 @@ def test_row_views():
     for bad in (t[:, :3], t[:1], t.int()):
         with pytest.raises(ValueError):
             ops._flat("t", bad, 41, torch.float32, -1)
-    assert ops._flat("t", None, 5, torch.float32, 0) is None
+    assert ops._flat("t", None, 5, torch.float32, 0) == 0
 
 
 def descriptor(**kw):
@@ -69,22 +69,35 @@ ARG, ALIGN = 1, 3
     (dict(d=136, ldq=544, ldo=544, ldk=272, ldv=272), ARG), (dict(scale=0.0), ARG), (dict(scale=float("nan")), ARG),
     (dict(scale=float("inf")), ARG), (dict(softcap=-1.0), ARG), (dict(softcap=float("nan")), ARG), (dict(prefix=4096), ARG),
     (dict(doc_q=4096), ARG), (dict(doc_k=4096), ARG), (dict(ldq=248), ARG), (dict(ldk=120), ARG), (dict(ldq=260), ALIGN),
-    (dict(ldv=132), ALIGN), (dict(q=4098), ALIGN), (dict(v=4104), ALIGN), (dict(ws=4100), ALIGN),
+    (dict(ldv=132), ALIGN), (dict(q=4098), ALIGN), (dict(v=4104), ALIGN),
     (dict(nb=1 << 20, tq=1 << 10), ARG), (dict(doc_q=4096, doc_k=4096), ARG), (dict(tq=1, tk=100000), ARG)])
 def test_entry_refuses(entry, kw, status):
-    """The last two want scratch that the descriptor does not bring."""
-    assert getattr(_lib.load(), entry)(descriptor(**kw), None) == status
+    """The last two want scratch that the call does not bring."""
+    assert getattr(_lib.load(), entry)(C.byref(descriptor(**kw)), None, 0, None) == status
 
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dout=None), ARG), (dict(dq=None), ARG), (dict(dk=None), ARG), (dict(dv=None), ARG), (dict(lddo=248), ARG),
     (dict(lddk=132), ALIGN), (dict(dv=4098), ALIGN), (dict(), ARG)])
 def test_backward_entry_refuses(kw, status):
-    assert _lib.load().dc_attn_mask_bwd(descriptor(**kw), None) == status
+    assert _lib.load().dc_attn_mask_bwd(C.byref(descriptor(**kw)), None, 0, None) == status
 
 
 def test_entries_take_no_null_descriptor():
     lib = _lib.load()
-    null = C.POINTER(_lib.AttnDesc)()
-    assert lib.dc_attn_mask_fwd(null, None) == ARG and lib.dc_attn_mask_bwd(null, None) == ARG
-    assert lib.dc_attn_mask_ws_bytes(null, 0) == 0
+    assert lib.dc_attn_mask_fwd(None, None, 0, None) == ARG and lib.dc_attn_mask_bwd(None, None, 0, None) == ARG
+    assert lib.dc_attn_mask_ws_bytes(None, 0) == 0
+
+
+def test_scratch_alignment():
+    lib, d = _lib.load(), C.byref(descriptor())
+    assert lib.dc_attn_mask_fwd(d, 4100, 1 << 30, None) == ALIGN and lib.dc_attn_mask_bwd(d, 4100, 1 << 30, None) == ALIGN
+
+
+@pytest.mark.parametrize("desc,pack", [(_lib.AttnDesc, _lib.PACK_ATTN), (_lib.RotaryDesc, _lib.PACK_ROTARY),
+                                       (_lib.ResnormDesc, _lib.PACK_RESNORM)])
+def test_packed_descriptors(desc, pack):
+    """The packed bytes are the structure's, field by field."""
+    values = [i + 1 for i in range(len(desc._fields_))]
+    d = desc(*values)
+    assert pack.size == C.sizeof(desc) and pack.pack(*values) == bytes(d)

@@ -43,12 +43,12 @@ BOTH = [(dict(type=3), ARG), (dict(type=-1), ARG), (dict(c=0), ARG), (dict(c=60)
         (dict(gate=None), ARG), (dict(gates=0), ARG), (dict(gates=4), ARG), (dict(gates=-2), ARG), (dict(first=0), ARG),
         (dict(second=0), ARG), (dict(eps=-1.0), ARG), (dict(eps=float("nan")), ARG), (dict(ldx=56), ARG), (dict(ldg=56), ARG),
         (dict(rows=1 << 42), ARG), (dict(ldx=68), ALIGN), (dict(ldg=68), ALIGN), (dict(x=4104), ALIGN), (dict(gate=4104), ALIGN),
-        (dict(w1=4098), ALIGN), (dict(stats=4100), ALIGN), (dict(ws=4100), ALIGN)]
+        (dict(w1=4098), ALIGN), (dict(stats=4100), ALIGN)]
 
 
 @pytest.mark.parametrize("kw,status", BOTH + [(dict(r=None), ARG), (dict(h=None), ARG), (dict(ldr=56), ARG), (dict(ldh=68), ALIGN)])
 def test_forward_entry_refuses(kw, status):
-    assert _lib.load().dc_resnorm_fwd(descriptor(**kw), None) == status
+    assert _lib.load().dc_resnorm_fwd(C.byref(descriptor(**kw)), None) == status
 
 
 @pytest.mark.parametrize("kw,status", BOTH + [
@@ -56,10 +56,12 @@ def test_forward_entry_refuses(kw, status):
     (dict(dgate=4096, lddg=56), ARG), (dict(dgate=4096, gates=0, gate=None), ARG), (dict(first=0, w1=None, dw1=4096), ARG),
     (dict(second=0, w2=None, dh=None, db2=4096), ARG), (dict(second=0, w2=None, dh=None, dr=None), ARG), (dict(dw1=4096), ARG)])
 def test_backward_entry_refuses(kw, status):
-    """The last wants scratch that the descriptor does not bring."""
-    assert _lib.load().dc_resnorm_bwd(descriptor(**kw), None) == status
+    """The last wants scratch that the call does not bring."""
+    assert _lib.load().dc_resnorm_bwd(C.byref(descriptor(**kw)), None, 0, None) == status
 
 
 def test_no_null_descriptor():
-    lib, null = _lib.load(), C.POINTER(_lib.ResnormDesc)()
-    assert lib.dc_resnorm_fwd(null, None) == ARG and lib.dc_resnorm_bwd(null, None) == ARG and lib.dc_resnorm_ws_bytes(null) == 0
+    lib = _lib.load()
+    assert lib.dc_resnorm_fwd(None, None) == ARG and lib.dc_resnorm_bwd(None, None, 0, None) == ARG
+    assert lib.dc_resnorm_ws_bytes(None) == 0
+    assert lib.dc_resnorm_bwd(C.byref(descriptor(dw1=4096)), 4100, 1 << 30, None) == ALIGN

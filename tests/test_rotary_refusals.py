@@ -1,4 +1,5 @@
 """Frequencies of the rotary positions (host), and what the rotary call refuses (CPU: nothing is launched)."""
+import ctypes as C
 import math
 
 import pytest
@@ -55,4 +56,8 @@ def test_call_refuses(kw):
 def test_entry_refuses(kw, status):
     a = dict(x=4096, ldx=128, y=8192, ldy=128, type=0, rows=4, heads=2, d=64, off=0, rot=64, freqs=4096, pos=None, pos0=0, t=4,
              mag=1.0, interleaved=0, inverse=0)
-    assert _lib.load().dc_rotary(*dict(a, **kw).values(), None) == status
+    assert _lib.load().dc_rotary(C.byref(_lib.RotaryDesc(**dict(a, **kw))), None) == status
+
+
+def test_no_null_descriptor():
+    assert _lib.load().dc_rotary(None, None) == 1
