@@ -84,6 +84,37 @@ __device__ __forceinline__ Vec<half>::v8 tr_frag(const half* tile, TrAt o) {
   return __builtin_bit_cast(Vec<half>::v8, r);
 }
 
+// Four transposed fragments of 128 columns (rows from tile + IMM bytes on), read and waited for in one block: the compiler, which
+// takes the builtin's reads for reads of what is still on its way into LDS, would wait for the next tile here.
+struct TrAt4 {
+  unsigned lo[4], hi[4];
+  template <typename T>
+  __device__ __forceinline__ void init(const T* lds, int lane) {
+    const unsigned base = (unsigned)(unsigned long)((DC_LDS const char*)lds);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const TrAt o = tr_at<128>(32 * n, lane);
+      lo[n] = base + o.lo * 2;
+      hi[n] = base + o.hi * 2;
+    }
+  }
+};
+template <typename T, int IMM>
+__device__ __forceinline__ void tr_frags(const TrAt4& a, typename Vec<T>::v8 (&f)[4]) {
+  struct Two { unsigned long long lo, hi; } r[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0].lo), "=&v"(r[0].hi), "=&v"(r[1].lo), "=&v"(r[1].hi), "=&v"(r[2].lo), "=&v"(r[2].hi), "=&v"(r[3].lo),
+        "=&v"(r[3].hi)
+      : "v"(a.lo[0]), "v"(a.hi[0]), "v"(a.lo[1]), "v"(a.hi[1]), "v"(a.lo[2]), "v"(a.hi[2]), "v"(a.lo[3]), "v"(a.hi[3]), "n"(IMM));
+#pragma unroll
+  for (int n = 0; n < 4; ++n) f[n] = __builtin_bit_cast(typename Vec<T>::v8, r[n]);
+}
+
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::v8 acc_frag(const f32x16& a, int half_of) {
   typename Vec<T>::v8 r;
@@ -99,33 +130,73 @@ __device__ __forceinline__ typename Vec<T>::v8 load8_or_0(const T* p, bool ok) {
   return v;
 }
 
-// ROWS x DP elements by 256 threads, through registers: load() issues the global reads of a tile (rows from `last` on and
-// columns from d on read a valid place instead, so that no load waits behind a branch), store() writes them to LDS with zeros
-// for those and for the rows that `keep` leaves out: nothing that lies in a masked place is ever multiplied.
-template <typename T, int DP, int ROWS>
-struct Stage {
-  static constexpr int CH = DP / 8, N = ROWS * CH / 256, STEP = 256 / CH;
-  uint4 reg[N];
-  __device__ __forceinline__ void load(const T* base, int ld, int d, int last) {
-    const int r = threadIdx.x / CH, c = threadIdx.x % CH;
+// 64 x DP elements into an LDS tile by 256 threads, straight from memory (16 bytes a lane, no registers between).  A lane's offsets
+// are the same for every tile; the tile's first row is in the scalar base (64 bits, so a long cache needs no wide offsets).  Rows
+// behind `last`, rows that `keep` leaves out and columns from d on take an offset outside the descriptor and arrive as zeros:
+// nothing that lies in a masked place is ever multiplied.
+template <typename T, int DP>
+struct Dma {
+  static constexpr int CH = DP / 8, N = 64 * CH / 256, STEP = 256 / CH;
+  static constexpr unsigned OUT = 0x80000000u;
+  unsigned off[N];
+  int row, wave;
+  __device__ __forceinline__ void init(int ld, int d) {
+    row = threadIdx.x / CH;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      reg[i] = *reinterpret_cast<const uint4*>(base + (long)min(r + STEP * i, last) * ld + (c * 8 < d ? c * 8 : 0));
+    for (int i = 0; i < N; ++i) {
+      const int r = row + STEP * i, c = (int)(threadIdx.x % CH) ^ sw<DP>(r);
+      off[i] = c * 8 < d ? ((unsigned)r * ld + c * 8) * sizeof(T) : OUT;
+    }
   }
-  __device__ __forceinline__ void store(T* tile) const {
-    const int r = threadIdx.x / CH, c = threadIdx.x % CH;
+  __device__ __forceinline__ static __amdgpu_buffer_rsrc_t rsrc(const T* base) {
+    const unsigned long long a = (unsigned long long)base;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), (short)0, 0x7fffffff, 0x00020000);
+  }
+  __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t r, T* tile, int i, unsigned o) const {
+#if defined(__HIP_DEVICE_COMPILE__)   // (the builtin exists in the device pass alone)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DC_LDS char*)(tile + (64 * wave + 256 * i) * 8), 16, o, 0, 0, 0);
+#endif
+  }
+  __device__ __forceinline__ void load(const T* base, T* tile, int last) const {
+    const __amdgpu_buffer_rsrc_t r = rsrc(base);
+    if (last >= 63) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(tile + tile_at<DP>(r + STEP * i, c)) = reg[i];
+      for (int i = 0; i < N; ++i) put(r, tile, i, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) put(r, tile, i, row + STEP * i <= last ? off[i] : OUT);
+    }
   }
   template <typename F>
-  __device__ __forceinline__ void store_some(T* tile, int d, int last, F&& keep) {
-    const int r = threadIdx.x / CH, c = threadIdx.x % CH;
+  __device__ __forceinline__ void load_some(const T* base, T* tile, int last, F&& keep) const {
+    const __amdgpu_buffer_rsrc_t r = rsrc(base);
+    bool in[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c * 8 >= d || r + STEP * i > last || !keep(r + STEP * i)) reg[i] = make_uint4(0, 0, 0, 0);
-    store(tile);
+    for (int i = 0; i < N; ++i) in[i] = row + STEP * i <= last && keep(row + STEP * i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(r, tile, i, in[i] ? off[i] : OUT);
   }
 };
+// 64 words into LDS, by one wave
+__device__ __forceinline__ void dma_words(const void* base, void* lds, int last) {
+  const int lane = threadIdx.x & 63;
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(Dma<bf16, 64>::rsrc((const bf16*)base), (DC_LDS char*)lds, 4,
+                                           lane <= last ? lane * 4u : Dma<bf16, 64>::OUT, 0, 0, 0);
+#endif
+}
+// Waits until at most N vector-memory operations of this wave are under way: those issued before the last N have landed.
+template <int N>
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// All waves: what each has waited for is there for all, and what each has read may be overwritten.  (__syncthreads() would also
+// wait for the tiles that are on their way.)
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 __device__ __forceinline__ int length_of(const Call& p, int b) {
   return p.kv_len ? min(max(p.kv_len[b], 0), p.tk) : p.tk;
@@ -141,17 +212,116 @@ __device__ __forceinline__ int wave_max_i(int v) {
   return v;
 }
 // the sum / maximum of a value over lanes l and l ^ 32, which hold the two halves of a query's scores
-__device__ __forceinline__ float pair_sum(float x) { return x + __shfl_xor(x, 32, 64); }
-__device__ __forceinline__ float pair_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
-
-// Blocks are dealt to the eight XCDs in turn; this gives each a contiguous run of work, so the blocks that read the same keys
-// share an L2.  Returns n where a block has nothing to do.
-__device__ __forceinline__ int xcd_work(int n) {
-  const int per = (n + 7) / 8;
-  const int i = blockIdx.x / 8, w = (blockIdx.x % 8) * per + i;
-  return i < per && w < n ? w : n;
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-inline unsigned xcd_grid(long n) { return (unsigned)((n + 7) / 8 * 8); }
+__device__ __forceinline__ float pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Blocks are dealt to the eight XCDs in turn.  Units (a key head of a sequence) go to an XCD whole as far as they come by eights, so
+// that the blocks that read the same keys share an L2; the blocks of the rest are spread over all (whole units left over would leave
+// XCDs idle: 5 heads of 71 blocks, half of them long, 169 us with runs of blocks to an XCD).
+__device__ __forceinline__ void unit_of(int units, int per_unit, int& unit, int& r) {
+  const int whole = units / 8 * 8, n = whole * per_unit, i = blockIdx.x;
+  if (i < n) {
+    unit = i / 8 / per_unit * 8 + i % 8;
+    r = i / 8 % per_unit;
+  } else {
+    unit = whole + (i - n) / per_unit;
+    r = (i - n) % per_unit;
+  }
+}
+
+// The query rows of a block of fwd_kernel or dq_kernel: 4 x 32 rows of one head.
+struct QueryBlock {
+  int b, kh, h, part, qi, len, pos, lim, mine;   // lim: the lane's query sees the keys below it (of its document `mine`)
+  bool live;
+  // of a unit's tiles of 128 rows (the longest rows of a causal call first) x splits x heads of the group
+  __device__ __forceinline__ void init(const Call& p, int splits) {
+    const int nqb = (p.tq + 127) / 128;
+    int unit, w;
+    unit_of(p.nb * p.kvh, nqb * p.grp * splits, unit, w);
+    b = unit / p.kvh;
+    kh = unit % p.kvh;
+    h = kh * p.grp + w % p.grp;
+    w /= p.grp;
+    part = w % splits;
+    len = length_of(p, b);
+    qi = (nqb - 1 - w / splits) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    live = qi < p.tq;
+    pos = qi + len - p.tq;
+    lim = p.causal ? min(len, max(pos + 1, p.prefix ? p.prefix[b] : 0)) : len;
+    mine = p.doc_q ? (live ? p.doc_q[(long)b * p.tq + qi] : -1) : 0;
+    if (mine < 0) lim = 0;
+  }
+  // The 64-key tiles [t0, t1) in which some row with `sees` may see a key.
+  __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1) const {
+    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; range[4] = 0; }
+    __syncthreads();
+    const int most = wave_max_i(sees ? lim : 0);
+    if ((threadIdx.x & 63) == 0) atomicMax(&range[1], most);
+    if (p.doc_q && sees && mine >= 0) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
+    __syncthreads();
+    t0 = 0;
+    t1 = (range[1] + 63) / 64;
+    if (p.doc_q) {
+      const int nt = (p.tk + 63) / 64, least = range[2], largest = range[3];
+      const int4* sum = p.sum_k + (long)b * nt;
+      int first = 0x7fffffff, last = -1;
+      for (int t = threadIdx.x; t < t1; t += blockDim.x) {
+        const int4 s = sum[t];
+        if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
+      }
+      if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[4], last + 1); }
+      __syncthreads();
+      t1 = range[4];
+      t0 = min(range[0], t1);
+    }
+    t0 = __builtin_amdgcn_readfirstlane(t0);
+    t1 = __builtin_amdgcn_readfirstlane(t1);
+  }
+};
+
+// The keys' tiles of a query block in LDS, S of them in turn: K, V and the keys' documents.
+template <typename T, int DP, int S>
+struct KeyRing {
+  static constexpr int TILE = 64 * DP;
+  struct Lds {
+    __attribute__((aligned(16))) T tiles[S][2 * TILE];
+    __attribute__((aligned(16))) int ids[S][64];
+  };
+  Dma<T, DP> k, v;
+  const T *kb, *vb;
+  const int* kid;
+  const int4* sum;
+  int len;
+  __device__ __forceinline__ void init(const Call& p, const QueryBlock& q) {
+    k.init(p.ldk, p.d);
+    v.init(p.ldv, p.d);
+    kb = (const T*)p.k + (long)q.b * p.tk * p.ldk + q.kh * p.d;
+    vb = (const T*)p.v + (long)q.b * p.tk * p.ldv + q.kh * p.d;
+    kid = p.doc_q ? p.doc_k + (long)q.b * p.tk : nullptr;
+    sum = p.doc_q ? p.sum_k + (long)q.b * ((p.tk + 63) / 64) : nullptr;
+    len = q.len;
+  }
+  // tile t on its way (each wave issues 2 Dma::N operations or more)
+  __device__ __forceinline__ void load(const Call& p, Lds& lds, int t, int buf) const {
+    const int r0 = t * 64, last = len - 1 - r0;
+    const T *ka = kb + (long)r0 * p.ldk, *va = vb + (long)r0 * p.ldv;
+    if (kid && sum[t].z) {   // a key in no document: its row may hold anything
+      auto keep = [&](int r) __attribute__((always_inline)) { return kid[min(r0 + r, len - 1)] >= 0; };
+      k.load_some(ka, lds.tiles[buf], last, keep);
+      v.load_some(va, lds.tiles[buf] + TILE, last, keep);
+    } else {
+      k.load(ka, lds.tiles[buf], last);
+      v.load(va, lds.tiles[buf] + TILE, last);
+    }
+    if (kid && k.wave == 0) dma_words(kid + r0, lds.ids[buf], last);
+  }
+};
 
 // Host side: what both directions share (attn_mask_fwd.hip).
 int make_call(const dc_attn_desc* d, Call& c, bool backward);

@@ -10,6 +10,7 @@
 // lies in [2^-4, 2^-3): gradients far below 1 keep their digits, and dS stays in range while |v| < 2000.  P in dV is held 2^14 times
 // as large for the same reason.  Both factors are taken out of the fp32 sums again.
 #include "attn_mask.h"
+#include <type_traits>
 
 namespace dcm {
 namespace {
@@ -31,36 +32,28 @@ __device__ __forceinline__ float near_sixteenth(float x) {
   return ldexpf(1.0f, min(max(-4 - e, -100), 100));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SHAPED>
 __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
-  constexpr int TILE = 64 * DP;
-  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
-  __shared__ int ids[2][64];
-  __shared__ int range[4];
-  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
-  const int nqb = (p.tq + 127) / 128, per_head = nqb * p.grp, total = p.nb * p.kvh * per_head;
-  int w = xcd_work(total);
-  if (w >= total) return;
-  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
-  w %= per_head;
-  const int h = kh * p.grp + w % p.grp, qb = nqb - 1 - w / p.grp;
-  const int len = length_of(p, b), q0 = qb * 128, qi = q0 + wid * 32 + (lane & 31);
-  const bool live = qi < p.tq;
-  const int pos = qi + len - p.tq;
-  const int pre = p.prefix ? p.prefix[b] : 0;
-  const long row = ((long)b * p.heads + h) * p.tq + (live ? qi : 0), trow = (long)b * p.tq + (live ? qi : 0);
+  constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
+  typedef KeyRing<T, DP, S> Ring;
+  __shared__ typename Ring::Lds lds;
+  __shared__ int range[5];
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
+  QueryBlock q;
+  q.init(p, 1);
+  const long row = ((long)q.b * p.heads + q.h) * p.tq + (q.live ? q.qi : 0), trow = (long)q.b * p.tq + (q.live ? q.qi : 0);
   const float lse = p.lse[row];
-  const bool sees = live && lse != -INFINITY;
+  const bool sees = q.live && lse != -INFINITY;
   v8 qf[DP / 16], df[DP / 16];
   float del = 0.0f, most = 0.0f;
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     const int c = 16 * s + 8 * hh;
     const bool ok = sees && c < p.d;
-    qf[s] = load8_or_0((const T*)p.q + trow * p.ldq + h * p.d + c, ok);
-    df[s] = load8_or_0((const T*)p.dout + trow * p.lddo + h * p.d + c, ok);
-    const v8 of = load8_or_0((const T*)p.o + trow * p.ldo + h * p.d + c, ok);
+    qf[s] = load8_or_0((const T*)p.q + trow * p.ldq + q.h * p.d + c, ok);
+    df[s] = load8_or_0((const T*)p.dout + trow * p.lddo + q.h * p.d + c, ok);
+    const v8 of = load8_or_0((const T*)p.o + trow * p.ldo + q.h * p.d + c, ok);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       del = fmaf((float)df[s][j], (float)of[j], del);
@@ -70,146 +63,120 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
   del = pair_sum(del);
   most = pair_max(most);
   const float nl = sees ? -lse * kLog2e : -INFINITY;
-  if (live && hh == 0) {
+  if (q.live && hh == 0) {
     bk.nlse[row] = nl;
     bk.ndel[row] = -del;
   }
   const float wave_most = wave_max(most);
-  const bool blind = __any(live && !sees);
-  if (lane == 0) bk.rows32[((long)b * p.heads + h) * bk.n32 + qb * 4 + wid] = make_int2(blind, __float_as_int(wave_most));
+  const bool blind = __any(q.live && !sees);
+  if (lane == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
   const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
+  int t0, t1;
+  q.tiles(p, sees, range, t0, t1);
 
-  int lim = p.causal ? min(len, max(pos + 1, pre)) : len;
-  const int mine = p.doc_q && live ? p.doc_q[(long)b * p.tq + qi] : 0;
-  if (!sees) lim = 0;
-  if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
-  __syncthreads();
-  atomicMax(&range[1], lim);
-  if (p.doc_q && sees) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
-  __syncthreads();
-  int t0 = 0, t1 = (range[1] + 63) / 64;
-  bool holes = false;
-  if (p.doc_q) {
-    const int nt = (p.tk + 63) / 64, least = range[2], largest = range[3];
-    const int4* sum = p.sum_k + (long)b * nt;
-    int first = 0x7fffffff, last = -1, none = 0;
-    for (int t = threadIdx.x; t < t1; t += 256) {
-      const int4 s = sum[t];
-      if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
-      none |= s.z;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) { range[1] = 0; range[2] = 0; }
-    __syncthreads();
-    if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
-    if (none) atomicOr(&range[2], 1);
-    __syncthreads();
-    t0 = min(range[0], range[1]);
-    t1 = range[1];
-    holes = range[2];
-  }
-
-  const T* kb = (const T*)p.k + (long)b * p.tk * p.ldk + kh * p.d;
-  const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
-  const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
-  Stage<T, DP, 64> ks, vs;
-  int id_next = -1;
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int r0 = t * 64, last = len - 1 - r0;
-    ks.load(kb + (long)r0 * p.ldk, p.ldk, p.d, min(last, 63));
-    vs.load(vb + (long)r0 * p.ldv, p.ldv, p.d, min(last, 63));
-    if (kid && threadIdx.x < 64) id_next = kid[min(r0 + (int)threadIdx.x, len - 1)];
-  };
-  auto put = [&](int t, int buf) __attribute__((always_inline)) {
-    const int r0 = t * 64, last = len - 1 - r0;
-    if (last >= 63 && p.d == DP && !holes) {
-      ks.store(tiles[buf]);
-      vs.store(tiles[buf] + TILE);
-    } else {
-      auto keep = [&](int r) { return !holes || (r <= last && kid[r0 + r] >= 0); };
-      ks.store_some(tiles[buf], p.d, last, keep);
-      vs.store_some(tiles[buf] + TILE, p.d, last, keep);
-    }
-    if (kid && threadIdx.x < 64) ids[buf][threadIdx.x] = id_next;
-  };
+  Ring ring;
+  ring.init(p, q);
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
-  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
-  TrAt ka[DP / 32];
+  TrAt ka[2];
+  TrAt4 ka4;
+  if constexpr (DP == 128) ka4.init(lds.tiles[0], lane);
+  else
 #pragma unroll
-  for (int n = 0; n < DP / 32; ++n) ka[n] = tr_at<DP>(32 * n, lane);
-  if (t0 < t1) {
-    fetch(t0);
-    put(t0, 0);
-  }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (t + 1 < t1) fetch(t + 1);
-    const T* kt = tiles[buf];
+    for (int n = 0; n < 2; ++n) ka[n] = tr_at<DP>(32 * n, lane);
+  const int seen_by_all = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? q.lim : 0x7fffffff));
+  vm_wait<0>();
+  if (t0 < t1) ring.load(p, lds, t0, 0);
+  if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
+  auto step = [&](int t, auto B) __attribute__((always_inline)) {   // as the forward's
+    constexpr int buf = decltype(B)::value;
+    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
+    else vm_wait<0>();
+    tile_barrier();
+    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
+    const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
-    bool partial = __any(sees && lim < t * 64 + 64);
-    if (kid) partial |= __any(sees && ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
-#pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
+    const int* id = lds.ids[buf];
+    bool partial = seen_by_all < t * 64 + 64;
+    if (ring.kid) partial |= __any(sees && id[0] != q.mine) || __any(id[lane] != id[0]);
+    auto half_tile = [&](auto K) __attribute__((always_inline)) {
+      constexpr int kb2 = decltype(K)::value;
       f32x16 s = {}, dp = {};
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         s = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s);
         dp = mfma(*reinterpret_cast<const v8*>(vt + 32 * kb2 * DP + koff[c]), df[c], dp);
       }
-      if (p.cap2 != 0.0f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float g;
-          s[r] = cap_score(p, s[r], &g);
-          dp[r] = (dp[r] - del) * g;
+      for (int r = 0; r < 16; ++r) dp[r] -= del;
+      if constexpr (SHAPED) {
+        if (p.cap2 != 0.0f) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float g;
+            s[r] = cap_score(p, s[r], &g);
+            dp[r] *= g;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= p.scale * kLog2e;
         }
-      } else {
+        if (p.slopes) {
+          const float dist = (float)(q.pos - t * 64 - 4 * hh);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] -= del;
-      }
-      if (p.slopes) {
-        const float mul = p.cap2 != 0.0f ? 1.0f : p.scale * kLog2e;
-        const float dist = (float)(pos - t * 64 - 4 * hh);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[r] * mul);
+          for (int r = 0; r < 16; ++r)
+            s[r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[r]);
+        }
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float pw = exp2_raw(fmaf(s[r], p.mul, nl));
+        const float pw = exp2_raw(SHAPED ? s[r] + nl : fmaf(s[r], p.mul, nl));
         s[r] = (is_half<T> ? pw * f : pw) * dp[r];
       }
       if (partial) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int key = 32 * kb2 + 8 * g + 4 * hh;
-          int4 id = make_int4(0, 0, 0, 0);
-          if (kid) id = *reinterpret_cast<const int4*>(&ids[buf][key]);
-          const int id4[4] = {id.x, id.y, id.z, id.w};
+          int4 i4 = make_int4(0, 0, 0, 0);
+          if (ring.kid) i4 = *reinterpret_cast<const int4*>(&id[key]);
+          const int id4[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t * 64 + key + e >= lim || (kid && id4[e] != mine)) s[4 * g + e] = 0.0f;
+            if (t * 64 + key + e >= q.lim || (ring.kid && id4[e] != q.mine)) s[4 * g + e] = 0.0f;
         }
       }
+      auto add = [&](auto C) __attribute__((always_inline)) {
+        constexpr int c = decltype(C)::value, at = (32 * kb2 + 16 * c) * DP;
+        v8 f2[DP / 32];
+        if constexpr (DP == 128) tr_frags<T, (buf * 2 * TILE + at) * 2>(ka4, f2);
+        else
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+          for (int n = 0; n < 2; ++n) f2[n] = tr_frag(kt + at, ka[n]);
         const v8 sf = acc_frag<T>(s, c);
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n) dq[n] = mfma(tr_frag(kt + (32 * kb2 + 16 * c) * DP, ka[n]), sf, dq[n]);
-      }
-    }
-    if (t + 1 < t1) put(t + 1, buf ^ 1);
-    __syncthreads();
+        for (int n = 0; n < DP / 32; ++n) dq[n] = mfma(f2[n], sf, dq[n]);
+      };
+      add(std::integral_constant<int, 0>{});
+      add(std::integral_constant<int, 1>{});
+    };
+    half_tile(std::integral_constant<int, 0>{});
+    half_tile(std::integral_constant<int, 1>{});
+    if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
+  };
+  for (int t = t0; t < t1; t += S) {
+    step(t, std::integral_constant<int, 0>{});
+    if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
+    if constexpr (S == 3)
+      if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{});
   }
-  if (!live) return;
+  if (!q.live) return;
   const float k = p.scale / f;
-  T* out = (T*)p.dq + ((long)b * p.tq + qi) * p.lddq + h * p.d;
+  T* out = (T*)p.dq + ((long)q.b * p.tq + q.qi) * p.lddq + q.h * p.d;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -222,6 +189,39 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
       *reinterpret_cast<typename Vec<T>::v4*>(out + col) = v;
     }
 }
+
+// 64 x DP elements by 256 threads, through registers, with the zeros that Dma leaves.
+template <typename T, int DP>
+struct Stage {
+  static constexpr int CH = DP / 8, N = 64 * CH / 256, STEP = 256 / CH;
+  uint4 reg[N];
+  unsigned first, step;   // bytes
+  int row, chunk;
+  __device__ __forceinline__ void init(int ld, int d) {
+    row = threadIdx.x / CH;
+    chunk = threadIdx.x % CH;
+    first = ((unsigned)row * ld + (chunk * 8 < d ? chunk * 8 : 0)) * sizeof(T);
+    step = (unsigned)STEP * ld * sizeof(T);
+  }
+  __device__ __forceinline__ void load(const T* base, int ld, int last) {
+    const char* at = reinterpret_cast<const char*>(base);
+    const unsigned back = (unsigned)ld * sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      reg[i] = *reinterpret_cast<const uint4*>(at + (first + i * step - back * (unsigned)max(row + STEP * i - last, 0)));
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(tile + tile_at<DP>(row + STEP * i, chunk)) = reg[i];
+  }
+  template <typename F>
+  __device__ __forceinline__ void store_some(T* tile, int d, int last, F&& keep) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (chunk * 8 >= d || row + STEP * i > last || !keep(row + STEP * i)) reg[i] = make_uint4(0, 0, 0, 0);
+    store(tile);
+  }
+};
 
 // the factor of dS in dK for a key head: by the largest |dO| of its query heads, the same in every block that needs it
 __device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int b, int kh, float* scratch) {
@@ -236,7 +236,7 @@ __device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int 
 
 constexpr float kPShift = 14.0f;   // fp16: P in dV is 2^14 times as large
 
-template <typename T, int DP>
+template <typename T, int DP, bool SHAPED>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
   constexpr int TILE = 64 * DP;
@@ -246,11 +246,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
   __shared__ int range[4];
   __shared__ float scratch[4];
   const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
-  const int nkb = (p.tk + 127) / 128, per_head = nkb * bk.nk, total = p.nb * p.kvh * per_head;
-  int w = xcd_work(total);
-  if (w >= total) return;
-  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
-  w %= per_head;
+  int unit, w;
+  unit_of(p.nb * p.kvh, (p.tk + 127) / 128 * bk.nk, unit, w);
+  const int b = unit / p.kvh, kh = unit % p.kvh;
   const int part = w % bk.nk, k0 = w / bk.nk * 128;   // the first keys of a causal call have the longest columns
   const int len = length_of(p, b), pre = p.prefix ? p.prefix[b] : 0, shift = len - p.tq;
   const int key = k0 + wid * 32 + (lane & 31);
@@ -289,7 +287,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
   const int nt = max(0, t1 - t0), steps = nt * p.grp;
   const int each = (steps + bk.nk - 1) / bk.nk, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
 
-  Stage<T, DP, 64> qs, ds;
+  Stage<T, DP> qs, ds;
+  qs.init(p.ldq, p.d);
+  ds.init(p.lddo, p.d);
   float cn_next = 0.0f, cd_next = 0.0f;
   int id_next = -1, blind = 0;
   int hg_next = nt ? i0 / nt : 0, t_next = nt ? t0 + i0 % nt : 0, put_row0 = 0;
@@ -297,8 +297,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
   auto fetch = [&]() __attribute__((always_inline)) {   // the next (query head, tile) of the sweep
     const int h = kh * p.grp + hg_next, r0 = t_next * 64, last = min(63, p.tq - 1 - r0);
     const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h;
-    qs.load((const T*)p.q + trow * p.ldq + h * p.d, p.ldq, p.d, last);
-    ds.load((const T*)p.dout + trow * p.lddo + h * p.d, p.lddo, p.d, last);
+    qs.load((const T*)p.q + trow * p.ldq + h * p.d, p.ldq, last);
+    ds.load((const T*)p.dout + trow * p.lddo + h * p.d, p.lddo, last);
     put_row0 = r0;
     put_at = head * p.tq + r0;
     if (threadIdx.x < 64) {
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
     const int pos0 = t * 64 + shift;   // position of the tile's first row
     bool partial = __any(from > pos0);
     if (p.doc_q) partial |= __any(ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
-    const float slope = p.slopes ? p.slopes[kh * p.grp + hg] * kLog2e : 0.0f;
+    const float slope = SHAPED && p.slopes ? p.slopes[kh * p.grp + hg] * kLog2e : 0.0f;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       f32x16 s = {}, dp;
@@ -369,26 +369,29 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
         s = mfma(*reinterpret_cast<const v8*>(qt + 32 * qb * DP + qoff[c]), kf[c], s);
         dp = mfma(*reinterpret_cast<const v8*>(dt + 32 * qb * DP + qoff[c]), vf[c], dp);
       }
-      if (p.cap2 != 0.0f) {
+      if constexpr (SHAPED) {
+        if (p.cap2 != 0.0f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float g;
-          s[r] = cap_score(p, s[r], &g);
-          dp[r] *= g;
+          for (int r = 0; r < 16; ++r) {
+            float g;
+            s[r] = cap_score(p, s[r], &g);
+            dp[r] *= g;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= p.scale * kLog2e;
         }
-      }
-      if (p.slopes) {
-        const float mul = p.cap2 != 0.0f ? 1.0f : p.scale * kLog2e;
-        const float dist = (float)(pos0 + 4 * hh - key);
+        if (p.slopes) {
+          const float dist = (float)(pos0 + 4 * hh - key);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(-slope, fabsf(dist + (float)(32 * qb + (r & 3) + 8 * (r >> 2))), s[r] * mul);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(dist + (float)(32 * qb + (r & 3) + 8 * (r >> 2))), s[r]);
+        }
       }
       const float fs = is_half<T> ? f * 6.103515625e-05f : 1.0f;   // 2^-14
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float up = is_half<T> ? kPShift : 0.0f;
-        s[r] = exp2_raw(fmaf(s[r], p.mul, nl[r >> 2][r & 3] + up));
+        s[r] = exp2_raw(fmaf(s[r], SHAPED ? 1.0f : p.mul, nl[r >> 2][r & 3] + up));
         dp[r] *= is_half<T> ? s[r] * fs : s[r];
       }
       if (partial) {
@@ -487,15 +490,20 @@ long part_bytes(const dc_attn_desc* d) {
 }
 long bwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d); }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SHAPED>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
-  hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(xcd_grid((long)c.nb * c.heads * ((c.tq + 127) / 128))), dim3(256), 0, st, c, bk);
-  hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(xcd_grid((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)), dim3(256), 0, st, c,
-                     bk);
+  hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.heads * ((c.tq + 127) / 128))), dim3(256), 0,
+                     st, c, bk);
+  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)), dim3(256), 0,
+                     st, c, bk);
   if (bk.nk > 1) {
     const long n = 2L * c.nb * c.tk * c.kvh * (DP / 4);
     hipLaunchKernelGGL((dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, c, bk);
   }
+}
+template <typename T, int DP>
+void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
+  c.cap2 != 0.0f || c.slopes ? launch_bwd<T, DP, true>(c, bk, st) : launch_bwd<T, DP, false>(c, bk, st);
 }
 
 }  // namespace

@@ -3,11 +3,12 @@
 //
 // Scores are held transposed (S^T = K Q^T, a query to a lane), so the running maximum and sum of a row stay in the lane and
 // P feeds O^T += V^T P^T straight from the accumulator.  Two kernels share that product:
-//   fwd_kernel    128 query rows of one head to a block; the keys' tiles pass through LDS, the next one on its way to registers.
+//   fwd_kernel    128 query rows of one head to a block; tiles of 64 keys pass through LDS, two of them on their way.
 //   token_kernel  few query rows: all rows of a key head's query heads (up to 32) to a wave, each wave its own 32 keys at a time,
 //                 keys read straight into fragments.  It reads every key and value once, whatever the group.
 // Where rows are few the keys are split over blocks; each writes (m, l, O) in 32 bits and join_kernel adds them in split order.
 #include "attn_mask.h"
+#include <type_traits>
 
 namespace dcm {
 namespace {
@@ -124,122 +125,66 @@ __device__ __forceinline__ void put_part(const Split& sp, const Row<T, DP>& s, f
   if (hh == 0) *reinterpret_cast<float2*>(sp.ml + (row * sp.n + part) * 2) = make_float2(s.m, l);
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void fwd_kernel(Call p, Split sp) {
+// A step: tile i has landed (waited for, barrier), S, softmax, P V; then tile i + 2 is sent to the buffer that tile i - 1 left.  The
+// transposed reads carry no alias information, so the compiler waits for every load into LDS before them: sent any earlier, a tile
+// would be waited for at once.  128 columns hold two tiles alone (three would leave one block to a CU): there tile i + 1 is sent when
+// the step begins, and the reads are waited for in blocks of their own (tr_frags).
+template <typename T, int DP, bool SHAPED>
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Split sp) {
   typedef typename Vec<T>::v8 v8;
-  constexpr int TILE = 64 * DP;
-  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
-  __shared__ int ids[2][64];
-  __shared__ int range[4];
-  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
-  const int nqb = (p.tq + 127) / 128, per_head = nqb * p.grp * sp.n, total = p.nb * p.kvh * per_head;
-  int w = xcd_work(total);
-  if (w >= total) return;
-  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
-  w %= per_head;
-  const int h = kh * p.grp + w % p.grp;
-  w /= p.grp;
-  const int part = w % sp.n, qb = nqb - 1 - w / sp.n;   // the longest rows of a causal call first
-
-  const int len = length_of(p, b), q0 = qb * 128, qi = q0 + wid * 32 + (lane & 31);
-  const bool live = qi < p.tq;
-  const int pos = qi + len - p.tq;
-  const int pre = p.prefix ? p.prefix[b] : 0;
-  const T* qrow = (const T*)p.q + ((long)b * p.tq + qi) * p.ldq + h * p.d;
+  constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
+  typedef KeyRing<T, DP, S> Ring;
+  __shared__ typename Ring::Lds lds;
+  __shared__ int range[5];
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
+  QueryBlock q;
+  q.init(p, sp.n);
+  const T* qrow = (const T*)p.q + ((long)q.b * p.tq + q.qi) * p.ldq + q.h * p.d;
   v8 qf[DP / 16];
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, live && 16 * s + 8 * hh < p.d);
-  // the lane's query sees the keys below lim (of its document)
-  int lim = p.causal ? min(len, max(pos + 1, pre)) : len;
-  const int mine = p.doc_q ? (live ? p.doc_q[(long)b * p.tq + qi] : -1) : 0;
-  if (mine < 0) lim = 0;
-  // tiles that some query of the block sees, in a range
-  if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
-  __syncthreads();
-  atomicMax(&range[1], live ? lim : 0);
-  if (p.doc_q && live && mine >= 0) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
-  __syncthreads();
-  int t0 = 0, t1 = (range[1] + 63) / 64;
-  bool holes = false;
-  if (p.doc_q) {
-    const int nt = (p.tk + 63) / 64, least = range[2], most = range[3];
-    const int4* sum = p.sum_k + (long)b * nt;
-    int first = 0x7fffffff, last = -1, none = 0;
-    for (int t = threadIdx.x; t < t1; t += 256) {
-      const int4 s = sum[t];
-      if (s.y >= least && s.x <= most) { first = min(first, t); last = t; }
-      none |= s.z;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) { range[1] = 0; range[2] = 0; }
-    __syncthreads();
-    if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
-    if (none) atomicOr(&range[2], 1);
-    __syncthreads();
-    t0 = min(range[0], range[1]);
-    t1 = range[1];
-    holes = range[2];
-  }
+  for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, q.live && 16 * s + 8 * hh < p.d);
+  int t0, t1;
+  q.tiles(p, q.live, range, t0, t1);
   if (sp.n > 1) {
     const int each = (t1 - t0 + sp.n - 1) / sp.n;
-    t0 = min(t1, t0 + part * each);
+    t0 = min(t1, t0 + q.part * each);
     t1 = min(t1, t0 + each);
   }
-
-  const T* kb = (const T*)p.k + (long)b * p.tk * p.ldk + kh * p.d;
-  const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
-  const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
-  Stage<T, DP, 64> ks, vs;
-  int id_next = -1;
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int r0 = t * 64, last = len - 1 - r0;
-    ks.load(kb + (long)r0 * p.ldk, p.ldk, p.d, min(last, 63));
-    vs.load(vb + (long)r0 * p.ldv, p.ldv, p.d, min(last, 63));
-    if (kid && threadIdx.x < 64) id_next = kid[min(r0 + (int)threadIdx.x, len - 1)];
-  };
-  auto put = [&](int t, int buf) __attribute__((always_inline)) {
-    const int r0 = t * 64, last = len - 1 - r0;
-    if (last >= 63 && p.d == DP && !holes) {
-      ks.store(tiles[buf]);
-      vs.store(tiles[buf] + TILE);
-    } else {
-      auto keep = [&](int r) { return !holes || (r <= last && kid[r0 + r] >= 0); };
-      ks.store_some(tiles[buf], p.d, last, keep);
-      vs.store_some(tiles[buf] + TILE, p.d, last, keep);
-    }
-    if (kid && threadIdx.x < 64) ids[buf][threadIdx.x] = id_next;
-  };
-
+  Ring ring;
+  ring.init(p, q);
   Row<T, DP> st;
   st.init();
-  const bool shaped = p.cap2 != 0.0f || p.slopes;
-  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
-  TrAt va[DP / 32];
+  TrAt va[2];
+  TrAt4 va4;
+  if constexpr (DP == 128) va4.init(lds.tiles[0], lane);
+  else
 #pragma unroll
-  for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
+    for (int n = 0; n < 2; ++n) va[n] = tr_at<DP>(32 * n, lane);
+  const int seen_by_all = __builtin_amdgcn_readfirstlane(wave_min_i(q.live ? q.lim : 0x7fffffff));   // keys that no row has to mask
 
-  if (t0 < t1) {
-    fetch(t0);
-    put(t0, 0);
-  }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (t + 1 < t1) fetch(t + 1);
-    const T* kt = tiles[buf];
+  vm_wait<0>();   // (the counts below are of tiles alone)
+  if (t0 < t1) ring.load(p, lds, t0, 0);
+  if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
+  auto step = [&](int t, auto B) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B)::value;
+    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
+    else vm_wait<0>();
+    tile_barrier();
+    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
+    const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
     f32x16 s[2];
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       s[kb2] = f32x16{};
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c)
-        s[kb2] = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s[kb2]);
+      for (int c = 0; c < DP / 16; ++c) s[kb2] = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s[kb2]);
     }
-    if (shaped) {
+    if constexpr (SHAPED) {
       if (p.cap2 != 0.0f) {
 #pragma unroll
         for (int kb2 = 0; kb2 < 2; ++kb2)
@@ -252,7 +197,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Call p, Split sp) {
           for (int r = 0; r < 16; ++r) s[kb2][r] *= p.scale * kLog2e;
       }
       if (p.slopes) {
-        const float dist = (float)(pos - t * 64 - 4 * hh);
+        const float dist = (float)(q.pos - t * 64 - 4 * hh);
 #pragma unroll
         for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
@@ -260,52 +205,67 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Call p, Split sp) {
             s[kb2][r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[kb2][r]);
       }
     }
-    bool partial = __any(live && lim < t * 64 + 64);
-    if (kid) partial |= __any(live && ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
+    const int* id = lds.ids[buf];
+    bool partial = seen_by_all < t * 64 + 64;
+    if (ring.kid) partial |= __any(q.live && id[0] != q.mine) || __any(id[lane] != id[0]);
     if (partial) {
+      asm volatile("" ::: "memory");   // a branch, not selects in every tile
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int key = 32 * kb2 + 8 * g + 4 * hh;
-          int4 id = make_int4(0, 0, 0, 0);
-          if (kid) id = *reinterpret_cast<const int4*>(&ids[buf][key]);
-          const int id4[4] = {id.x, id.y, id.z, id.w};
+          int4 i4 = make_int4(0, 0, 0, 0);
+          if (ring.kid) i4 = *reinterpret_cast<const int4*>(&id[key]);
+          const int id4[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t * 64 + key + e >= lim || (kid && id4[e] != mine)) s[kb2][4 * g + e] = -INFINITY;
+            if (t * 64 + key + e >= q.lim || (ring.kid && id4[e] != q.mine)) s[kb2][4 * g + e] = -INFINITY;
         }
     }
-    st.weigh(s, p.mul);
+    st.weigh(s, SHAPED ? 1.0f : p.mul);
+    auto add = [&](auto C) __attribute__((always_inline)) {
+      constexpr int c = decltype(C)::value;
+      v8 f[DP / 32];
+      if constexpr (DP == 128) tr_frags<T, (buf * 2 * TILE + TILE + 16 * c * DP) * 2>(va4, f);
+      else
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+        for (int n = 0; n < 2; ++n) f[n] = tr_frag(vt + 16 * c * DP, va[n]);
       const v8 pf = acc_frag<T>(s[c >> 1], c & 1);
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n) st.o[n] = mfma(tr_frag(vt + 16 * c * DP, va[n]), pf, st.o[n]);
-    }
-    if (t + 1 < t1) put(t + 1, buf ^ 1);
-    __syncthreads();
+      for (int n = 0; n < DP / 32; ++n) st.o[n] = mfma(f[n], pf, st.o[n]);
+    };
+    add(std::integral_constant<int, 0>{});
+    add(std::integral_constant<int, 1>{});
+    add(std::integral_constant<int, 2>{});
+    add(std::integral_constant<int, 3>{});
+    if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
+  };
+  for (int t = t0; t < t1; t += S) {
+    step(t, std::integral_constant<int, 0>{});
+    if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
+    if constexpr (S == 3)
+      if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{});
   }
   const float l = pair_sum(st.l);
-  if (!live) return;
-  const long row = ((long)b * p.heads + h) * p.tq + qi;
-  if (sp.n > 1) put_part<T, DP>(sp, st, l, row, part, hh);
-  else put_row<T, DP>(p, st, l, row, (long)b * p.tq + qi, h, hh);
+  if (!q.live) return;
+  const long row = ((long)q.b * p.heads + q.h) * p.tq + q.qi;
+  if (sp.n > 1) put_part<T, DP>(sp, st, l, row, q.part, hh);
+  else put_row<T, DP>(p, st, l, row, (long)q.b * p.tq + q.qi, q.h, hh);
 }
 
 // One block: up to 32 of the rows (query, head of the group) of one key head, `sp.tiles` steps of 4 x 32 keys.
-template <typename T, int DP>
+template <typename T, int DP, bool SHAPED>
 __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   typedef typename Vec<T>::v8 v8;
   constexpr int SUB = 32 * DP, NV = SUB / 8 / 64, CH = DP / 8, RED = (2 + DP / 2) * 64;
   constexpr int BYTES = 4 * SUB * 2 > 3 * RED * 4 ? 4 * SUB * 2 : 3 * RED * 4;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
-  const int rows = p.tq * p.grp, nrb = (rows + 31) / 32, per_head = nrb * sp.n, total = p.nb * p.kvh * per_head;
-  int w = xcd_work(total);
-  if (w >= total) return;
-  const int b = w / per_head / p.kvh, kh = w / per_head % p.kvh;
-  w %= per_head;
+  const int rows = p.tq * p.grp, nrb = (rows + 31) / 32;
+  int unit, w;
+  unit_of(p.nb * p.kvh, nrb * sp.n, unit, w);
+  const int b = unit / p.kvh, kh = unit % p.kvh;
   const int rb = w % nrb, part = w / nrb;
   const int r = rb * 32 + (lane & 31);
   const bool live = r < rows;
@@ -323,8 +283,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
   const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
   T* vt = reinterpret_cast<T*>(smem) + wid * SUB;
-  const bool shaped = p.cap2 != 0.0f || p.slopes;
-  const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
   TrAt va[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
@@ -370,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) s[0] = mfma(kf[c], qf[c], s[0]);   // qf is zero where the columns end
     if (u + 4 < u1) fetch(u + 4);
-    if (shaped) {
+    if constexpr (SHAPED) {
       if (p.cap2 != 0.0f) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[0][e] = cap_score(p, s[0][e], nullptr);
@@ -392,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
         if (u * 32 + key >= lim || other) s[0][e] = -INFINITY;
       }
     }
-    st.weigh(s, p.mul);
+    st.weigh(s, SHAPED ? 1.0f : p.mul);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const v8 pf = acc_frag<T>(s[0], c);
@@ -464,8 +423,9 @@ constexpr int kMaxSplit = 64;
 // Few query rows (at most 32 in a sequence, a quarter of fwd_kernel's block): token_kernel.
 bool few_rows(int tq) { return tq <= 32; }
 
-// How the keys are split.  Enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or more for
-// few rows (the steps a block has cover its start and its merge) and 8 tiles of 64 for many.
+// How the keys are split.  Few rows: enough blocks to give every CU four where the keys allow it, each with 4
+// steps of 128 keys or more (the steps a block has cover its start and its merge).  Many rows: a block to every CU, each with 16 tiles
+// of 64 keys or more.
 Split split_of(const dc_attn_desc* d) {
   Split s{1, 0, nullptr, nullptr};
   const long grp = d->heads / d->kv_heads;
@@ -477,7 +437,7 @@ Split split_of(const dc_attn_desc* d) {
     s.n = (int)((steps + s.tiles - 1) / s.tiles);
   } else {
     const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
-    if (blocks < 256) s.n = (int)min(min((512 + blocks - 1) / blocks, max(tiles / 8, 1L)), (long)kMaxSplit);
+    if (blocks < 128) s.n = (int)min(min((256 + blocks - 1) / blocks, max(tiles / 16, 1L)), (long)kMaxSplit);
   }
   return s;
 }
@@ -487,17 +447,21 @@ long part_floats(const dc_attn_desc* d, const Split& s) {
   return (long)d->nb * d->heads * d->tq * s.n * ((d->d > 64 ? 128 : 64) + 2);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SHAPED>
 void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
   if (few_rows(d->tq)) {
     const long blocks = (long)c.nb * c.kvh * ((c.tq * c.grp + 31) / 32) * s.n;
-    hipLaunchKernelGGL((token_kernel<T, DP>), dim3(xcd_grid(blocks)), dim3(256), 0, st, c, s);
+    hipLaunchKernelGGL((token_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   } else {
     const long blocks = (long)c.nb * c.heads * ((c.tq + 127) / 128) * s.n;
-    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(xcd_grid(blocks)), dim3(256), 0, st, c, s);
+    hipLaunchKernelGGL((fwd_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   }
   const long rows = (long)c.nb * c.heads * c.tq;
   if (s.n > 1) hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, c, s, rows);
+}
+template <typename T, int DP>
+void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
+  c.cap2 != 0.0f || c.slopes ? launch_fwd<T, DP, true>(c, d, s, st) : launch_fwd<T, DP, false>(c, d, s, st);
 }
 
 }  // namespace
@@ -533,12 +497,13 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
     return DC_ERR_ARG;
   const int hq = d->heads * d->d, hk = d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
+  if (d->ldk > (1 << 23) || d->ldv > (1 << 23)) return DC_ERR_ARG;   // 128 rows within 32 bits
   if (d->ldq % 8 || d->ldk % 8 || d->ldv % 8 || d->ldo % 8) return DC_ERR_ALIGN;
   const uintptr_t at = (uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o;
   if (at & 15) return DC_ERR_ALIGN;
   if (backward) {
     if (!d->dout || !d->dq || !d->dk || !d->dv) return DC_ERR_ARG;
-    if (d->lddo < hq || d->lddq < hq || d->lddk < hk || d->lddv < hk) return DC_ERR_ARG;
+    if (d->ldq > (1 << 23) || d->lddo > (1 << 23) || d->lddo < hq || d->lddq < hq || d->lddk < hk || d->lddv < hk) return DC_ERR_ARG;
     if (d->lddo % 8 || d->lddq % 8 || d->lddk % 8 || d->lddv % 8) return DC_ERR_ALIGN;
     if (((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) & 15) return DC_ERR_ALIGN;
   }
