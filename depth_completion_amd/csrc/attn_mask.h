@@ -39,7 +39,7 @@ struct Call {
   const float* slopes;
   int causal;
   const int *prefix, *kv_len, *doc_q, *doc_k;
-  const int4 *sum_q, *sum_k;   // per 64 rows: least and largest document, whether a row is in none
+  const int4 *sum_q, *sum_k;   // per 64 rows: least and largest document, whether a row is in none (NULL: short rows, no documents)
 };
 
 // Scores of a call with a cap or a distance bias, in units of log2: s = cap2 tanh(scale s / cap), then - slope |pos - key|.
@@ -130,13 +130,13 @@ __device__ __forceinline__ typename Vec<T>::v8 load8_or_0(const T* p, bool ok) {
   return v;
 }
 
-// 64 x DP elements into an LDS tile by 256 threads, straight from memory (16 bytes a lane, no registers between).  A lane's offsets
+// 64 x DP elements into an LDS tile by NT threads, straight from memory (16 bytes a lane, no registers between).  A lane's offsets
 // are the same for every tile; the tile's first row is in the scalar base (64 bits, so a long cache needs no wide offsets).  Rows
 // behind `last`, rows that `keep` leaves out and columns from d on take an offset outside the descriptor and arrive as zeros:
 // nothing that lies in a masked place is ever multiplied.
-template <typename T, int DP>
+template <typename T, int DP, int NT = 256>
 struct Dma {
-  static constexpr int CH = DP / 8, N = 64 * CH / 256, STEP = 256 / CH;
+  static constexpr int CH = DP / 8, N = 64 * CH / NT, STEP = NT / CH;
   static constexpr unsigned OUT = 0x80000000u;
   unsigned off[N];
   int row, wave;
@@ -156,7 +156,7 @@ struct Dma {
   }
   __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t r, T* tile, int i, unsigned o) const {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the builtin exists in the device pass alone)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DC_LDS char*)(tile + (64 * wave + 256 * i) * 8), 16, o, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DC_LDS char*)(tile + (64 * wave + NT * i) * 8), 16, o, 0, 0, 0);
 #endif
   }
   __device__ __forceinline__ void load(const T* base, T* tile, int last) const {
@@ -257,17 +257,17 @@ struct QueryBlock {
     mine = p.doc_q ? (live ? p.doc_q[(long)b * p.tq + qi] : -1) : 0;
     if (mine < 0) lim = 0;
   }
-  // The 64-key tiles [t0, t1) in which some row with `sees` may see a key.
-  __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1) const {
-    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; range[4] = 0; }
+  // The 64-key tiles [t0, t1) in which some row with `sees` may see a key; holes: some key of theirs is (or may be) in no document.
+  __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1, bool& holes) const {
+    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; range[4] = 0; range[5] = 0; }
     __syncthreads();
     const int most = wave_max_i(sees ? lim : 0);
     if ((threadIdx.x & 63) == 0) atomicMax(&range[1], most);
-    if (p.doc_q && sees && mine >= 0) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
+    if (p.sum_k && sees && mine >= 0) { atomicMin(&range[2], mine); atomicMax(&range[3], mine); }
     __syncthreads();
     t0 = 0;
     t1 = (range[1] + 63) / 64;
-    if (p.doc_q) {
+    if (p.sum_k) {
       const int nt = (p.tk + 63) / 64, least = range[2], largest = range[3];
       const int4* sum = p.sum_k + (long)b * nt;
       int first = 0x7fffffff, last = -1;
@@ -279,7 +279,12 @@ struct QueryBlock {
       __syncthreads();
       t1 = range[4];
       t0 = min(range[0], t1);
+      int none = 0;
+      for (int t = t0 + threadIdx.x; t < t1; t += blockDim.x) none |= sum[t].z;
+      if (none) range[5] = 1;
+      __syncthreads();
     }
+    holes = p.doc_q && (!p.sum_k || __builtin_amdgcn_readfirstlane(range[5]));
     t0 = __builtin_amdgcn_readfirstlane(t0);
     t1 = __builtin_amdgcn_readfirstlane(t1);
   }
@@ -298,20 +303,23 @@ struct KeyRing {
   const int* kid;
   const int4* sum;
   int len;
-  __device__ __forceinline__ void init(const Call& p, const QueryBlock& q) {
+  bool holes;
+  __device__ __forceinline__ void init(const Call& p, const QueryBlock& q, bool some_holes) {
+    holes = some_holes;
     k.init(p.ldk, p.d);
     v.init(p.ldv, p.d);
     kb = (const T*)p.k + (long)q.b * p.tk * p.ldk + q.kh * p.d;
     vb = (const T*)p.v + (long)q.b * p.tk * p.ldv + q.kh * p.d;
     kid = p.doc_q ? p.doc_k + (long)q.b * p.tk : nullptr;
-    sum = p.doc_q ? p.sum_k + (long)q.b * ((p.tk + 63) / 64) : nullptr;
+    sum = p.sum_k ? p.sum_k + (long)q.b * ((p.tk + 63) / 64) : nullptr;
     len = q.len;
   }
   // tile t on its way (each wave issues 2 Dma::N operations or more)
   __device__ __forceinline__ void load(const Call& p, Lds& lds, int t, int buf) const {
     const int r0 = t * 64, last = len - 1 - r0;
     const T *ka = kb + (long)r0 * p.ldk, *va = vb + (long)r0 * p.ldv;
-    if (kid && sum[t].z) {   // a key in no document: its row may hold anything
+    // a key in no document: its row may hold anything (asked for each tile, the answer would be waited for in each)
+    if (holes && (!sum || sum[t].z)) {
       auto keep = [&](int r) __attribute__((always_inline)) { return kid[min(r0 + r, len - 1)] >= 0; };
       k.load_some(ka, lds.tiles[buf], last, keep);
       v.load_some(va, lds.tiles[buf] + TILE, last, keep);
@@ -325,7 +333,7 @@ struct KeyRing {
 
 // Host side: what both directions share (attn_mask_fwd.hip).
 int make_call(const dc_attn_desc* d, Call& c, bool backward);
-long long summary_bytes(const dc_attn_desc* d);
-void launch_summaries(const dc_attn_desc* d, Call& c, char* ws, hipStream_t st);
+long long summary_bytes(const dc_attn_desc* d, bool backward);
+void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st);
 
 }  // namespace dcm

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
   typedef KeyRing<T, DP, S> Ring;
   __shared__ typename Ring::Lds lds;
-  __shared__ int range[5];
+  __shared__ int range[6];
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   QueryBlock q;
   q.init(p, 1);
@@ -72,10 +72,11 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
   if (lane == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
   const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
   int t0, t1;
-  q.tiles(p, sees, range, t0, t1);
+  bool holes;
+  q.tiles(p, sees, range, t0, t1, holes);
 
   Ring ring;
-  ring.init(p, q);
+  ring.init(p, q, holes);
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
@@ -190,68 +191,46 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
     }
 }
 
-// 64 x DP elements by 256 threads, through registers, with the zeros that Dma leaves.
-template <typename T, int DP>
-struct Stage {
-  static constexpr int CH = DP / 8, N = 64 * CH / 256, STEP = 256 / CH;
-  uint4 reg[N];
-  unsigned first, step;   // bytes
-  int row, chunk;
-  __device__ __forceinline__ void init(int ld, int d) {
-    row = threadIdx.x / CH;
-    chunk = threadIdx.x % CH;
-    first = ((unsigned)row * ld + (chunk * 8 < d ? chunk * 8 : 0)) * sizeof(T);
-    step = (unsigned)STEP * ld * sizeof(T);
-  }
-  __device__ __forceinline__ void load(const T* base, int ld, int last) {
-    const char* at = reinterpret_cast<const char*>(base);
-    const unsigned back = (unsigned)ld * sizeof(T);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      reg[i] = *reinterpret_cast<const uint4*>(at + (first + i * step - back * (unsigned)max(row + STEP * i - last, 0)));
-  }
-  __device__ __forceinline__ void store(T* tile) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(tile + tile_at<DP>(row + STEP * i, chunk)) = reg[i];
-  }
-  template <typename F>
-  __device__ __forceinline__ void store_some(T* tile, int d, int last, F&& keep) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (chunk * 8 >= d || row + STEP * i > last || !keep(row + STEP * i)) reg[i] = make_uint4(0, 0, 0, 0);
-    store(tile);
-  }
-};
-
 // the factor of dS in dK for a key head: by the largest |dO| of its query heads, the same in every block that needs it
 __device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int b, int kh, float* scratch) {
   const int2* r = bk.rows32 + ((long)b * p.heads + kh * p.grp) * bk.n32;
   float most = 0.0f;
-  for (int i = threadIdx.x; i < p.grp * bk.n32; i += 256) most = fmaxf(most, __int_as_float(r[i].y));
+  for (int i = threadIdx.x; i < p.grp * bk.n32; i += blockDim.x) most = fmaxf(most, __int_as_float(r[i].y));
   most = wave_max(most);
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = most;
   __syncthreads();
-  return near_sixteenth(fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3])));
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) most = fmaxf(most, scratch[i]);
+  return near_sixteenth(most);
 }
 
 constexpr float kPShift = 14.0f;   // fp16: P in dV is 2^14 times as large
 
+// 128 keys to a block, held in registers; tiles of 64 query rows pass through LDS, three of them in turn.
+// 64 columns: a wave has 32 keys with both of their sums.  128 columns: a pair of waves has 32 keys.  Of a tile each takes 32 rows to
+// P and dS; the first then sums dV and needs P of all rows, the second dK and dS of all: they exchange the half that the other sums
+// (2 KB each way), and a wave carries one sum, not two, which is what lets two waves share a SIMD (one wave with both took 416
+// registers and 24 % of the matrix units' time: 4097 x 32/8 heads causal 511 us for 398; at 64 columns, where both fit, pairs lose:
+// 8 x 4096 x 16 heads with dQ 2020 us for 2824).
 template <typename T, int DP, bool SHAPED>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back bk) {
+__global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
-  constexpr int TILE = 64 * DP;
-  __shared__ __attribute__((aligned(16))) T tiles[2][2 * TILE];
-  __shared__ __attribute__((aligned(16))) float cn[2][64], cd[2][64];
-  __shared__ __attribute__((aligned(16))) int ids[2][64];
-  __shared__ int range[4];
-  __shared__ float scratch[4];
-  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
+  constexpr bool PAIR = DP == 128;
+  constexpr int NT = PAIR ? 512 : 256;
+  typedef Dma<T, DP, NT> D;
+  constexpr int TILE = 64 * DP, OPS = 2 * D::N;
+  __shared__ __attribute__((aligned(16))) T tiles[3][2 * TILE];   // Q, dO
+  __shared__ __attribute__((aligned(16))) float cn[3][64], cd[3][64];
+  __shared__ __attribute__((aligned(16))) int ids[3][64];
+  __shared__ __attribute__((aligned(16))) T swap[PAIR ? 8 : 1][2][64 * 8];
+  __shared__ int range[4], blind_rows;
+  __shared__ float scratch[8];
+  const int lane = threadIdx.x & 63, hh = lane >> 5, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), second = PAIR ? wid & 1 : 0;
   int unit, w;
   unit_of(p.nb * p.kvh, (p.tk + 127) / 128 * bk.nk, unit, w);
   const int b = unit / p.kvh, kh = unit % p.kvh;
   const int part = w % bk.nk, k0 = w / bk.nk * 128;   // the first keys of a causal call have the longest columns
   const int len = length_of(p, b), pre = p.prefix ? p.prefix[b] : 0, shift = len - p.tq;
-  const int key = k0 + wid * 32 + (lane & 31);
+  const int key = k0 + (PAIR ? wid >> 1 : wid) * 32 + (lane & 31);
   const int mine = p.doc_q ? (key < len ? p.doc_k[(long)b * p.tk + key] : -1) : 0;
   const bool ok = key < len && mine >= 0;
   v8 kf[DP / 16], vf[DP / 16];
@@ -264,10 +243,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
   const float f = is_half<T> ? head_factor(p, bk, b, kh, scratch) : 1.0f;
   // the lane's key is seen from position `from` on
   const int from = !ok ? 0x7fffffff : p.causal && key >= pre ? key : -0x7fffffff;
+  const int from_last = __builtin_amdgcn_readfirstlane(wave_max_i(from));
   int t0 = 0, t1 = (p.tq + 63) / 64;
   if (p.causal && k0 >= pre) t0 = max(0, k0 - shift) / 64;
   if (k0 >= len) t1 = 0;
-  if (p.doc_q) {
+  if (p.sum_q) {
     const int nt = (p.tq + 63) / 64;
     if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; }
     __syncthreads();
@@ -275,99 +255,93 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
     __syncthreads();
     const int least = range[2], largest = range[3];
     int first = 0x7fffffff, last = -1;
-    for (int t = t0 + threadIdx.x; t < t1; t += 256) {
+    for (int t = t0 + threadIdx.x; t < t1; t += NT) {
       const int4 s = p.sum_q[(long)b * nt + t];
       if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
     }
     if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[1], last + 1); }
     __syncthreads();
-    t0 = range[0];
-    t1 = range[1];
+    t0 = __builtin_amdgcn_readfirstlane(range[0]);
+    t1 = __builtin_amdgcn_readfirstlane(range[1]);
   }
   const int nt = max(0, t1 - t0), steps = nt * p.grp;
-  const int each = (steps + bk.nk - 1) / bk.nk, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
-
-  Stage<T, DP> qs, ds;
-  qs.init(p.ldq, p.d);
-  ds.init(p.lddo, p.d);
-  float cn_next = 0.0f, cd_next = 0.0f;
-  int id_next = -1, blind = 0;
-  int hg_next = nt ? i0 / nt : 0, t_next = nt ? t0 + i0 % nt : 0, put_row0 = 0;
-  long put_at = 0;
-  auto fetch = [&]() __attribute__((always_inline)) {   // the next (query head, tile) of the sweep
-    const int h = kh * p.grp + hg_next, r0 = t_next * 64, last = min(63, p.tq - 1 - r0);
-    const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h;
-    qs.load((const T*)p.q + trow * p.ldq + h * p.d, p.ldq, last);
-    ds.load((const T*)p.dout + trow * p.lddo + h * p.d, p.lddo, last);
-    put_row0 = r0;
-    put_at = head * p.tq + r0;
-    if (threadIdx.x < 64) {
-      const int r = min((int)threadIdx.x, last);
-      cn_next = bk.nlse[put_at + r];
-      cd_next = bk.ndel[put_at + r];
-      if (p.doc_q) id_next = p.doc_q[trow + r];
-    }
-    const int2* fl = bk.rows32 + head * bk.n32 + r0 / 32;
-    blind = fl[0].x | (r0 + 32 < p.tq ? fl[1].x : 0);
-    if (++t_next == t1) { t_next = t0; ++hg_next; }
-  };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    const int last = p.tq - 1 - put_row0;
-    if (last >= 63 && p.d == DP && !blind) {
-      qs.store(tiles[buf]);
-      ds.store(tiles[buf] + TILE);
-    } else {
-      auto keep = [&](int r) { return !blind || (r <= last && bk.nlse[put_at + r] != -INFINITY); };
-      qs.store_some(tiles[buf], p.d, last, keep);
-      ds.store_some(tiles[buf] + TILE, p.d, last, keep);
-    }
-    if (threadIdx.x < 64) {
-      const bool in = (int)threadIdx.x <= last;
-      cn[buf][threadIdx.x] = in ? cn_next : -INFINITY;
-      cd[buf][threadIdx.x] = in ? cd_next : 0.0f;
-      ids[buf][threadIdx.x] = id_next;
-    }
-  };
-  f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int n = 0; n < DP / 32; ++n) { dk[n] = f32x16{}; dv[n] = f32x16{}; }
-  int qoff[DP / 16];
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) qoff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
-  TrAt ta[DP / 32];
-#pragma unroll
-  for (int n = 0; n < DP / 32; ++n) ta[n] = tr_at<DP>(32 * n, lane);
-  if (i0 < i1) {
-    fetch();
-    put(0);
+  // whether some row of the sweep sees no key (asked for each tile, the answer would be waited for in each)
+  if (threadIdx.x == 0) blind_rows = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < steps; i += NT) {
+    const int2* fl = bk.rows32 + ((long)b * p.heads + kh * p.grp + i / nt) * bk.n32 + (t0 + i % nt) * 2;
+    if (fl[0].x | fl[1].x) blind_rows = 1;
   }
   __syncthreads();
+  const bool blind = __builtin_amdgcn_readfirstlane(blind_rows);
+  const int each = (steps + bk.nk - 1) / bk.nk, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
+
+  D qs, ds;
+  qs.init(p.ldq, p.d);
+  ds.init(p.lddo, p.d);
+  int hg_next = nt ? i0 / nt : 0, t_next = nt ? t0 + i0 % nt : 0;
+  auto load = [&](int buf) __attribute__((always_inline)) {   // the next (query head, tile) of the sweep
+    const int h = kh * p.grp + hg_next, r0 = t_next * 64, last = p.tq - 1 - r0;
+    const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h, at = head * p.tq + r0;
+    const T *qa = (const T*)p.q + trow * p.ldq + h * p.d, *da = (const T*)p.dout + trow * p.lddo + h * p.d;
+    const int2* fl = bk.rows32 + head * bk.n32 + r0 / 32;
+    if (blind && (fl[0].x | fl[1].x)) {   // a row that sees no key: it may hold anything
+      auto keep = [&](int r) __attribute__((always_inline)) { return bk.nlse[at + min(r, last)] != -INFINITY; };
+      qs.load_some(qa, tiles[buf], last, keep);
+      ds.load_some(da, tiles[buf] + TILE, last, keep);
+    } else {
+      qs.load(qa, tiles[buf], last);
+      ds.load(da, tiles[buf] + TILE, last);
+    }
+    if (wid == 0) {
+      dma_words(bk.nlse + at, cn[buf], last);
+      dma_words(bk.ndel + at, cd[buf], last);
+      if (p.doc_q) dma_words(p.doc_q + trow, ids[buf], last);
+    }
+    if (++t_next == t1) { t_next = t0; ++hg_next; }
+  };
+  f32x16 dv[DP / 32], dk[PAIR ? 1 : DP / 32];   // (a pair has dv alone: dV in the first wave, dK in the second)
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) {
+    dv[n] = f32x16{};
+    if constexpr (!PAIR) dk[n] = f32x16{};
+  }
+  int qoff[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) qoff[s] = tile_at<DP>(lane & 31, 2 * s + hh) + 32 * second * DP;
+  TrAt ta[DP / 32];   // (of a pair: dO^T for the first wave, Q^T for the second)
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n) {
+    ta[n] = tr_at<DP>(32 * n, lane);
+    if (PAIR && !second) { ta[n].lo += TILE; ta[n].hi += TILE; }
+  }
+  vm_wait<0>();
+  if (i0 < i1) load(0);
+  if (i0 + 1 < i1) load(1);
   int hg = nt ? i0 / nt : 0, t = nt ? t0 + i0 % nt : 0;
-  for (int i = i0; i < i1; ++i) {
-    const int buf = (i - i0) & 1;
-    if (i + 1 < i1) fetch();
+  auto step = [&](int i, auto B) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B)::value;
+    if (i + 1 < i1) vm_wait<OPS>();
+    else vm_wait<0>();
+    tile_barrier();
     const T* qt = tiles[buf];
     const T* dt = qt + TILE;
-    const int pos0 = t * 64 + shift;   // position of the tile's first row
-    bool partial = __any(from > pos0);
-    if (p.doc_q) partial |= __any(ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
-    const float slope = SHAPED && p.slopes ? p.slopes[kh * p.grp + hg] * kLog2e : 0.0f;
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
+    // P and dS of 32 rows of the tile (a pair's: qoff is at the wave's own)
+    auto weights = [&](int at, v8 (&pf)[2], v8 (&sf)[2]) __attribute__((always_inline)) {
+      const int rows = at + 32 * second, row0 = rows + 4 * hh, pos0 = t * 64 + shift + row0;   // of the lane's first row
       f32x16 s = {}, dp;
       f32x4 nl[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int r = 32 * qb + 8 * g + 4 * hh;
-        nl[g] = *reinterpret_cast<const f32x4*>(&cn[buf][r]);
-        const f32x4 nd = *reinterpret_cast<const f32x4*>(&cd[buf][r]);
+        nl[g] = *reinterpret_cast<const f32x4*>(&cn[buf][row0 + 8 * g]);
+        const f32x4 nd = *reinterpret_cast<const f32x4*>(&cd[buf][row0 + 8 * g]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * g + e] = nd[e];
       }
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        s = mfma(*reinterpret_cast<const v8*>(qt + 32 * qb * DP + qoff[c]), kf[c], s);
-        dp = mfma(*reinterpret_cast<const v8*>(dt + 32 * qb * DP + qoff[c]), vf[c], dp);
+        s = mfma(*reinterpret_cast<const v8*>(qt + at * DP + qoff[c]), kf[c], s);
+        dp = mfma(*reinterpret_cast<const v8*>(dt + at * DP + qoff[c]), vf[c], dp);
       }
       if constexpr (SHAPED) {
         if (p.cap2 != 0.0f) {
@@ -382,9 +356,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
           for (int r = 0; r < 16; ++r) s[r] *= p.scale * kLog2e;
         }
         if (p.slopes) {
-          const float dist = (float)(pos0 + 4 * hh - key);
+          const float slope = p.slopes[kh * p.grp + hg] * kLog2e, dist = (float)(pos0 - key);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(dist + (float)(32 * qb + (r & 3) + 8 * (r >> 2))), s[r]);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(dist + (float)((r & 3) + 8 * (r >> 2))), s[r]);
         }
       }
       const float fs = is_half<T> ? f * 6.103515625e-05f : 1.0f;   // 2^-14
@@ -394,16 +368,18 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
         s[r] = exp2_raw(fmaf(s[r], SHAPED ? 1.0f : p.mul, nl[r >> 2][r & 3] + up));
         dp[r] *= is_half<T> ? s[r] * fs : s[r];
       }
+      bool partial = from_last > t * 64 + shift + rows;
+      if (p.doc_q) partial |= __any(ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
       if (partial) {
+        asm volatile("" ::: "memory");   // a branch, not selects in every tile
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int r = 32 * qb + 8 * g + 4 * hh;
           int4 id = make_int4(0, 0, 0, 0);
-          if (p.doc_q) id = *reinterpret_cast<const int4*>(&ids[buf][r]);
+          if (p.doc_q) id = *reinterpret_cast<const int4*>(&ids[buf][row0 + 8 * g]);
           const int id4[4] = {id.x, id.y, id.z, id.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (pos0 + r + e < from || (p.doc_q && id4[e] != mine)) {
+            if (pos0 + 8 * g + e < from || (p.doc_q && id4[e] != mine)) {
               s[4 * g + e] = 0.0f;
               dp[4 * g + e] = 0.0f;
             }
@@ -411,47 +387,80 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void dkv_kernel(Call p, Back
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const v8 pf = acc_frag<T>(s, c), sf = acc_frag<T>(dp, c);
+        pf[c] = acc_frag<T>(s, c);
+        sf[c] = acc_frag<T>(dp, c);
+      }
+    };
+    v8 pf[2], sf[2];
+    if constexpr (PAIR) {
+      weights(0, pf, sf);
+      v8 own[2], other[2];
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n) {
-          dv[n] = mfma(tr_frag(dt + (32 * qb + 16 * c) * DP, ta[n]), pf, dv[n]);
-          dk[n] = mfma(tr_frag(qt + (32 * qb + 16 * c) * DP, ta[n]), sf, dk[n]);
-        }
+      for (int c = 0; c < 2; ++c) {
+        own[c] = second ? sf[c] : pf[c];
+        *reinterpret_cast<v8*>(&swap[wid][c][lane * 8]) = second ? pf[c] : sf[c];
+      }
+      tile_barrier();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) other[c] = *reinterpret_cast<const v8*>(&swap[wid ^ 1][c][lane * 8]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const v8 mid = (c >> 1) == second ? own[c & 1] : other[c & 1];
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) dv[n] = mfma(tr_frag(qt + 16 * c * DP, ta[n]), mid, dv[n]);
+      }
+    } else {
+#pragma unroll
+      for (int rows = 0; rows < 64; rows += 32) {
+        weights(rows, pf, sf);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int n = 0; n < DP / 32; ++n) {
+            dv[n] = mfma(tr_frag(dt + (rows + 16 * c) * DP, ta[n]), pf[c], dv[n]);
+            dk[n] = mfma(tr_frag(qt + (rows + 16 * c) * DP, ta[n]), sf[c], dk[n]);
+          }
       }
     }
-    if (i + 1 < i1) put(buf ^ 1);
     if (++t == t1) { t = t0; ++hg; }
-    __syncthreads();
+    if (i + 2 < i1) load((buf + 2) % 3);
+  };
+  for (int i = i0; i < i1; i += 3) {
+    step(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
+    if (i + 2 < i1) step(i + 2, std::integral_constant<int, 2>{});
   }
   if (key >= p.tk) return;
-  const float kk = p.scale / f, kv = is_half<T> ? 6.103515625e-05f : 1.0f;
   const long krow = (long)b * p.tk + key;
-  float* pk = nullptr;
-  if (bk.nk > 1) pk = bk.part + (((long)part * 2 * p.nb * p.tk + krow) * p.kvh + kh) * DP;
-  const long other = (long)p.nb * p.tk * p.kvh * DP;
+  auto leave = [&](const f32x16 (&acc)[DP / 32], float k, int which, T* out) __attribute__((always_inline)) {   // which: 0 dK, 1 dV
+    float* pk = bk.nk > 1 ? bk.part + ((((long)part * 2 + which) * p.nb * p.tk + krow) * p.kvh + kh) * DP : nullptr;
 #pragma unroll
-  for (int n = 0; n < DP / 32; ++n)
+    for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int col = 32 * n + 8 * g + 4 * hh;
-      if (col >= p.d) continue;
-      f32x4 a, c;
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * n + 8 * g + 4 * hh;
+        if (col >= p.d) continue;
+        f32x4 a;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = ok ? dk[n][4 * g + e] * kk : 0.0f;
-        c[e] = ok ? dv[n][4 * g + e] * kv : 0.0f;
+        for (int e = 0; e < 4; ++e) a[e] = ok ? acc[n][4 * g + e] * k : 0.0f;
+        if (pk) {
+          *reinterpret_cast<f32x4*>(pk + col) = a;
+        } else {
+          typename Vec<T>::v4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = (T)a[e];
+          *reinterpret_cast<typename Vec<T>::v4*>(out + col) = x;
+        }
       }
-      if (pk) {
-        *reinterpret_cast<f32x4*>(pk + col) = a;
-        *reinterpret_cast<f32x4*>(pk + other + col) = c;
-      } else {
-        typename Vec<T>::v4 ta4, tc4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { ta4[e] = (T)a[e]; tc4[e] = (T)c[e]; }
-        *reinterpret_cast<typename Vec<T>::v4*>((T*)p.dk + krow * p.lddk + kh * p.d + col) = ta4;
-        *reinterpret_cast<typename Vec<T>::v4*>((T*)p.dv + krow * p.lddv + kh * p.d + col) = tc4;
-      }
-    }
+  };
+  T *to_k = (T*)p.dk + krow * p.lddk + kh * p.d, *to_v = (T*)p.dv + krow * p.lddv + kh * p.d;
+  const float of_k = p.scale / f, of_v = is_half<T> ? 6.103515625e-05f : 1.0f;
+  if constexpr (PAIR) {
+    leave(dv, second ? of_k : of_v, !second, second ? to_k : to_v);
+  } else {
+    leave(dk, of_k, 0, to_k);
+    leave(dv, of_v, 1, to_v);
+  }
 }
 
 // dK and dV of a split sweep: the parts added in their order, four columns to a thread.
@@ -488,14 +497,14 @@ long part_bytes(const dc_attn_desc* d) {
   const int n = dkv_splits(d);
   return n > 1 ? 8L * n * d->nb * d->tk * d->kv_heads * (d->d > 64 ? 128 : 64) : 0;
 }
-long bwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d); }
+long bwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d, true) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d); }
 
 template <typename T, int DP, bool SHAPED>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
   hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.heads * ((c.tq + 127) / 128))), dim3(256), 0,
                      st, c, bk);
-  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)), dim3(256), 0,
-                     st, c, bk);
+  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)),
+                     dim3(DP == 64 ? 256 : 512), 0, st, c, bk);
   if (bk.nk > 1) {
     const long n = 2L * c.nb * c.tk * c.kvh * (DP / 4);
     hipLaunchKernelGGL((dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, c, bk);
@@ -526,8 +535,8 @@ extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* scratch, long long 
   if ((uintptr_t)scratch & 15) return DC_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
   char* ws = static_cast<char*>(scratch);
-  launch_summaries(d, c, ws, st);
-  ws += summary_bytes(d);
+  launch_summaries(d, c, true, ws, st);
+  ws += summary_bytes(d, true);
   Back bk;
   bk.nlse = reinterpret_cast<float*>(ws);
   bk.ndel = reinterpret_cast<float*>(ws + rows_bytes(d));

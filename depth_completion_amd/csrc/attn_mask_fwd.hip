@@ -13,15 +13,22 @@
 namespace dcm {
 namespace {
 
-// least and largest document of 64 rows (rows in none left out), and whether a row is in none
-__global__ __launch_bounds__(256) void summary_kernel(const int* doc, int t, int nt, int total, int4* out) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (i >= total) return;
+// least and largest document of 64 rows (rows in none left out), and whether a row is in none: the keys' tiles, then the queries'
+__global__ __launch_bounds__(256) void summary_kernel(const int* doc_k, int tk, int nk, const int* doc_q, int tq, int nq, int nb,
+                                                      int4* out) {
+  int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (i >= nb * (nk + nq)) return;
+  int4* to = out + i;
+  const bool q = i >= nb * nk;
+  if (q) i -= nb * nk;
+  const int* doc = q ? doc_q : doc_k;
+  const int t = q ? tq : tk, nt = q ? nq : nk;
   const int b = i / nt, r = (i % nt) * 64 + lane;
   const int id = r < t ? doc[(long)b * t + r] : -1;
   const int lo = wave_min_i(id >= 0 ? id : 0x7fffffff), hi = wave_max_i(id);
   const bool none = __any(r < t && id < 0);
-  if (lane == 0) out[i] = make_int4(lo, hi, none, 0);
+  if (lane == 0) *to = make_int4(lo, hi, none, 0);
 }
 
 // Running softmax of one lane's query over tiles of scores.  m is the reference of the weights 2^(x - m); it follows the row's
@@ -113,6 +120,8 @@ __device__ __forceinline__ void put_row(const Call& p, const Row<T, DP>& s, floa
 template <typename T, int DP>
 __device__ __forceinline__ void put_part(const Split& sp, const Row<T, DP>& s, float l, long row, int part, int hh) {
   float* o = sp.o + (row * sp.n + part) * DP;
+  if (hh == 0) *reinterpret_cast<float2*>(sp.ml + (row * sp.n + part) * 2) = make_float2(s.m, l);
+  if (s.m == -INFINITY) return;   // no weight in it: join_kernel does not read O
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -122,7 +131,6 @@ __device__ __forceinline__ void put_part(const Split& sp, const Row<T, DP>& s, f
       for (int e = 0; e < 4; ++e) v[e] = s.o[n][4 * g + e];
       *reinterpret_cast<f32x4*>(o + 32 * n + 8 * g + 4 * hh) = v;
     }
-  if (hh == 0) *reinterpret_cast<float2*>(sp.ml + (row * sp.n + part) * 2) = make_float2(s.m, l);
 }
 
 // A step: tile i has landed (waited for, barrier), S, softmax, P V; then tile i + 2 is sent to the buffer that tile i - 1 left.  The
@@ -135,7 +143,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
   typedef KeyRing<T, DP, S> Ring;
   __shared__ typename Ring::Lds lds;
-  __shared__ int range[5];
+  __shared__ int range[6];
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   QueryBlock q;
   q.init(p, sp.n);
@@ -144,14 +152,15 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, q.live && 16 * s + 8 * hh < p.d);
   int t0, t1;
-  q.tiles(p, q.live, range, t0, t1);
+  bool holes;
+  q.tiles(p, q.live, range, t0, t1, holes);
   if (sp.n > 1) {
     const int each = (t1 - t0 + sp.n - 1) / sp.n;
     t0 = min(t1, t0 + q.part * each);
     t1 = min(t1, t0 + each);
   }
   Ring ring;
-  ring.init(p, q);
+  ring.init(p, q, holes);
   Row<T, DP> st;
   st.init();
   const float slope = SHAPED && p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
@@ -423,9 +432,11 @@ constexpr int kMaxSplit = 64;
 // Few query rows (at most 32 in a sequence, a quarter of fwd_kernel's block): token_kernel.
 bool few_rows(int tq) { return tq <= 32; }
 
-// How the keys are split.  Few rows: enough blocks to give every CU four where the keys allow it, each with 4
-// steps of 128 keys or more (the steps a block has cover its start and its merge).  Many rows: a block to every CU, each with 16 tiles
-// of 64 keys or more.
+// How the keys are split.  Few rows: enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or
+// more (the steps a block has cover its start and its merge).  Many rows: only where the card is not full, to 4/3 of what it holds (a
+// few long blocks more than it has CUs for would double the time), each split 16 tiles of 64 or more.  us with 1, 2, 4, 8 splits:
+// 6912 x 5 heads of 64 (270 blocks) 142, 121, 110, 116; 4608 x 5 (180) 84, 67, 59, 63; 1728 x 10 (140 blocks of 27 tiles) 32, 35,
+// 36, 38; 8 x 1728 x 10 (1120) 95, 140, 156, 240: the 32-bit parts of O cost their writing and reading.
 Split split_of(const dc_attn_desc* d) {
   Split s{1, 0, nullptr, nullptr};
   const long grp = d->heads / d->kv_heads;
@@ -437,7 +448,8 @@ Split split_of(const dc_attn_desc* d) {
     s.n = (int)((steps + s.tiles - 1) / s.tiles);
   } else {
     const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
-    if (blocks < 128) s.n = (int)min(min((256 + blocks - 1) / blocks, max(tiles / 16, 1L)), (long)kMaxSplit);
+    const long slots = 256 * (d->d > 64 ? 2 : 3);   // blocks that the card holds at once
+    if (3 * blocks < 2 * slots) s.n = (int)min(min((4 * slots / 3 + blocks - 1) / blocks, max(tiles / 16, 1L)), (long)kMaxSplit);
   }
   return s;
 }
@@ -466,22 +478,24 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
 
 }  // namespace
 
-long long summary_bytes(const dc_attn_desc* d) {
-  if (!d->doc_q) return 0;
-  return 16LL * d->nb * ((d->tq + 63L) / 64 + (d->tk + 63L) / 64);
+// Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.
+bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
+// the queries' tiles are the keys' where the documents are the same rows; the forward does not ask for them
+bool query_tiles(const dc_attn_desc* d, bool backward) { return backward && !(d->doc_q == d->doc_k && d->tq == d->tk); }
+
+long long summary_bytes(const dc_attn_desc* d, bool backward) {
+  if (!summarised(d)) return 0;
+  return 16LL * d->nb * ((d->tk + 63L) / 64 + (query_tiles(d, backward) ? (d->tq + 63L) / 64 : 0));
 }
 
-void launch_summaries(const dc_attn_desc* d, Call& c, char* ws, hipStream_t st) {
-  if (!d->doc_q) return;
-  const int nk = (d->tk + 63) / 64, nq = (d->tq + 63) / 64;
+void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st) {
+  if (!summarised(d)) return;
+  const int nk = (d->tk + 63) / 64, nq = query_tiles(d, backward) ? (d->tq + 63) / 64 : 0;
   int4* k = reinterpret_cast<int4*>(ws);
-  int4* q = k + (long)d->nb * nk;
   c.sum_k = k;
-  c.sum_q = q;
-  hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * nk + 3) / 4)), dim3(256), 0, st, d->doc_k, d->tk, nk,
-                     d->nb * nk, k);
-  hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * nq + 3) / 4)), dim3(256), 0, st, d->doc_q, d->tq, nq,
-                     d->nb * nq, q);
+  c.sum_q = nq ? k + (long)d->nb * nk : k;
+  hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * (nk + nq) + 3) / 4)), dim3(256), 0, st, d->doc_k, d->tk, nk, d->doc_q,
+                     d->tq, nq, d->nb, k);
 }
 
 int make_call(const dc_attn_desc* d, Call& c, bool backward) {
@@ -491,10 +505,9 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   if (!(d->scale <= 1e30f) || !(d->softcap <= 1e30f) || (d->softcap > 0.0f && !(d->scale / d->softcap <= 1e30f))) return DC_ERR_ARG;
   if (d->prefix && !d->causal) return DC_ERR_ARG;
   if (!d->doc_q != !d->doc_k) return DC_ERR_ARG;
-  // row and block counts stay within 31 bits
+  // row and block counts stay within 31 bits, splits included
   const long long rows = (long long)d->nb * d->heads * d->tq;
-  if (rows >= (1LL << 31) || (long long)d->nb * d->tk * d->kv_heads >= (1LL << 31) || d->tq > (1 << 30) || d->tk > (1 << 30))
-    return DC_ERR_ARG;
+  if (rows >= (1LL << 30) || (long long)d->nb * d->tk * d->kv_heads >= (1LL << 30)) return DC_ERR_ARG;
   const int hq = d->heads * d->d, hk = d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
   if (d->ldk > (1 << 23) || d->ldv > (1 << 23)) return DC_ERR_ARG;   // 128 rows within 32 bits
@@ -525,7 +538,7 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   return DC_OK;
 }
 
-long long fwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d) + 4LL * part_floats(d, split_of(d)); }
+long long fwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d, false) + 4LL * part_floats(d, split_of(d)); }
 
 }  // namespace dcm
 
@@ -538,10 +551,10 @@ extern "C" int dc_attn_mask_fwd(const dc_attn_desc* d, void* scratch, long long 
   if ((uintptr_t)scratch & 15) return DC_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
   char* ws = static_cast<char*>(scratch);
-  launch_summaries(d, c, ws, st);
+  launch_summaries(d, c, false, ws, st);
   Split s = split_of(d);
   if (s.n > 1) {
-    s.o = reinterpret_cast<float*>(ws + summary_bytes(d));
+    s.o = reinterpret_cast<float*>(ws + summary_bytes(d, false));
     s.ml = s.o + (long)d->nb * d->heads * d->tq * s.n * (d->d > 64 ? 128 : 64);
   }
   if (d->type == 0) d->d > 64 ? launch_fwd<bf16, 128>(c, d, s, st) : launch_fwd<bf16, 64>(c, d, s, st);

@@ -70,7 +70,7 @@ ARG, ALIGN = 1, 3
     (dict(scale=float("inf")), ARG), (dict(softcap=-1.0), ARG), (dict(softcap=float("nan")), ARG), (dict(prefix=4096), ARG),
     (dict(doc_q=4096), ARG), (dict(doc_k=4096), ARG), (dict(ldq=248), ARG), (dict(ldk=120), ARG), (dict(ldq=260), ALIGN),
     (dict(ldv=132), ALIGN), (dict(q=4098), ALIGN), (dict(v=4104), ALIGN),
-    (dict(nb=1 << 20, tq=1 << 10), ARG), (dict(doc_q=4096, doc_k=4096), ARG), (dict(tq=1, tk=100000), ARG)])
+    (dict(nb=1 << 20, tq=1 << 10), ARG), (dict(doc_q=4096, doc_k=4096, tk=1000), ARG), (dict(tq=1, tk=100000), ARG)])
 def test_entry_refuses(entry, kw, status):
     """The last two want scratch that the call does not bring."""
     assert getattr(_lib.load(), entry)(C.byref(descriptor(**kw)), None, 0, None) == status
