@@ -239,6 +239,7 @@ __device__ __forceinline__ void unit_of(int units, int per_unit, int& unit, int&
 struct QueryBlock {
   int b, kh, h, part, qi, len, pos, lim, mine;   // lim: the lane's query sees the keys below it (of its document `mine`)
   bool live;
+  int4 sum0;   // the thread's first tile summary, read along with the rows
   // of a unit's tiles of 128 rows (the longest rows of a causal call first) x splits x heads of the group
   __device__ __forceinline__ void init(const Call& p, int splits) {
     const int nqb = (p.tq + 127) / 128;
@@ -256,6 +257,10 @@ struct QueryBlock {
     lim = p.causal ? min(len, max(pos + 1, p.prefix ? p.prefix[b] : 0)) : len;
     mine = p.doc_q ? (live ? p.doc_q[(long)b * p.tq + qi] : -1) : 0;
     if (mine < 0) lim = 0;
+    if (p.sum_k) {
+      const int nt = (p.tk + 63) / 64;
+      sum0 = p.sum_k[(long)b * nt + min((int)threadIdx.x, nt - 1)];
+    }
   }
   // The 64-key tiles [t0, t1) in which some row with `sees` may see a key; holes: some key of theirs is (or may be) in no document.
   __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1, bool& holes) const {
@@ -271,22 +276,43 @@ struct QueryBlock {
       const int nt = (p.tk + 63) / 64, least = range[2], largest = range[3];
       const int4* sum = p.sum_k + (long)b * nt;
       int first = 0x7fffffff, last = -1;
-      for (int t = threadIdx.x; t < t1; t += blockDim.x) {
-        const int4 s = sum[t];
+      for (int t = threadIdx.x; t < t1; t += 256) {
+        const int4 s = t < 256 ? sum0 : sum[t];
         if (s.y >= least && s.x <= largest) { first = min(first, t); last = t; }
       }
       if (last >= 0) { atomicMin(&range[0], first); atomicMax(&range[4], last + 1); }
       __syncthreads();
       t1 = range[4];
       t0 = min(range[0], t1);
-      int none = 0;
-      for (int t = t0 + threadIdx.x; t < t1; t += blockDim.x) none |= sum[t].z;
-      if (none) range[5] = 1;
+      for (int t = threadIdx.x; t < t1; t += 256)
+        if (t >= t0 && (t < 256 ? sum0 : sum[t]).z) range[5] = 1;
       __syncthreads();
     }
     holes = p.doc_q && (!p.sum_k || __builtin_amdgcn_readfirstlane(range[5]));
     t0 = __builtin_amdgcn_readfirstlane(t0);
     t1 = __builtin_amdgcn_readfirstlane(t1);
+  }
+};
+
+// What a wave has to do with a tile of keys: nothing (no row sees one of them), all without a mask, or a mask.
+struct WaveRange {
+  int all, any, least, most;   // keys that every live row sees, that some row does; the rows' documents
+  __device__ __forceinline__ void init(const QueryBlock& q, bool live) {
+    all = __builtin_amdgcn_readfirstlane(wave_min_i(live ? q.lim : 0x7fffffff));
+    any = __builtin_amdgcn_readfirstlane(wave_max_i(live ? q.lim : 0));
+    least = __builtin_amdgcn_readfirstlane(wave_min_i(live && q.mine >= 0 ? q.mine : 0x7fffffff));
+    most = __builtin_amdgcn_readfirstlane(wave_max_i(live ? q.mine : -1));
+  }
+  // id: the keys' documents, or NULL
+  __device__ __forceinline__ bool nothing(int t, const int* id) const {
+    if (t * 64 >= any) return true;
+    if (!id) return false;
+    const int i = id[threadIdx.x & 63];
+    return !__any(i >= least && i <= most);
+  }
+  __device__ __forceinline__ bool masked(int t, const int* id, const QueryBlock& q, bool live) const {
+    if (t * 64 + 64 > all) return true;
+    return id && (__any(live && id[0] != q.mine) || __any(id[threadIdx.x & 63] != id[0]));
   }
 };
 

@@ -33,7 +33,7 @@ __device__ __forceinline__ float near_sixteenth(float x) {
 }
 
 template <typename T, int DP, bool SHAPED>
-__global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
   typedef KeyRing<T, DP, S> Ring;
@@ -90,21 +90,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
   else
 #pragma unroll
     for (int n = 0; n < 2; ++n) ka[n] = tr_at<DP>(32 * n, lane);
-  const int seen_by_all = __builtin_amdgcn_readfirstlane(wave_min_i(sees ? q.lim : 0x7fffffff));
+  WaveRange range_of;
+  range_of.init(q, sees);
   vm_wait<0>();
   if (t0 < t1) ring.load(p, lds, t0, 0);
   if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
-  auto step = [&](int t, auto B) __attribute__((always_inline)) {   // as the forward's
+  auto tile = [&](int t, auto B, const int* id) __attribute__((always_inline)) {
     constexpr int buf = decltype(B)::value;
-    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
-    else vm_wait<0>();
-    tile_barrier();
-    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
     const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
-    const int* id = lds.ids[buf];
-    bool partial = seen_by_all < t * 64 + 64;
-    if (ring.kid) partial |= __any(sees && id[0] != q.mine) || __any(id[lane] != id[0]);
+    const bool masked = range_of.masked(t, id, q, sees);
     auto half_tile = [&](auto K) __attribute__((always_inline)) {
       constexpr int kb2 = decltype(K)::value;
       f32x16 s = {}, dp = {};
@@ -139,16 +134,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
         const float pw = exp2_raw(SHAPED ? s[r] + nl : fmaf(s[r], p.mul, nl));
         s[r] = (is_half<T> ? pw * f : pw) * dp[r];
       }
-      if (partial) {
+      if (masked) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int key = 32 * kb2 + 8 * g + 4 * hh;
           int4 i4 = make_int4(0, 0, 0, 0);
-          if (ring.kid) i4 = *reinterpret_cast<const int4*>(&id[key]);
+          if (id) i4 = *reinterpret_cast<const int4*>(&id[key]);
           const int id4[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t * 64 + key + e >= q.lim || (ring.kid && id4[e] != q.mine)) s[4 * g + e] = 0.0f;
+            if (t * 64 + key + e >= q.lim || (id && id4[e] != q.mine)) s[4 * g + e] = 0.0f;
         }
       }
       auto add = [&](auto C) __attribute__((always_inline)) {
@@ -167,6 +162,15 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Call p, Back bk) {
     };
     half_tile(std::integral_constant<int, 0>{});
     half_tile(std::integral_constant<int, 1>{});
+  };
+  auto step = [&](int t, auto B) __attribute__((always_inline)) {   // as the forward's
+    constexpr int buf = decltype(B)::value;
+    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
+    else vm_wait<0>();
+    tile_barrier();
+    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
+    const int* id = ring.kid ? lds.ids[buf] : nullptr;
+    if (!range_of.nothing(t, id)) tile(t, B, id);
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   for (int t = t0; t < t1; t += S) {
@@ -243,7 +247,9 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   const float f = is_half<T> ? head_factor(p, bk, b, kh, scratch) : 1.0f;
   // the lane's key is seen from position `from` on
   const int from = !ok ? 0x7fffffff : p.causal && key >= pre ? key : -0x7fffffff;
-  const int from_last = __builtin_amdgcn_readfirstlane(wave_max_i(from));
+  const int from_last = __builtin_amdgcn_readfirstlane(wave_max_i(from)), from_first = __builtin_amdgcn_readfirstlane(wave_min_i(from));
+  const int id_least = __builtin_amdgcn_readfirstlane(wave_min_i(mine >= 0 ? mine : 0x7fffffff));
+  const int id_most = __builtin_amdgcn_readfirstlane(wave_max_i(mine));
   int t0 = 0, t1 = (p.tq + 63) / 64;
   if (p.causal && k0 >= pre) t0 = max(0, k0 - shift) / 64;
   if (k0 >= len) t1 = 0;
@@ -326,6 +332,9 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     tile_barrier();
     const T* qt = tiles[buf];
     const T* dt = qt + TILE;
+    // none of the wave's keys is seen from the tile
+    const bool nothing = from_first > t * 64 + shift + 63 ||
+                         (p.doc_q && !__any(ids[buf][lane] >= id_least && ids[buf][lane] <= id_most));
     // P and dS of 32 rows of the tile (a pair's: qoff is at the wave's own)
     auto weights = [&](int at, v8 (&pf)[2], v8 (&sf)[2]) __attribute__((always_inline)) {
       const int rows = at + 32 * second, row0 = rows + 4 * hh, pos0 = t * 64 + shift + row0;   // of the lane's first row
@@ -393,7 +402,12 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     };
     v8 pf[2], sf[2];
     if constexpr (PAIR) {
-      weights(0, pf, sf);
+      if (!nothing) {
+        weights(0, pf, sf);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) pf[c] = sf[c] = v8{};
+      }
       v8 own[2], other[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -403,13 +417,14 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
       tile_barrier();
 #pragma unroll
       for (int c = 0; c < 2; ++c) other[c] = *reinterpret_cast<const v8*>(&swap[wid ^ 1][c][lane * 8]);
+      if (!nothing)   // (the same for both of a pair)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const v8 mid = (c >> 1) == second ? own[c & 1] : other[c & 1];
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n) dv[n] = mfma(tr_frag(qt + 16 * c * DP, ta[n]), mid, dv[n]);
       }
-    } else {
+    } else if (!nothing) {
 #pragma unroll
       for (int rows = 0; rows < 64; rows += 32) {
         weights(rows, pf, sf);

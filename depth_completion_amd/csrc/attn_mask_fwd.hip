@@ -173,17 +173,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   else
 #pragma unroll
     for (int n = 0; n < 2; ++n) va[n] = tr_at<DP>(32 * n, lane);
-  const int seen_by_all = __builtin_amdgcn_readfirstlane(wave_min_i(q.live ? q.lim : 0x7fffffff));   // keys that no row has to mask
+  WaveRange range_of;
+  range_of.init(q, q.live);
 
   vm_wait<0>();   // (the counts below are of tiles alone)
   if (t0 < t1) ring.load(p, lds, t0, 0);
   if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
-  auto step = [&](int t, auto B) __attribute__((always_inline)) {
+  auto tile = [&](int t, auto B, const int* id) __attribute__((always_inline)) {
     constexpr int buf = decltype(B)::value;
-    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
-    else vm_wait<0>();
-    tile_barrier();
-    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
     const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
     f32x16 s[2];
@@ -214,10 +211,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
             s[kb2][r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[kb2][r]);
       }
     }
-    const int* id = lds.ids[buf];
-    bool partial = seen_by_all < t * 64 + 64;
-    if (ring.kid) partial |= __any(q.live && id[0] != q.mine) || __any(id[lane] != id[0]);
-    if (partial) {
+    if (range_of.masked(t, id, q, q.live)) {
       asm volatile("" ::: "memory");   // a branch, not selects in every tile
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2)
@@ -225,11 +219,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
         for (int g = 0; g < 4; ++g) {
           const int key = 32 * kb2 + 8 * g + 4 * hh;
           int4 i4 = make_int4(0, 0, 0, 0);
-          if (ring.kid) i4 = *reinterpret_cast<const int4*>(&id[key]);
+          if (id) i4 = *reinterpret_cast<const int4*>(&id[key]);
           const int id4[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t * 64 + key + e >= q.lim || (ring.kid && id4[e] != q.mine)) s[kb2][4 * g + e] = -INFINITY;
+            if (t * 64 + key + e >= q.lim || (id && id4[e] != q.mine)) s[kb2][4 * g + e] = -INFINITY;
         }
     }
     st.weigh(s, SHAPED ? 1.0f : p.mul);
@@ -248,6 +242,15 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
     add(std::integral_constant<int, 1>{});
     add(std::integral_constant<int, 2>{});
     add(std::integral_constant<int, 3>{});
+  };
+  auto step = [&](int t, auto B) __attribute__((always_inline)) {
+    constexpr int buf = decltype(B)::value;
+    if (S == 3 && t + 1 < t1) vm_wait<OPS>();
+    else vm_wait<0>();
+    tile_barrier();
+    if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
+    const int* id = ring.kid ? lds.ids[buf] : nullptr;
+    if (!range_of.nothing(t, id)) tile(t, B, id);
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   for (int t = t0; t < t1; t += S) {
@@ -394,37 +397,39 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   else put_row<T, DP>(p, st, st.l, row, (long)b * p.tq + qi, h, hh);
 }
 
-// One wave: one row's splits, joined in their order.
+// A row's splits, joined in their order, by DP / 4 lanes with four columns each.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) {
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  constexpr int LANES = DP / 4;
+  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int col = threadIdx.x % LANES * 4;
   if (row >= rows) return;
-  float2 ml = make_float2(-INFINITY, 0.0f);
-  if (lane < sp.n) ml = *reinterpret_cast<const float2*>(sp.ml + (row * sp.n + lane) * 2);
-  const float top = wave_max(ml.x);
-  const float f = ml.x == -INFINITY ? 0.0f : exp2_raw(ml.x - top);
-  // (a split that saw NaN scores alone has m = -inf and l = NaN: it has to reach the result)
-  const float l = wave_sum(ml.y * (ml.y != ml.y ? 1.0f : f));
-  constexpr int E = DP / 64;
-  float o[E] = {};
-  const float* src = sp.o + row * sp.n * DP + lane * E;
+  const float2* ml = reinterpret_cast<const float2*>(sp.ml) + row * sp.n;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < sp.n; ++i) top = fmaxf(top, ml[i].x);
+  float l = 0.0f;
+  f32x4 o = {};
+  const float* src = sp.o + row * sp.n * DP + col;
+#pragma unroll 4
   for (int i = 0; i < sp.n; ++i) {
-    const float k = __shfl(f, i, 64);
-    if (k == 0.0f) continue;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(src[(long)i * DP + e], k, o[e]);
+    const float2 x = ml[i];
+    // a split without weights left no O; one that saw NaN scores alone has m = -inf and l = NaN, which has to reach the result
+    const float k = x.x == -INFINITY ? 0.0f : exp2_raw(x.x - top);
+    l += x.y != x.y ? x.y : x.y * k;
+    if (x.x != -INFINITY) o += *reinterpret_cast<const f32x4*>(src + (long)i * DP) * k;
   }
   const long bh = row / p.tq, q = row % p.tq, b = bh / p.heads;
   const int h = (int)(bh % p.heads);
   const bool none = l == 0.0f;
   const float inv = 1.0f / l;
-  if (lane * E < p.d) {
-    T* dst = (T*)p.o + (b * p.tq + q) * p.ldo + h * p.d + lane * E;
+  if (col < p.d) {
+    typename Vec<T>::v4 v;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = (T)(none ? 0.0f : o[e] * inv);
+    for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] * inv);
+    *reinterpret_cast<typename Vec<T>::v4*>((T*)p.o + (b * p.tq + q) * p.ldo + h * p.d + col) = v;
   }
-  if (lane == 0) p.lse[row] = none ? -INFINITY : (top + (__builtin_amdgcn_logf(l) - Row<T, DP>::SHIFT)) * kLn2;
+  if (col == 0) p.lse[row] = none ? -INFINITY : (top + (__builtin_amdgcn_logf(l) - Row<T, DP>::SHIFT)) * kLn2;
 }
 
 constexpr int kMaxSplit = 64;
@@ -469,7 +474,8 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
     hipLaunchKernelGGL((fwd_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   }
   const long rows = (long)c.nb * c.heads * c.tq;
-  if (s.n > 1) hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, c, s, rows);
+  if (s.n > 1) hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)((rows * (DP / 4) + 255) / 256)), dim3(256), 0, st, c,
+                                   s, rows);
 }
 template <typename T, int DP>
 void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
