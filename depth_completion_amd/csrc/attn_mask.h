@@ -42,12 +42,12 @@ struct Call {
   const int4 *sum_q, *sum_k;   // per 64 rows: least and largest document, whether a row is in none (NULL: short rows, no documents)
 };
 
-// Scores of a call with a cap or a distance bias, in units of log2: s = cap2 tanh(scale s / cap), then - slope |pos - key|.
-// tanh(x) = 1 - 2 / (1 + e^2x): absolute error below 2e-7, so the exponent is off by under 1e-5 at cap = 50.
+// Scores of a call with a cap, in units of log2: cap2 tanh(scale s / cap), with tanh(x) = 1 - 2 r, r = 1 / (1 + e^2x): absolute error
+// of tanh below 2e-7, so the exponent is off by under 1e-5 at cap = 50.  slope: r - r^2, a quarter of 1 - tanh^2.
 __device__ __forceinline__ float cap_score(const Call& p, float s, float* slope) {
-  const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_raw(s * p.icap));
-  if (slope) *slope = 1.0f - t * t;
-  return t * p.cap2;
+  const float r = __builtin_amdgcn_rcpf(1.0f + exp2_raw(s * p.icap));
+  if (slope) *slope = fmaf(-r, r, r);
+  return fmaf(-2.0f * p.cap2, r, p.cap2);
 }
 
 // ---------------------------------------------------------------- LDS tiles
@@ -358,6 +358,8 @@ struct KeyRing {
 };
 
 // Host side: what both directions share (attn_mask_fwd.hip).
+constexpr int kMaxSplit = 64;
+int tile_splits(const dc_attn_desc* d);
 int make_call(const dc_attn_desc* d, Call& c, bool backward);
 long long summary_bytes(const dc_attn_desc* d, bool backward);
 void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st);

@@ -19,11 +19,22 @@ struct Back {
   float *nlse, *ndel;   // [nb heads][tq]: -lse log2 e (-inf: the row sees no key), -rowsum(dO o)
   int2* rows32;         // [nb heads][n32]: of 32 rows, whether one sees no key, and the largest |dO| (its bits)
   int n32;
-  int nk;               // splits of dkv_kernel's sweep
-  float* part;          // [nk][2][nb tk][kvh][DP]
+  int nq, nk;           // splits of dq_kernel's sweep over the keys, of dkv_kernel's over the queries
+  float *part_q, *part; // [nq][nb tq][heads][DP]; [nk][2][nb tk][kvh][DP]
 };
 
 template <typename T> constexpr bool is_half = __is_same(T, half);
+
+// what dS as the kernels hold it lacks (cap_score gives a quarter of the slope)
+__device__ __forceinline__ float ds_scale(const Call& p) { return p.cap2 != 0.0f ? 4.0f * p.scale : p.scale; }
+
+template <typename T>
+__device__ __forceinline__ void put4(T* out, f32x4 a) {
+  typename Vec<T>::v4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (T)a[e];
+  *reinterpret_cast<typename Vec<T>::v4*>(out) = v;
+}
 
 // power of two that brings a positive finite x into [2^-4, 2^-3)
 __device__ __forceinline__ float near_sixteenth(float x) {
@@ -41,7 +52,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   __shared__ int range[6];
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   QueryBlock q;
-  q.init(p, 1);
+  q.init(p, bk.nq);
   const long row = ((long)q.b * p.heads + q.h) * p.tq + (q.live ? q.qi : 0), trow = (long)q.b * p.tq + (q.live ? q.qi : 0);
   const float lse = p.lse[row];
   const bool sees = q.live && lse != -INFINITY;
@@ -63,17 +74,22 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   del = pair_sum(del);
   most = pair_max(most);
   const float nl = sees ? -lse * kLog2e : -INFINITY;
-  if (q.live && hh == 0) {
+  if (q.live && hh == 0 && q.part == 0) {
     bk.nlse[row] = nl;
     bk.ndel[row] = -del;
   }
   const float wave_most = wave_max(most);
   const bool blind = __any(q.live && !sees);
-  if (lane == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
+  if (lane == 0 && q.part == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
   const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
   int t0, t1;
   bool holes;
   q.tiles(p, sees, range, t0, t1, holes);
+  if (bk.nq > 1) {
+    const int each = (t1 - t0 + bk.nq - 1) / bk.nq;
+    t0 = min(t1, t0 + q.part * each);
+    t1 = min(t1, t0 + each);
+  }
 
   Ring ring;
   ring.init(p, q, holes);
@@ -180,18 +196,20 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
       if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{});
   }
   if (!q.live) return;
-  const float k = p.scale / f;
+  const float k = ds_scale(p) / f;
   T* out = (T*)p.dq + ((long)q.b * p.tq + q.qi) * p.lddq + q.h * p.d;
+  float* pq = bk.nq > 1 ? bk.part_q + ((((long)q.part * p.nb + q.b) * p.tq + q.qi) * p.heads + q.h) * DP : nullptr;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int col = 32 * n + 8 * g + 4 * hh;
       if (col >= p.d) continue;
-      typename Vec<T>::v4 v;
+      f32x4 a;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(sees ? dq[n][4 * g + e] * k : 0.0f);
-      *reinterpret_cast<typename Vec<T>::v4*>(out + col) = v;
+      for (int e = 0; e < 4; ++e) a[e] = sees ? dq[n][4 * g + e] * k : 0.0f;
+      if (pq) *reinterpret_cast<f32x4*>(pq + col) = a;
+      else put4(out + col, a);
     }
 }
 
@@ -458,18 +476,12 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
         f32x4 a;
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] = ok ? acc[n][4 * g + e] * k : 0.0f;
-        if (pk) {
-          *reinterpret_cast<f32x4*>(pk + col) = a;
-        } else {
-          typename Vec<T>::v4 x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (T)a[e];
-          *reinterpret_cast<typename Vec<T>::v4*>(out + col) = x;
-        }
+        if (pk) *reinterpret_cast<f32x4*>(pk + col) = a;
+        else put4(out + col, a);
       }
   };
   T *to_k = (T*)p.dk + krow * p.lddk + kh * p.d, *to_v = (T*)p.dv + krow * p.lddv + kh * p.d;
-  const float of_k = p.scale / f, of_v = is_half<T> ? 6.103515625e-05f : 1.0f;
+  const float of_k = ds_scale(p) / f, of_v = is_half<T> ? 6.103515625e-05f : 1.0f;
   if constexpr (PAIR) {
     leave(dv, second ? of_k : of_v, !second, second ? to_k : to_v);
   } else {
@@ -478,31 +490,34 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   }
 }
 
-// dK and dV of a split sweep: the parts added in their order, four columns to a thread.
+// The parts of split sweeps added in their order, four columns to a thread: [n][rows][per][DP] to rows of `per` heads of d columns.
+struct Parts {
+  const float* part;
+  int n, per;
+  long rows, stride;   // stride: from a part to the next
+  void* out;
+  int ld;
+};
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void dkv_join_kernel(Call p, Back bk) {
-  const long rows = (long)p.nb * p.tk * p.kvh, i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long rk = i / (DP / 4);
+__global__ __launch_bounds__(256) void add_parts_kernel(Parts a, Parts b, Parts c, int d) {
+  const Parts p = blockIdx.y == 0 ? a : blockIdx.y == 1 ? b : c;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, rh = i / (DP / 4);
   const int col = (int)(i % (DP / 4)) * 4;
-  if (rk >= 2 * rows || col >= p.d) return;
-  const bool v = rk >= rows;
-  const float* src = bk.part + rk * DP + col;
-  f32x4 a = {};
-  for (int s = 0; s < bk.nk; ++s) a += *reinterpret_cast<const f32x4*>(src + 2L * s * rows * DP);
-  const long r = v ? rk - rows : rk, krow = r / p.kvh;
-  T* out = (v ? (T*)p.dv + krow * p.lddv : (T*)p.dk + krow * p.lddk) + r % p.kvh * p.d + col;
-  typename Vec<T>::v4 x;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = (T)a[e];
-  *reinterpret_cast<typename Vec<T>::v4*>(out) = x;
+  if (rh >= p.rows * p.per || col >= d) return;
+  const float* src = p.part + rh * DP + col;
+  f32x4 s = {};
+#pragma unroll 4
+  for (int k = 0; k < p.n; ++k) s += *reinterpret_cast<const f32x4*>(src + k * p.stride);
+  put4((T*)p.out + rh / p.per * p.ld + rh % p.per * d + col, s);
 }
 
-// Splits of dkv_kernel's sweep: where its blocks are fewer than two to a CU, up to 8 and no shorter than 8 tiles each.
+// Splits of dkv_kernel's sweep, where its blocks do not fill the card: no shorter than 8 tiles each.  us of the whole backward with
+// 1, 2, 3, 4, 8: 6912 x 5 heads of 64 (270 blocks) 390, 354, 325, 328, 344; 4608 x 5 (180) 200, 166, 184, 166, 176; 8 x 1728 x 10 (1120)
+// 294, 312, 345, 365, 508; causal, heads of 128: 4096 x 32/8 (256) 691, 520, 553, 542, 617; 2 x 2500 x 16/4 (160) 401, 269, 254, 257, 282.
 int dkv_splits(const dc_attn_desc* d) {
   const long blocks = (long)d->nb * d->kv_heads * ((d->tk + 127L) / 128);
   const long steps = (long)(d->heads / d->kv_heads) * ((d->tq + 63L) / 64);
-  if (blocks >= 512) return 1;
-  return (int)max(1L, min(min((1024 + blocks - 1) / blocks, steps / 8), 8L));
+  return (int)max(1L, min(min((d->d > 64 ? 600 : 900) / blocks, steps / 8), 8L));
 }
 long pad16(long bytes) { return (bytes + 15) / 16 * 16; }
 
@@ -512,18 +527,28 @@ long part_bytes(const dc_attn_desc* d) {
   const int n = dkv_splits(d);
   return n > 1 ? 8L * n * d->nb * d->tk * d->kv_heads * (d->d > 64 ? 128 : 64) : 0;
 }
-long bwd_ws_bytes(const dc_attn_desc* d) { return summary_bytes(d, true) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d); }
+long part_q_bytes(const dc_attn_desc* d) {
+  const int n = tile_splits(d);
+  return n > 1 ? 4L * n * d->nb * d->tq * d->heads * (d->d > 64 ? 128 : 64) : 0;
+}
+long bwd_ws_bytes(const dc_attn_desc* d) {
+  return summary_bytes(d, true) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d) + part_q_bytes(d);
+}
 
 template <typename T, int DP, bool SHAPED>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
-  hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.heads * ((c.tq + 127) / 128))), dim3(256), 0,
-                     st, c, bk);
+  hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.heads * ((c.tq + 127) / 128) * bk.nq)),
+                     dim3(256), 0, st, c, bk);
   hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)),
                      dim3(DP == 64 ? 256 : 512), 0, st, c, bk);
-  if (bk.nk > 1) {
-    const long n = 2L * c.nb * c.tk * c.kvh * (DP / 4);
-    hipLaunchKernelGGL((dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, c, bk);
-  }
+  const long nk = (long)c.nb * c.tk * c.kvh, nq = (long)c.nb * c.tq * c.heads;
+  const Parts none{};
+  const Parts dk{bk.part, bk.nk, c.kvh, (long)c.nb * c.tk, 2 * nk * DP, c.dk, c.lddk}, dv{bk.part + nk * DP, bk.nk, c.kvh,
+                 (long)c.nb * c.tk, 2 * nk * DP, c.dv, c.lddv}, dq{bk.part_q, bk.nq, c.heads, (long)c.nb * c.tq, nq * DP, c.dq, c.lddq};
+  const long most = max(bk.nk > 1 ? nk : 0, bk.nq > 1 ? nq : 0);
+  if (most)
+    hipLaunchKernelGGL((add_parts_kernel<T, DP>), dim3((unsigned)((most * (DP / 4) + 255) / 256), bk.nk > 1 ? 3 : 1), dim3(256), 0,
+                       st, bk.nq > 1 ? dq : none, bk.nk > 1 ? dk : none, bk.nk > 1 ? dv : none, c.d);
 }
 template <typename T, int DP>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
@@ -557,8 +582,10 @@ extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* scratch, long long 
   bk.ndel = reinterpret_cast<float*>(ws + rows_bytes(d));
   bk.rows32 = reinterpret_cast<int2*>(ws + 2 * rows_bytes(d));
   bk.n32 = (d->tq + 127) / 128 * 4;
+  bk.nq = tile_splits(d);
   bk.nk = dkv_splits(d);
   bk.part = reinterpret_cast<float*>(ws + 2 * rows_bytes(d) + rows32_bytes(d));
+  bk.part_q = reinterpret_cast<float*>(ws + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d));
   if (d->type == 0) d->d > 64 ? launch_bwd<bf16, 128>(c, bk, st) : launch_bwd<bf16, 64>(c, bk, st);
   else d->d > 64 ? launch_bwd<half, 128>(c, bk, st) : launch_bwd<half, 64>(c, bk, st);
   DC_CHECK_LAUNCH();

@@ -397,27 +397,46 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   else put_row<T, DP>(p, st, st.l, row, (long)b * p.tq + qi, h, hh);
 }
 
-// A row's splits, joined in their order, by DP / 4 lanes with four columns each.
-template <typename T, int DP>
+// A row's splits joined, four columns to a lane.  G groups of lanes take every G-th split each and are added in order: one group to a
+// row where there are many rows, a whole block where there are few (one token over 131072 keys in 64
+// splits: 142 us with one group, 119 with eight).
+template <typename T, int DP, int G>
 __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) {
   constexpr int LANES = DP / 4;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
-  const int col = threadIdx.x % LANES * 4;
+  __shared__ float red[G == 1 ? 1 : G][G == 1 ? 1 : LANES][5];
+  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / (LANES * G);
+  const int lane = threadIdx.x % LANES, col = lane * 4, grp = G == 1 ? 0 : threadIdx.x / LANES;
   if (row >= rows) return;
   const float2* ml = reinterpret_cast<const float2*>(sp.ml) + row * sp.n;
   float top = -INFINITY;
+  if constexpr (G == 1) {
 #pragma unroll 4
-  for (int i = 0; i < sp.n; ++i) top = fmaxf(top, ml[i].x);
+    for (int i = 0; i < sp.n; ++i) top = fmaxf(top, ml[i].x);
+  } else {
+    top = wave_max((int)(threadIdx.x & 63) < sp.n ? ml[threadIdx.x & 63].x : -INFINITY);   // (at most 64 splits)
+  }
   float l = 0.0f;
   f32x4 o = {};
   const float* src = sp.o + row * sp.n * DP + col;
 #pragma unroll 4
-  for (int i = 0; i < sp.n; ++i) {
+  for (int i = grp; i < sp.n; i += G) {
     const float2 x = ml[i];
     // a split without weights left no O; one that saw NaN scores alone has m = -inf and l = NaN, which has to reach the result
     const float k = x.x == -INFINITY ? 0.0f : exp2_raw(x.x - top);
     l += x.y != x.y ? x.y : x.y * k;
     if (x.x != -INFINITY) o += *reinterpret_cast<const f32x4*>(src + (long)i * DP) * k;
+  }
+  if constexpr (G > 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[grp][lane][e] = o[e];
+    red[grp][lane][4] = l;
+    __syncthreads();
+    if (grp) return;
+    for (int i = 1; i < G; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += red[i][lane][e];
+      l += red[i][lane][4];
+    }
   }
   const long bh = row / p.tq, q = row % p.tq, b = bh / p.heads;
   const int h = (int)(bh % p.heads);
@@ -432,16 +451,11 @@ __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) 
   if (col == 0) p.lse[row] = none ? -INFINITY : (top + (__builtin_amdgcn_logf(l) - Row<T, DP>::SHIFT)) * kLn2;
 }
 
-constexpr int kMaxSplit = 64;
-
 // Few query rows (at most 32 in a sequence, a quarter of fwd_kernel's block): token_kernel.
 bool few_rows(int tq) { return tq <= 32; }
 
-// How the keys are split.  Few rows: enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or
-// more (the steps a block has cover its start and its merge).  Many rows: only where the card is not full, to 4/3 of what it holds (a
-// few long blocks more than it has CUs for would double the time), each split 16 tiles of 64 or more.  us with 1, 2, 4, 8 splits:
-// 6912 x 5 heads of 64 (270 blocks) 142, 121, 110, 116; 4608 x 5 (180) 84, 67, 59, 63; 1728 x 10 (140 blocks of 27 tiles) 32, 35,
-// 36, 38; 8 x 1728 x 10 (1120) 95, 140, 156, 240: the 32-bit parts of O cost their writing and reading.
+// How the keys of few rows are split: enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or
+// more (the steps a block has cover its start and its merge); of many rows, tile_splits.
 Split split_of(const dc_attn_desc* d) {
   Split s{1, 0, nullptr, nullptr};
   const long grp = d->heads / d->kv_heads;
@@ -452,9 +466,7 @@ Split split_of(const dc_attn_desc* d) {
     s.tiles = (int)((steps + n - 1) / n);
     s.n = (int)((steps + s.tiles - 1) / s.tiles);
   } else {
-    const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
-    const long slots = 256 * (d->d > 64 ? 2 : 3);   // blocks that the card holds at once
-    if (3 * blocks < 2 * slots) s.n = (int)min(min((4 * slots / 3 + blocks - 1) / blocks, max(tiles / 16, 1L)), (long)kMaxSplit);
+    s.n = tile_splits(d);
   }
   return s;
 }
@@ -473,9 +485,12 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
     const long blocks = (long)c.nb * c.heads * ((c.tq + 127) / 128) * s.n;
     hipLaunchKernelGGL((fwd_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   }
-  const long rows = (long)c.nb * c.heads * c.tq;
-  if (s.n > 1) hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)((rows * (DP / 4) + 255) / 256)), dim3(256), 0, st, c,
-                                   s, rows);
+  const long rows = (long)c.nb * c.heads * c.tq, threads = rows * (DP / 4);
+  if (s.n <= 1) return;
+  if (threads >= 65536)   // a thread to every lane of the card
+    hipLaunchKernelGGL((join_kernel<T, DP, 1>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, c, s, rows);
+  else
+    hipLaunchKernelGGL((join_kernel<T, DP, 1024 / DP>), dim3((unsigned)rows), dim3(256), 0, st, c, s, rows);
 }
 template <typename T, int DP>
 void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
@@ -483,6 +498,17 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
 }
 
 }  // namespace
+
+// Splits of the keys of blocks of 128 rows: only where the card is not full, to 4/3 of what it holds (a few long blocks more than it
+// has CUs for would double the time), each split 16 tiles of 64 or more.  Forward, us with 1, 2, 4, 8 splits: 6912 x 5 heads of 64
+// (270 blocks) 147, 108, 100, 106; 4608 x 5 (180) 86, 59, 50, 56; 1728 x 10 (140 blocks of 27 tiles) 33, 33, 31, 34; 8 x 1728 x 10
+// (1120) 94, 106, 125, 194: the 32-bit parts cost their writing and reading.
+int tile_splits(const dc_attn_desc* d) {
+  const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
+  const long slots = 256 * (d->d > 64 ? 2 : 3);   // blocks that the card holds at once
+  if (3 * blocks >= 2 * slots) return 1;
+  return (int)min(min((4 * slots / 3 + blocks - 1) / blocks, max(tiles / 16, 1L)), (long)kMaxSplit);
+}
 
 // Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.
 bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
