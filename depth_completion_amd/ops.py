@@ -7,6 +7,7 @@ PyTorch is used only for device memory and the current stream handle.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import json
 import os
 import sys
@@ -442,14 +443,17 @@ TYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 def _row_view(name: str, t, rows: int, cols: int, dtype, dev: int) -> tuple:
     """(pointer, row stride) of a 2-D operand that holds ``rows`` x ``cols`` of ``dtype`` on device ``dev``."""
     col = 0
-    if isinstance(t, Slice):
+    if t.__class__ is Slice:
         t, col = t.t, t.col
     shape, stride = t.shape, t.stride()
     if t.dtype is not dtype or len(shape) != 2 or shape[0] < rows or col < 0 or shape[1] - col < cols \
             or (stride[1] != 1 and cols > 1) or t.get_device() != dev:
         raise ValueError(f"{name}: needs {rows} rows of {cols} contiguous columns of {dtype} on device {dev}, "
                          f"got {tuple(shape)} from column {col} of {t.dtype} on {t.device}")
-    return t.data_ptr() + col * t.element_size(), stride[0] if shape[0] > 1 else -(-cols // 8) * 8
+    at = t.data_ptr()
+    if col:
+        at += col * t.element_size()
+    return at, stride[0] if shape[0] > 1 else -(-cols // 8) * 8
 
 
 def _flat(name: str, t, n: int, dtype, dev: int) -> int:
@@ -461,15 +465,21 @@ def _flat(name: str, t, n: int, dtype, dev: int) -> int:
     return t.data_ptr()
 
 
+@functools.lru_cache(None)
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
 def _launch(dev: int, name: str, *args):
     """An entry point on the current stream of ``dev``, which has to be the current device while a kernel is launched."""
-    f = getattr(_lib.load(), name)
+    f = _entry(name)
     if torch.cuda.current_device() == dev:
         status = f(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
             status = f(*args, torch._C._cuda_getCurrentRawStream(dev))
-    _lib.check(status, name)
+    if status:
+        _lib.check(status, name)
 
 
 def _scratch(need: int, dev: int) -> tuple:
@@ -482,9 +492,11 @@ def _scratch(need: int, dev: int) -> tuple:
 
 
 def _device_of(ctx: Ctx) -> int:
-    if ctx.device.type != "cuda":
-        raise ValueError(f"needs a GPU context, got one on {ctx.device}")
-    return ctx.device.index if ctx.device.index is not None else torch.cuda.current_device()
+    device = ctx.device
+    if device.type != "cuda":
+        raise ValueError(f"needs a GPU context, got one on {device}")
+    n = device.index
+    return torch.cuda.current_device() if n is None else n
 
 
 NO_GRADIENTS = (0,) * 8
@@ -520,9 +532,10 @@ def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, 
         grads = p + ld
     desc = PACK_ATTN.pack(
         kind, nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po, _flat("lse", lse, nb * heads * tq, f4, dev), ldq, ldk, ldv, ldo,
-        scale, softcap, _flat("slopes", slopes, heads, f4, dev), bool(causal), _flat("prefix", prefix, nb, i4, dev),
-        _flat("kv_len", kv_len, nb, i4, dev), _flat("doc_q", doc_q, nq, i4, dev), _flat("doc_k", doc_k, nk, i4, dev), *grads)
-    need = _lib.load().dc_attn_mask_ws_bytes(desc, back is not None)
+        scale, softcap, slopes is not None and _flat("slopes", slopes, heads, f4, dev), bool(causal),
+        prefix is not None and _flat("prefix", prefix, nb, i4, dev), kv_len is not None and _flat("kv_len", kv_len, nb, i4, dev),
+        doc_q is not None and _flat("doc_q", doc_q, nq, i4, dev), doc_k is not None and _flat("doc_k", doc_k, nk, i4, dev), *grads)
+    need = _entry("dc_attn_mask_ws_bytes")(desc, back is not None)
     keep, ws = _scratch(need, dev)
     _launch(dev, "dc_attn_mask_fwd" if back is None else "dc_attn_mask_bwd", desc, ws, need)
 
@@ -652,7 +665,7 @@ def resnorm_bwd(ctx: Ctx, x, y, rows: int, c: int, stats, dr, dh, dx, dy, *, fir
         for n, v, m in (("dr", dr, rows), ("dh", dh, rows), ("dx", dx, rows), ("dy", dy, rows), ("dgate", dgate, gates)))
     sums = (_flat(n, v, c, torch.float32, dev) for n, v in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2)))
     desc = PACK_RESNORM.pack(*common, 0, 0, a, s, eps, 0, 0, pst, pdr, pdh, pdx, pdy, pdg, *sums, lddr, lddh, lddx, lddy, lddg)
-    need = _lib.load().dc_resnorm_ws_bytes(desc)
+    need = _entry("dc_resnorm_ws_bytes")(desc)
     keep, ws = _scratch(need, dev)
     _launch(dev, "dc_resnorm_bwd", desc, ws, need)
     return dx, dy
