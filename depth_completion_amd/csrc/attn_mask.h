@@ -303,16 +303,17 @@ struct WaveRange {
     least = __builtin_amdgcn_readfirstlane(wave_min_i(live && q.mine >= 0 ? q.mine : 0x7fffffff));
     most = __builtin_amdgcn_readfirstlane(wave_max_i(live ? q.mine : -1));
   }
+  enum { NOTHING, WHOLE, MASKED };
   // id: the keys' documents, or NULL
-  __device__ __forceinline__ bool nothing(int t, const int* id) const {
-    if (t * 64 >= any) return true;
-    if (!id) return false;
-    const int i = id[threadIdx.x & 63];
-    return !__any(i >= least && i <= most);
-  }
-  __device__ __forceinline__ bool masked(int t, const int* id, const QueryBlock& q, bool live) const {
-    if (t * 64 + 64 > all) return true;
-    return id && (__any(live && id[0] != q.mine) || __any(id[threadIdx.x & 63] != id[0]));
+  __device__ __forceinline__ int look(int t, const int* id) const {
+    if (t * 64 >= any) return NOTHING;
+    bool masked = t * 64 + 64 > all;
+    if (id) {
+      const int i = id[threadIdx.x & 63];
+      if (!__any(i >= least && i <= most)) return NOTHING;
+      masked |= least != most || __any(i != least);
+    }
+    return masked ? MASKED : WHOLE;
   }
 };
 

@@ -109,12 +109,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   range_of.init(q, sees);
   // FIRST: the sum of P dP goes to `exact`; else dS K to dq
   float exact = 0.0f;
-  auto tile = [&](int t, auto B, const int* id, auto F) __attribute__((always_inline)) {
+  auto tile = [&](int t, auto B, const int* id, bool masked, auto F) __attribute__((always_inline)) {
     constexpr int buf = decltype(B)::value;
     constexpr bool FIRST = decltype(F)::value;
     const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
-    const bool masked = range_of.masked(t, id, q, sees);
     auto half_tile = [&](auto K) __attribute__((always_inline)) {
       constexpr int kb2 = decltype(K)::value;
       f32x16 s = {}, dp = {};
@@ -184,6 +183,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
       add(std::integral_constant<int, 1>{});
     };
     half_tile(std::integral_constant<int, 0>{});
+    __builtin_amdgcn_sched_barrier(0);   // (halves that overlap need 20 registers more, which spill: 8 x 4096 x 16 heads 2007 us for 2076)
     half_tile(std::integral_constant<int, 1>{});
   };
   auto step = [&](int t, auto B, auto F) __attribute__((always_inline)) {   // as the forward's
@@ -193,7 +193,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     tile_barrier();
     if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
     const int* id = ring.kid ? lds.ids[buf] : nullptr;
-    if (!range_of.nothing(t, id)) tile(t, B, id, F);
+    const int look = range_of.look(t, id);
+    if (look != WaveRange::NOTHING) tile(t, B, id, look == WaveRange::MASKED, F);
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   auto sweep = [&](auto F) __attribute__((always_inline)) {
@@ -372,9 +373,10 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     tile_barrier();
     const T* qt = tiles[buf];
     const T* dt = qt + TILE;
+    const int id = p.doc_q ? ids[buf][lane] : 0;
     // none of the wave's keys is seen from the tile
-    const bool nothing = from_first > t * 64 + shift + 63 ||
-                         (p.doc_q && !__any(ids[buf][lane] >= id_least && ids[buf][lane] <= id_most));
+    const bool nothing = from_first > t * 64 + shift + 63 || (p.doc_q && !__any(id >= id_least && id <= id_most));
+    const bool mixed = p.doc_q && (id_least != id_most || __any(id != id_least));
     // P and dS of 32 rows of the tile (a pair's: qoff is at the wave's own)
     auto weights = [&](int at, v8 (&pf)[2], v8 (&sf)[2]) __attribute__((always_inline)) {
       const int rows = at + 32 * second, row0 = rows + 4 * hh, pos0 = t * 64 + shift + row0;   // of the lane's first row
@@ -417,15 +419,13 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
         s[r] = exp2_raw(fmaf(s[r], SHAPED ? 1.0f : p.mul, nl[r >> 2][r & 3] + up));
         dp[r] *= is_half<T> ? s[r] * fs : s[r];
       }
-      bool partial = from_last > t * 64 + shift + rows;
-      if (p.doc_q) partial |= __any(ids[buf][0] != mine) || __any(ids[buf][lane] != ids[buf][0]);
-      if (partial) {
+      if (mixed || from_last > t * 64 + shift + rows) {
         asm volatile("" ::: "memory");   // a branch, not selects in every tile
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          int4 id = make_int4(0, 0, 0, 0);
-          if (p.doc_q) id = *reinterpret_cast<const int4*>(&ids[buf][row0 + 8 * g]);
-          const int id4[4] = {id.x, id.y, id.z, id.w};
+          int4 i4 = make_int4(0, 0, 0, 0);
+          if (p.doc_q) i4 = *reinterpret_cast<const int4*>(&ids[buf][row0 + 8 * g]);
+          const int id4[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (pos0 + 8 * g + e < from || (p.doc_q && id4[e] != mine)) {

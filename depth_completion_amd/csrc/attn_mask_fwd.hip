@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   vm_wait<0>();   // (the counts below are of tiles alone)
   if (t0 < t1) ring.load(p, lds, t0, 0);
   if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
-  auto tile = [&](int t, auto B, const int* id) __attribute__((always_inline)) {
+  auto tile = [&](int t, auto B, const int* id, bool masked) __attribute__((always_inline)) {
     constexpr int buf = decltype(B)::value;
     const T* kt = lds.tiles[buf];
     const T* vt = kt + TILE;
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
             s[kb2][r] = fmaf(-slope, fabsf(dist - (float)(32 * kb2 + (r & 3) + 8 * (r >> 2))), s[kb2][r]);
       }
     }
-    if (range_of.masked(t, id, q, q.live)) {
+    if (masked) {
       asm volatile("" ::: "memory");   // a branch, not selects in every tile
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2)
@@ -250,7 +250,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
     tile_barrier();
     if (S == 2 && t + 1 < t1) ring.load(p, lds, t + 1, buf ^ 1);
     const int* id = ring.kid ? lds.ids[buf] : nullptr;
-    if (!range_of.nothing(t, id)) tile(t, B, id);
+    const int look = range_of.look(t, id);
+    if (look != WaveRange::NOTHING) tile(t, B, id, look == WaveRange::MASKED);
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   for (int t = t0; t < t1; t += S) {
