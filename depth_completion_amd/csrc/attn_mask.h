@@ -187,7 +187,8 @@ __device__ __forceinline__ void dma_words(const void* base, void* lds, int last)
                                            lane <= last ? lane * 4u : Dma<bf16, 64>::OUT, 0, 0, 0);
 #endif
 }
-// Waits until at most N vector-memory operations of this wave are under way: those issued before the last N have landed.
+// Waits until at most N vector-memory operations of this wave are under way: those issued before the last N have landed (whatever
+// else was issued before them among these).
 template <int N>
 __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // All waves: what each has waited for is there for all, and what each has read may be overwritten.  (__syncthreads() would also
@@ -251,7 +252,8 @@ struct QueryBlock {
     w /= p.grp;
     part = w % splits;
     len = length_of(p, b);
-    qi = (nqb - 1 - w / splits) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    w /= splits;
+    qi = (p.causal ? nqb - 1 - w : w) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
     live = qi < p.tq;
     pos = qi + len - p.tq;
     lim = p.causal ? min(len, max(pos + 1, p.prefix ? p.prefix[b] : 0)) : len;

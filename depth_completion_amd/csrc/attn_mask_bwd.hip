@@ -198,7 +198,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   auto sweep = [&](auto F) __attribute__((always_inline)) {
-    vm_wait<0>();
     if (t0 < t1) ring.load(p, lds, t0, 0);
     if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
     for (int t = t0; t < t1; t += S) {
@@ -362,7 +361,6 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     ta[n] = tr_at<DP>(32 * n, lane);
     if (PAIR && !second) { ta[n].lo += TILE; ta[n].hi += TILE; }
   }
-  vm_wait<0>();
   if (i0 < i1) load(0);
   if (i0 + 1 < i1) load(1);
   int hg = nt ? i0 / nt : 0, t = nt ? t0 + i0 % nt : 0;

@@ -176,7 +176,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   WaveRange range_of;
   range_of.init(q, q.live);
 
-  vm_wait<0>();   // (the counts below are of tiles alone)
   if (t0 < t1) ring.load(p, lds, t0, 0);
   if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
   auto tile = [&](int t, auto B, const int* id, bool masked) __attribute__((always_inline)) {
@@ -541,7 +540,7 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   // row and block counts stay within 31 bits, splits included
   const long long rows = (long long)d->nb * d->heads * d->tq;
   if (rows >= (1LL << 30) || (long long)d->nb * d->tk * d->kv_heads >= (1LL << 30)) return DC_ERR_ARG;
-  const int hq = d->heads * d->d, hk = d->kv_heads * d->d;
+  const long long hq = (long long)d->heads * d->d, hk = (long long)d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
   if (d->ldk > (1 << 23) || d->ldv > (1 << 23)) return DC_ERR_ARG;   // 128 rows within 32 bits
   if (d->ldq % 8 || d->ldk % 8 || d->ldv % 8 || d->ldo % 8) return DC_ERR_ALIGN;
