@@ -362,6 +362,7 @@ struct KeyRing {
 
 // Host side: what both directions share (attn_mask_fwd.hip).
 constexpr int kMaxSplit = 64;
+bool shape_ok(const dc_attn_desc* d);
 int tile_splits(const dc_attn_desc* d);
 int make_call(const dc_attn_desc* d, Call& c, bool backward);
 long long summary_bytes(const dc_attn_desc* d, bool backward);

@@ -586,7 +586,7 @@ long long fwd_ws_bytes(const dc_attn_desc* d);
 using namespace dcm;
 
 extern "C" long long dc_attn_mask_ws_bytes(const dc_attn_desc* d, int backward) {
-  if (!d || d->nb <= 0 || d->tq <= 0 || d->tk <= 0 || d->heads <= 0 || d->kv_heads <= 0) return 0;
+  if (!shape_ok(d)) return 0;
   return backward ? bwd_ws_bytes(d) : fwd_ws_bytes(d);
 }
 

@@ -532,16 +532,20 @@ void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, h
                      d->tq, nq, d->nb, k);
 }
 
+// Lengths and heads that make sense, with row counts within 31 bits (splits included) and the threads of a launch within 32.
+bool shape_ok(const dc_attn_desc* d) {
+  if (!d || d->nb <= 0 || d->tq <= 0 || d->tk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return false;
+  const long long q = (long long)d->nb * d->heads, k = (long long)d->nb * d->kv_heads;
+  return q < (1LL << 30) / d->tq && k < (1LL << 30) / d->tk && q * ((d->tq + 127LL) / 128) < (1LL << 23) &&
+         k * ((d->tk + 127LL) / 128) < (1LL << 23);
+}
+
 int make_call(const dc_attn_desc* d, Call& c, bool backward) {
-  if (!d || !d->q || !d->k || !d->v || !d->o || !d->lse || d->type < 0 || d->type > 1) return DC_ERR_ARG;
-  if (d->nb <= 0 || d->tq <= 0 || d->tk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads) return DC_ERR_ARG;
+  if (!shape_ok(d) || !d->q || !d->k || !d->v || !d->o || !d->lse || d->type < 0 || d->type > 1) return DC_ERR_ARG;
   if (d->d <= 0 || d->d > 128 || d->d % 8 || !(d->scale > 0.0f) || !(d->softcap >= 0.0f)) return DC_ERR_ARG;
   if (!(d->scale <= 1e30f) || !(d->softcap <= 1e30f) || (d->softcap > 0.0f && !(d->scale / d->softcap <= 1e30f))) return DC_ERR_ARG;
   if (d->prefix && !d->causal) return DC_ERR_ARG;
   if (!d->doc_q != !d->doc_k) return DC_ERR_ARG;
-  // row and block counts stay within 31 bits, splits included
-  const long long rows = (long long)d->nb * d->heads * d->tq;
-  if (rows >= (1LL << 30) || (long long)d->nb * d->tk * d->kv_heads >= (1LL << 30)) return DC_ERR_ARG;
   const long long hq = (long long)d->heads * d->d, hk = (long long)d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
   if (d->ldk > (1 << 23) || d->ldv > (1 << 23)) return DC_ERR_ARG;   // 128 rows within 32 bits

@@ -437,7 +437,7 @@ extern "C" int dc_resnorm_fwd(const dc_resnorm_desc* d, void* stream) {
 }
 
 extern "C" long long dc_resnorm_ws_bytes(const dc_resnorm_desc* d) {
-  if (!d || d->rows <= 0 || d->c <= 0 || (d->gates > 0 && d->rows < d->gates)) return 0;
+  if (!d || d->rows <= 0 || d->c <= 0 || d->rows > (1LL << 40) / d->c || (d->gates > 0 && d->rows < d->gates)) return 0;
   Desc p{};
   plan(d, p);
   return ws_of(p);

@@ -107,25 +107,27 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotary p) {
 }
 
 template <typename T, int V>
-void launch(Rotary p, int interleaved, hipStream_t st) {
+int launch(Rotary p, int interleaved, hipStream_t st) {
   p.nturn = p.rot / (2 * V);
   p.units = p.nturn + (p.x == p.y ? 0 : ((p.d - p.rot) / V + 1) / 2);
+  if (p.rows >= (1LL << 32) / p.units) return DC_ERR_ARG;   // a launch's threads
   // enough threads to fill the card (2^19) come before heads that share their sines; past 8 heads these cost nothing
   const long all = p.rows * p.units * p.heads;
   p.hpt = (int)min((long)min(p.heads, 8), max(1L, all >> 19));
   const dim3 grid((unsigned)((p.rows * p.units + 255) / 256), (unsigned)((p.heads + p.hpt - 1) / p.hpt));
   if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, V, true>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((rotary_kernel<T, V, false>), grid, dim3(256), 0, st, p);
+  DC_CHECK_LAUNCH();
+  return DC_OK;
 }
 
 // Packs of 16 bytes where every pack of a head starts on one, else single columns.
 template <typename T>
-void launch_type(const Rotary& p, int interleaved, hipStream_t st) {
+int launch_type(const Rotary& p, int interleaved, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = p.rot % (2 * V) == 0 && p.off % V == 0 && p.d % V == 0 && p.ldx % V == 0 && p.ldy % V == 0 &&
                     (((uintptr_t)p.x | (uintptr_t)p.y) & 15) == 0;
-  if (wide) launch<T, V>(p, interleaved, st);
-  else launch<T, 1>(p, interleaved, st);
+  return wide ? launch<T, V>(p, interleaved, st) : launch<T, 1>(p, interleaved, st);
 }
 
 }  // namespace
@@ -136,17 +138,15 @@ extern "C" int dc_rotary(const dc_rotary_desc* r, void* stream) {
   if (r->rot <= 0 || r->rot % 2 || r->off < 0 || r->off > d || r->rot > d - r->off || d > 65536 || heads > 65535) return DC_ERR_ARG;
   if ((long long)heads * d >= (1LL << 31) || (r->x == r->y && r->ldx != r->ldy)) return DC_ERR_ARG;
   if (r->ldx < (long long)heads * d || r->ldy < (long long)heads * d || (!r->pos && r->t <= 0)) return DC_ERR_ARG;
-  if (r->rows > (1LL << 38) / d) return DC_ERR_ARG;   // the grid's blocks of 256 units
+  if (r->rows > (1LL << 38) / d) return DC_ERR_ARG;
   const uintptr_t size = r->type == 2 ? 4 : 2;
   if ((((uintptr_t)r->x | (uintptr_t)r->y) & (size - 1)) || ((uintptr_t)r->freqs & 7) || ((uintptr_t)r->pos & 3)) return DC_ERR_ALIGN;
   Rotary p{r->x, r->y, (long)r->ldx, (long)r->ldy, (long)r->rows, heads, d, r->off, r->rot, r->freqs, r->pos, r->pos0, r->t, r->mag,
            r->inverse, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
-  if (r->type == 0) launch_type<bf16>(p, r->interleaved, st);
-  else if (r->type == 1) launch_type<half>(p, r->interleaved, st);
-  else launch_type<float>(p, r->interleaved, st);
-  DC_CHECK_LAUNCH();
-  return DC_OK;
+  if (r->type == 0) return launch_type<bf16>(p, r->interleaved, st);
+  if (r->type == 1) return launch_type<half>(p, r->interleaved, st);
+  return launch_type<float>(p, r->interleaved, st);
 }
 
 extern "C" int dc_rotary_freqs(int rot, double theta, int scaling, double factor, double trained, double fast, double slow,

@@ -10,6 +10,7 @@ import ctypes as C
 import functools
 import json
 import os
+import struct
 import sys
 from dataclasses import dataclass
 from pathlib import Path
@@ -456,6 +457,14 @@ def _row_view(name: str, t, rows: int, cols: int, dtype, dev: int) -> tuple:
     return at, stride[0] if shape[0] > 1 else -(-cols // 8) * 8
 
 
+def _pack(layout, name: str, *fields) -> bytes:
+    """A descriptor's bytes; a count or stride that its field does not hold is refused."""
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:
+        raise ValueError(f"{name}: {e}") from None
+
+
 def _flat(name: str, t, n: int, dtype, dev: int) -> int:
     """Pointer of a contiguous operand of at least ``n`` values of ``dtype`` on device ``dev`` (0 for None)."""
     if t is None:
@@ -530,8 +539,8 @@ def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, 
         p, ld = zip(*(_row_view(n, t, rows, cols, dt, dev) for n, t, rows, cols in
                       (("dout", back[0], nq, hq), ("dq", back[1], nq, hq), ("dk", back[2], nk, hk), ("dv", back[3], nk, hk))))
         grads = p + ld
-    desc = PACK_ATTN.pack(
-        kind, nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po, _flat("lse", lse, nb * heads * tq, f4, dev), ldq, ldk, ldv, ldo,
+    desc = _pack(
+        PACK_ATTN, "attn_mask", kind, nb, tq, tk, heads, kv_heads, d, pq, pk, pv, po, _flat("lse", lse, nb * heads * tq, f4, dev), ldq, ldk, ldv, ldo,
         scale, softcap, slopes is not None and _flat("slopes", slopes, heads, f4, dev), bool(causal),
         prefix is not None and _flat("prefix", prefix, nb, i4, dev), kv_len is not None and _flat("kv_len", kv_len, nb, i4, dev),
         doc_q is not None and _flat("doc_q", doc_q, nq, i4, dev), doc_k is not None and _flat("doc_k", doc_k, nk, i4, dev), *grads)
@@ -597,8 +606,8 @@ def rotary(ctx: Ctx, x, rows: int, heads: int, d: int, freqs, y=None, *, pos=Non
     dev = _device_of(ctx)
     px, ldx = _row_view("x", x, rows, heads * d, dt, dev)
     py, ldy = (px, ldx) if y is None else _row_view("y", y, rows, heads * d, dt, dev)
-    _launch(dev, "dc_rotary", PACK_ROTARY.pack(
-        px, py, _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), ldx, ldy, rows,
+    _launch(dev, "dc_rotary", _pack(
+        PACK_ROTARY, "rotary", px, py, _flat("freqs", freqs, rot // 2, torch.float64, dev), _flat("pos", pos, rows, torch.int32, dev), ldx, ldy, rows,
         TYPE_IDS[dt], heads, d, off, rot, pos0, t, bool(interleaved), bool(inverse), mag))
     return x if y is None else y
 
@@ -643,7 +652,7 @@ def resnorm_fwd(ctx: Ctx, x, y, rows: int, c: int, r, h, stats, *, first: str = 
         raise ValueError("resnorm: h goes with a second norm")
     pr, ldr = _row_view("r", r, rows, c, dt, dev)
     ph, ldh = (0, 0) if h is None else _row_view("h", h, rows, c, dt, dev)
-    _launch(dev, "dc_resnorm_fwd", PACK_RESNORM.pack(*common, ldr, ldh, a, s, eps, pr, ph, pst, *NO_SUMS))
+    _launch(dev, "dc_resnorm_fwd", _pack(PACK_RESNORM, "resnorm", *common, ldr, ldh, a, s, eps, pr, ph, pst, *NO_SUMS))
     return r, h
 
 
@@ -664,7 +673,7 @@ def resnorm_bwd(ctx: Ctx, x, y, rows: int, c: int, stats, dr, dh, dx, dy, *, fir
         (0, 0) if v is None else _row_view(n, v, m, c, dt, dev)
         for n, v, m in (("dr", dr, rows), ("dh", dh, rows), ("dx", dx, rows), ("dy", dy, rows), ("dgate", dgate, gates)))
     sums = (_flat(n, v, c, torch.float32, dev) for n, v in (("dw1", dw1), ("db1", db1), ("dw2", dw2), ("db2", db2)))
-    desc = PACK_RESNORM.pack(*common, 0, 0, a, s, eps, 0, 0, pst, pdr, pdh, pdx, pdy, pdg, *sums, lddr, lddh, lddx, lddy, lddg)
+    desc = _pack(PACK_RESNORM, "resnorm", *common, 0, 0, a, s, eps, 0, 0, pst, pdr, pdh, pdx, pdy, pdg, *sums, lddr, lddh, lddx, lddy, lddg)
     need = _entry("dc_resnorm_ws_bytes")(desc)
     keep, ws = _scratch(need, dev)
     _launch(dev, "dc_resnorm_bwd", desc, ws, need)

@@ -461,7 +461,9 @@ int dc_complete(dc_session* s, const void* imgs_u8, const float* sparses, int n,
  * A visible key that is not finite may also reach other rows of its tile of 64 keys.  Sums and softmax statistics are fp32, the
  * weights P and dS are rounded to the type for the matrix units (dS of fp16 scaled by a power of two so that small gradients
  * keep their digits).  Gradients of shared key heads are summed over their query heads in a fixed order; no atomics.
- * type: 0 bf16, 1 fp16.  d: a multiple of 8.  Pointers 16-byte aligned, ld* multiples of 8.  Inputs and outputs may not overlap. */
+ * type: 0 bf16, 1 fp16.  d: a multiple of 8.  Pointers 16-byte aligned, ld* multiples of 8.  Inputs and outputs may not overlap.
+ * nb heads tq and nb kv_heads tk below 2^30, nb heads (and kv_heads) times blocks of 128 rows below 2^23, ldk and ldv (in the
+ * backward ldq and lddo too) at most 2^23. */
 typedef struct dc_attn_desc {
   int type, nb, tq, tk, heads, kv_heads, d;
   const void *q, *k, *v;        /* [nb tq][ldq] head h at column h d; [nb tk][ldk], [nb tk][ldv] */
@@ -488,7 +490,8 @@ int dc_attn_mask_bwd(const dc_attn_desc* d, void* ws, long long ws_bytes, void* 
  * i < rot / 2, and multiplied by mag: pairs (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; inverse turns back, which is the
  * gradient (dL/dx from dL/dy).  y may be x (same ldx); else the other columns are copied.  Angles are formed in 64 bits.
  * type: 0 bf16, 1 fp16, 2 fp32.  pos: int [rows], or NULL: row r stands at pos0 + r % t.  freqs: [rot / 2] in device memory.
- * Any d, off and even rot; 16-byte accesses where base, ld, d and off allow them and rot is whole packs. */
+ * Any d, off and even rot; 16-byte accesses where base, ld, d and off allow them and rot is whole packs.  rows times the pairs
+ * (or packs of pairs) and copied columns of a head below 2^32. */
 typedef struct dc_rotary_desc {
   const void* x;
   void* y;

@@ -101,3 +101,24 @@ def test_packed_descriptors(desc, pack):
     values = [i + 1 for i in range(len(desc._fields_))]
     d = desc(*values)
     assert pack.size == C.sizeof(desc) and pack.pack(*values) == bytes(d)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(kv_heads=8), dict(kv_heads=3), dict(tq=0), dict(nb=1 << 30, heads=1 << 30, kv_heads=1 << 30, tq=16), dict(nb=1 << 22, tq=1)])
+@pytest.mark.parametrize("back", [0, 1])
+def test_scratch_of_impossible_shapes(kw, back):
+    """More key heads than heads, products that pass 64 bits, more blocks than a launch has: no scratch, and no division by none."""
+    d = descriptor(**kw)
+    assert _lib.load().dc_attn_mask_ws_bytes(C.byref(d), back) == 0
+    assert _lib.load().dc_attn_mask_fwd(C.byref(d), 4096, 1 << 40, None) == ARG
+
+
+def test_fields_that_do_not_hold():
+    """Numbers beyond a descriptor's fields are refused as arguments, not as an error of the packing."""
+    fields = [0] * len(_lib.AttnDesc._fields_)
+    for i, v in ((1, 1 << 31), (3, -1 << 40), (12, 1 << 31)):
+        bad = list(fields)
+        bad[i] = v
+        with pytest.raises(ValueError, match="attn"):
+            ops._pack(_lib.PACK_ATTN, "attn_mask", *bad)
+    assert ops._pack(_lib.PACK_ATTN, "attn_mask", *fields) == bytes(_lib.AttnDesc())

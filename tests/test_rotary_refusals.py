@@ -61,3 +61,11 @@ def test_entry_refuses(kw, status):
 
 def test_no_null_descriptor():
     assert _lib.load().dc_rotary(None, None) == 1
+
+
+@pytest.mark.parametrize("rows,y", [(1 << 30, 8192), (1 << 27, 8194)])
+def test_entry_refuses_more_threads_than_a_launch_has(rows, y):
+    """2^32 packs of pairs, and as many single pairs where the rows start between two packs."""
+    a = _lib.RotaryDesc(x=4096, ldx=128, y=y, ldy=128, type=0, rows=rows, heads=2, d=64, off=0, rot=64, freqs=4096, pos=None, pos0=0,
+                        t=4, mag=1.0, interleaved=0, inverse=0)
+    assert _lib.load().dc_rotary(C.byref(a), None) == 1
