@@ -398,8 +398,9 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
 }
 
 // A row's splits joined, four columns to a lane.  G groups of lanes take every G-th split each and are added in order: one group to a
-// row where there are many rows, a whole block where there are few (one token over 131072 keys in 64
-// splits: 142 us with one group, 119 with eight).
+// row where there are many rows, a whole block where there are few.  us of calls with one group and with a block to a row: one token
+// over 131072 keys in 64 splits 142 119, 4 tokens over 4096 keys, 32/8 heads of 128, 19 16; 512 over 4096, 16 of 64, 32 38; 4608 x 5
+// of 64 45 61.
 template <typename T, int DP, int G>
 __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) {
   constexpr int LANES = DP / 4;
@@ -451,8 +452,10 @@ __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) 
   if (col == 0) p.lse[row] = none ? -INFINITY : (top + (__builtin_amdgcn_logf(l) - Row<T, DP>::SHIFT)) * kLn2;
 }
 
-// Few query rows (at most 32 in a sequence, a quarter of fwd_kernel's block): token_kernel.
-bool few_rows(int tq) { return tq <= 32; }
+// Few query rows (at most 64 in a sequence, half of fwd_kernel's block): token_kernel.  us with token_kernel and fwd_kernel for 8, 32, 64
+// and 96 rows a sequence: 1 x 4096 keys, 32/8 heads of 128: 16 33, 17 34, 27 36, 35 39; 8 x 4096, 32/8 of 128: 42 100, 74 104, 113 114,
+// 157 121; 16 x 2048, 16/2 of 64: 13 27, 25 27, 33 33, 43 37; 4 x 1000, 20 of 64: 13 22, 14 22, 16 23, 17 23.
+bool few_rows(int tq) { return tq <= 64; }
 
 // How the keys of few rows are split: enough blocks to give every CU four where the keys allow it, each with 4 steps of 128 keys or
 // more (the steps a block has cover its start and its merge); of many rows, tile_splits.
@@ -512,7 +515,8 @@ int tile_splits(const dc_attn_desc* d) {
   return (int)min(min(n, max(tiles / 16, 1L)), (long)kMaxSplit);
 }
 
-// Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.
+// Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.  us with and
+// without, 10 heads of 64, forward and gradients: 8 x 256 in 2 documents 47 38, 4 x 512 in 1 76 70, in 4 47 51, 4 x 1024 in 2 112 131.
 bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
 // the queries' tiles are the keys' where the documents are the same rows; the forward does not ask for them
 bool query_tiles(const dc_attn_desc* d, bool backward) { return backward && !(d->doc_q == d->doc_k && d->tq == d->tk); }
