@@ -40,6 +40,7 @@ struct Call {
   int causal;
   const int *prefix, *kv_len, *doc_q, *doc_k;
   const int4 *sum_q, *sum_k;   // per 64 rows: least and largest document, whether a row is in none (NULL: short rows, no documents)
+  const int *order_q, *order_k;   // blocks of 128 rows of all sequences, those with the most tiles first (NULL: not sorted)
 };
 
 // Scores of a call with a cap, in units of log2: cap2 tanh(scale s / cap), with tanh(x) = 1 - 2 r, r = 1 / (1 + e^2x): absolute error
@@ -202,15 +203,25 @@ __device__ __forceinline__ void tile_barrier() {
 __device__ __forceinline__ int length_of(const Call& p, int b) {
   return p.kv_len ? min(max(p.kv_len[b], 0), p.tk) : p.tk;
 }
+// over a wave, in every lane, by cross-lane moves
+template <int CTRL>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+template <typename F>
+__device__ __forceinline__ int lanes_reduce(int v, F&& f) {
+  v = f(v, moved<0xb1>(v));    // lane ^ 1
+  v = f(v, moved<0x4e>(v));    // lane ^ 2
+  v = f(v, moved<0x141>(v));   // the other four of eight
+  v = f(v, moved<0x140>(v));   // the other eight of sixteen
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = f((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f((int)r[0], (int)r[1]);
+}
 __device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
+  return lanes_reduce(v, [](int a, int b) __attribute__((always_inline)) { return min(a, b); });
 }
 __device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
+  return lanes_reduce(v, [](int a, int b) __attribute__((always_inline)) { return max(a, b); });
 }
 // the sum / maximum of a value over lanes l and l ^ 32, which hold the two halves of a query's scores
 __device__ __forceinline__ float pair_sum(float x) {
@@ -222,18 +233,31 @@ __device__ __forceinline__ float pair_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Blocks are dealt to the eight XCDs in turn.  Units (a key head of a sequence) go to an XCD whole as far as they come by eights, so
-// that the blocks that read the same keys share an L2; the blocks of the rest are spread over all (whole units left over would leave
-// XCDs idle: 5 heads of 71 blocks, half of them long, 169 us with runs of blocks to an XCD).
-__device__ __forceinline__ void unit_of(int units, int per_unit, int& unit, int& r) {
-  const int whole = units / 8 * 8, n = whole * per_unit, i = blockIdx.x;
-  if (i < n) {
-    unit = i / 8 / per_unit * 8 + i % 8;
-    r = i / 8 % per_unit;
+// Which unit (a key head of a sequence, or of all where the items are sorted), item (its blocks of rows, the longest first) and part of
+// an item a block takes.  Blocks are dealt to the eight XCDs in turn, and by these to their CUs in turn, 256 at a time.
+//   Many blocks (or the decode's): units go to an XCD whole as far as they come by eights, so that the blocks that read the same keys
+//   share an L2; the blocks of the rest are spread over all (whole units left over would leave XCDs idle).
+//   At most 1536, which are on the card at once or nearly, so that no later block evens out what the first have left: the longest items
+//   of all units first, and the second 256 in the reverse order (`fold`), a short block beside each long one.  Causal, forward and
+//   gradients, us by whole units and so: 4096 x 16 heads of 64 306 255, 2 x 2048 x 16 170 145, 8 x 1024 x 16 210 191, 4608 x 5 155 134.
+constexpr int kSpread = 1536;
+struct Place { int unit, item, part; };
+__device__ __forceinline__ Place place_of(int units, int items, int parts, bool spread, bool fold) {
+  Place at;
+  int i = blockIdx.x;
+  if (spread) {
+    const int j = i / 8, end = min((int)gridDim.x, 512) / 8;
+    if (fold && j >= 32 && j < end) i = (31 + end - j) * 8 + i % 8;
+    at.unit = i % units;
+    i /= units;
   } else {
-    unit = whole + (i - n) / per_unit;
-    r = (i - n) % per_unit;
+    const int per_unit = items * parts, whole = units / 8 * 8, n = whole * per_unit;
+    at.unit = i < n ? i / 8 / per_unit * 8 + i % 8 : whole + (i - n) / per_unit;
+    i = i < n ? i / 8 % per_unit : (i - n) % per_unit;
   }
+  at.part = i % parts;
+  at.item = i / parts;
+  return at;
 }
 
 // The query rows of a block of fwd_kernel or dq_kernel: 4 x 32 rows of one head.
@@ -241,19 +265,17 @@ struct QueryBlock {
   int b, kh, h, part, qi, len, pos, lim, mine;   // lim: the lane's query sees the keys below it (of its document `mine`)
   bool live;
   int4 sum0;   // the thread's first tile summary, read along with the rows
-  // of a unit's tiles of 128 rows (the longest rows of a causal call first) x splits x heads of the group
   __device__ __forceinline__ void init(const Call& p, int splits) {
     const int nqb = (p.tq + 127) / 128;
-    int unit, w;
-    unit_of(p.nb * p.kvh, nqb * p.grp * splits, unit, w);
-    b = unit / p.kvh;
-    kh = unit % p.kvh;
-    h = kh * p.grp + w % p.grp;
-    w /= p.grp;
-    part = w % splits;
+    const Place at = p.order_q ? place_of(p.kvh, p.nb * nqb, p.grp * splits, true, true)
+                               : place_of(p.nb * p.kvh, nqb, p.grp * splits, gridDim.x <= kSpread, true);
+    const int item = p.order_q ? p.order_q[at.item] : p.causal ? nqb - 1 - at.item : at.item;
+    b = p.order_q ? item / nqb : at.unit / p.kvh;
+    kh = at.unit % p.kvh;
+    h = kh * p.grp + at.part % p.grp;
+    part = at.part / p.grp;
     len = length_of(p, b);
-    w /= splits;
-    qi = (p.causal ? nqb - 1 - w : w) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    qi = (p.order_q ? item % nqb : item) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
     live = qi < p.tq;
     pos = qi + len - p.tq;
     lim = p.causal ? min(len, max(pos + 1, p.prefix ? p.prefix[b] : 0)) : len;

@@ -269,10 +269,13 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   __shared__ int range[4], blind_rows;
   __shared__ float scratch[8];
   const int lane = threadIdx.x & 63, hh = lane >> 5, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), second = PAIR ? wid & 1 : 0;
-  int unit, w;
-  unit_of(p.nb * p.kvh, (p.tk + 127) / 128 * bk.nk, unit, w);
-  const int b = unit / p.kvh, kh = unit % p.kvh;
-  const int part = w % bk.nk, k0 = w / bk.nk * 128;   // the first keys of a causal call have the longest columns
+  // (the first keys of a causal call have the longest columns; 128 columns have one block to a CU, and what comes later fills the gaps)
+  const int nkb = (p.tk + 127) / 128;
+  const Place place = p.order_k ? place_of(p.kvh, p.nb * nkb, bk.nk, true, !PAIR)
+                                : place_of(p.nb * p.kvh, nkb, bk.nk, gridDim.x <= kSpread, !PAIR);
+  const int item = p.order_k ? p.order_k[place.item] : place.item;
+  const int b = p.order_k ? item / nkb : place.unit / p.kvh, kh = place.unit % p.kvh;
+  const int part = place.part, k0 = (p.order_k ? item % nkb : item) * 128;
   const int len = length_of(p, b), pre = p.prefix ? p.prefix[b] : 0, shift = len - p.tq;
   const int key = k0 + (PAIR ? wid >> 1 : wid) * 32 + (lane & 31);
   const int mine = p.doc_q ? (key < len ? p.doc_k[(long)b * p.tk + key] : -1) : 0;

@@ -31,6 +31,82 @@ __global__ __launch_bounds__(256) void summary_kernel(const int* doc_k, int tk, 
   if (lane == 0) *to = make_int4(lo, hi, none, 0);
 }
 
+// The same tiles by one block, for calls of few blocks, and the orders in which these are taken: blocks of 128 rows by the number of the
+// other side's tiles that their documents meet (a prefix left out), the most first.  order_k: NULL in the forward.  Packed documents
+// in unlucky order cost what the longest CU has: 9001 x 5 heads with the longest document last 157 us unsorted, 91 with it first.
+constexpr int kSorted = 1024;   // tiles, and blocks of either side
+__global__ __launch_bounds__(1024) void plan_kernel(Call p, int nk, int nq, int4* out, int* order_q, int* order_k) {
+  __shared__ int4 sum[kSorted];
+  __shared__ int cost[kSorted];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // a tile to a wave, eight on their way
+  auto side = [&](const int* doc, int rows, int nt, int4* to, int4* copy) __attribute__((always_inline)) {
+    int b = 0, t = wid;   // of the wave's next tile
+    auto settle = [&]() __attribute__((always_inline)) {
+      while (t >= nt && b < p.nb) { t -= nt; ++b; }
+    };
+    settle();
+    while (b < p.nb) {
+      int id[8], at[8], left[8], m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (b >= p.nb) break;
+        left[k] = rows - t * 64;
+        at[k] = b * nt + t;
+        id[k] = doc[(long)b * rows + t * 64 + min(lane, left[k] - 1)];
+        t += 16;
+        settle();
+        m = k + 1;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= m) break;
+        // (lanes behind the last row have its document)
+        const int lo = wave_min_i(id[k] >= 0 ? id[k] : 0x7fffffff), hi = wave_max_i(max(id[k], -1));
+        const bool none = __any(id[k] < 0);
+        if (lane == 0) to[at[k]] = copy[at[k]] = make_int4(lo, hi, none, 0);
+      }
+    }
+  };
+  side(p.doc_k, p.tk, nk, out, sum);
+  if (nq) side(p.doc_q, p.tq, nq, out + p.nb * nk, sum + p.nb * nk);
+  const int4* sum_q = nq ? sum + p.nb * nk : sum;
+  const int nt_q = (p.tq + 63) / 64;
+  auto sort = [&](bool keys, int* order) __attribute__((always_inline)) {   // an item to a wave
+    const int nt = keys ? nk : nt_q, blocks = (nt + 1) / 2, items = p.nb * blocks;
+    __syncthreads();
+    int b = 0, w = wid;
+    for (int i = wid; i < items; i += 16, w += 16) {
+      while (w >= blocks) { w -= blocks; ++b; }
+      const int len = length_of(p, b), shift = len - p.tq;
+      const int4 *own = (keys ? sum : sum_q) + b * nt, first = own[2 * w], second = own[min(2 * w + 1, nt - 1)];
+      const int least = min(first.x, second.x), most = max(first.y, second.y);
+      const int4* other = keys ? sum_q + b * nt_q : sum + b * nk;
+      const int seen = min(len, p.causal ? w * 128 + 128 + shift : len);   // keys that the queries w 128 .. see
+      const int from = keys && p.causal ? max(0, w * 128 - shift) / 64 : 0;
+      const int to = !keys ? (max(seen, 0) + 63) / 64 : w * 128 < len ? nt_q : 0;
+      int c = 0;
+      for (int t = from; t < to; t += 64) {
+        const int4 o = other[min(t + lane, to - 1)];
+        c += __popcll(__ballot(t + lane < to && o.y >= least && o.x <= most));
+      }
+      if (lane == 0) cost[i] = c;
+    }
+    __syncthreads();
+    for (int i = wid; i < items; i += 16) {
+      const int c = cost[i];
+      int rank = 0;
+      for (int j = 0; j < items; j += 64) {
+        const int o = cost[min(j + lane, items - 1)];
+        rank += __popcll(__ballot(j + lane < items && (o > c || (o == c && j + lane < i))));
+      }
+      if (lane == 0) order[rank] = i;
+    }
+  };
+  sort(false, order_q);
+  if (order_k) sort(true, order_k);
+}
+
 // Running softmax of one lane's query over tiles of scores.  m is the reference of the weights 2^(x - m); it follows the row's
 // maximum only when that has grown by more than 8 log2 e, so that most tiles leave O alone.  A row that has seen no key keeps
 // m = -inf and weights of zero.  fp16 weights are held 2^4 times as large: with the slack they reach 2^15.6, and one key among
@@ -275,10 +351,9 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int lane = threadIdx.x & 63, hh = lane >> 5, wid = threadIdx.x >> 6;
   const int rows = p.tq * p.grp, nrb = (rows + 31) / 32;
-  int unit, w;
-  unit_of(p.nb * p.kvh, nrb * sp.n, unit, w);
-  const int b = unit / p.kvh, kh = unit % p.kvh;
-  const int rb = w % nrb, part = w / nrb;
+  const Place at = place_of(p.nb * p.kvh, sp.n, nrb, false, false);
+  const int b = at.unit / p.kvh, kh = at.unit % p.kvh;
+  const int rb = at.part, part = at.item;
   const int r = rb * 32 + (lane & 31);
   const bool live = r < rows;
   const int qi = live ? r / p.grp : 0, h = kh * p.grp + (live ? r % p.grp : 0);
@@ -518,12 +593,20 @@ int tile_splits(const dc_attn_desc* d) {
 // Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.  us with and
 // without, 10 heads of 64, forward and gradients: 8 x 256 in 2 documents 47 38, 4 x 512 in 1 76 70, in 4 47 51, 4 x 1024 in 2 112 131.
 bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
-// the queries' tiles are the keys' where the documents are the same rows; the forward does not ask for them
-bool query_tiles(const dc_attn_desc* d, bool backward) { return backward && !(d->doc_q == d->doc_k && d->tq == d->tk); }
+// Blocks are sorted where they are few (place_of) and one block can look at all tiles.
+bool sorted(const dc_attn_desc* d) {
+  const long nk = (d->tk + 63L) / 64, nq = (d->tq + 63L) / 64;
+  return summarised(d) && !few_rows(d->tq) && d->nb * (nk + nq) <= kSorted && (long)d->nb * d->heads * ((nq + 1) / 2) <= kSpread;
+}
+// the queries' tiles are the keys' where the documents are the same rows; the forward asks for them only to sort
+bool query_tiles(const dc_attn_desc* d, bool backward) {
+  return (backward || sorted(d)) && !(d->doc_q == d->doc_k && d->tq == d->tk);
+}
 
 long long summary_bytes(const dc_attn_desc* d, bool backward) {
   if (!summarised(d)) return 0;
-  return 16LL * d->nb * ((d->tk + 63L) / 64 + (query_tiles(d, backward) ? (d->tq + 63L) / 64 : 0));
+  const long long sums = 16LL * d->nb * ((d->tk + 63L) / 64 + (query_tiles(d, backward) ? (d->tq + 63L) / 64 : 0));
+  return sums + (sorted(d) ? (4LL * d->nb * ((d->tk + 127L) / 128 + (d->tq + 127L) / 128) + 15) / 16 * 16 : 0);
 }
 
 void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st) {
@@ -532,6 +615,13 @@ void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, h
   int4* k = reinterpret_cast<int4*>(ws);
   c.sum_k = k;
   c.sum_q = nq ? k + (long)d->nb * nk : k;
+  if (sorted(d)) {
+    int* order = reinterpret_cast<int*>(k + (long)d->nb * (nk + nq));
+    c.order_q = order;
+    c.order_k = backward ? order + (long)d->nb * ((d->tq + 127) / 128) : nullptr;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, c, nk, nq, k, order, const_cast<int*>(c.order_k));
+    return;
+  }
   hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * (nk + nq) + 3) / 4)), dim3(256), 0, st, d->doc_k, d->tk, nk, d->doc_q,
                      d->tq, nq, d->nb, k);
 }
