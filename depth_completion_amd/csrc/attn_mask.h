@@ -40,7 +40,10 @@ struct Call {
   int causal;
   const int *prefix, *kv_len, *doc_q, *doc_k;
   const int4 *sum_q, *sum_k;   // per 64 rows: least and largest document, whether a row is in none (NULL: short rows, no documents)
-  const int *order_q, *order_k;   // blocks of 128 rows of all sequences, those with the most tiles first (NULL: not sorted)
+  // documents in few blocks: (block of 128 rows, part | parts << 8) or (-1, 0), the longest parts first; parts of each block (NULL: not)
+  const int2 *list_q, *list_k;
+  const int *parts_q, *parts_k;
+  int entries_q, entries_k;
 };
 
 // Scores of a call with a cap, in units of log2: cap2 tanh(scale s / cap), with tanh(x) = 1 - 2 r, r = 1 / (1 + e^2x): absolute error
@@ -260,22 +263,32 @@ __device__ __forceinline__ Place place_of(int units, int items, int parts, bool 
   return at;
 }
 
+// (the same for all lanes, which the compiler does not see of a load)
+__device__ __forceinline__ int2 entry_of(const int2* list, int i) {
+  const int2 e = list[i];
+  return make_int2(__builtin_amdgcn_readfirstlane(e.x), __builtin_amdgcn_readfirstlane(e.y));
+}
+
 // The query rows of a block of fwd_kernel or dq_kernel: 4 x 32 rows of one head.
 struct QueryBlock {
-  int b, kh, h, part, qi, len, pos, lim, mine;   // lim: the lane's query sees the keys below it (of its document `mine`)
-  bool live;
+  int b, kh, h, part, parts, qi, len, pos, lim, mine;   // lim: the lane's query sees the keys below it (of its document `mine`)
+  bool live, idle;   // idle: the block has nothing to do
   int4 sum0;   // the thread's first tile summary, read along with the rows
   __device__ __forceinline__ void init(const Call& p, int splits) {
     const int nqb = (p.tq + 127) / 128;
-    const Place at = p.order_q ? place_of(p.kvh, p.nb * nqb, p.grp * splits, true, true)
-                               : place_of(p.nb * p.kvh, nqb, p.grp * splits, gridDim.x <= kSpread, true);
-    const int item = p.order_q ? p.order_q[at.item] : p.causal ? nqb - 1 - at.item : at.item;
-    b = p.order_q ? item / nqb : at.unit / p.kvh;
+    const Place at = p.list_q ? place_of(p.kvh, p.entries_q, p.grp, true, true)
+                              : place_of(p.nb * p.kvh, nqb, p.grp * splits, gridDim.x <= kSpread, true);
+    const int2 e = p.list_q ? entry_of(p.list_q, at.item)
+                            : make_int2(p.causal ? nqb - 1 - at.item : at.item, at.part / p.grp | splits << 8);
+    const int item = max(e.x, 0);
+    idle = e.x < 0;
+    b = p.list_q ? item / nqb : at.unit / p.kvh;
     kh = at.unit % p.kvh;
     h = kh * p.grp + at.part % p.grp;
-    part = at.part / p.grp;
+    part = e.y & 255;
+    parts = e.y >> 8;
     len = length_of(p, b);
-    qi = (p.order_q ? item % nqb : item) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    qi = (p.list_q ? item % nqb : item) * 128 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
     live = qi < p.tq;
     pos = qi + len - p.tq;
     lim = p.causal ? min(len, max(pos + 1, p.prefix ? p.prefix[b] : 0)) : len;
@@ -286,9 +299,10 @@ struct QueryBlock {
       sum0 = p.sum_k[(long)b * nt + min((int)threadIdx.x, nt - 1)];
     }
   }
-  // The 64-key tiles [t0, t1) in which some row with `sees` may see a key; holes: some key of theirs is (or may be) in no document.
-  __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1, bool& holes) const {
-    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; range[4] = 0; range[5] = 0; }
+  // The 64-key tiles [t0, t1) in which some row with `sees` may see a key; holes: the first of them with a key that is (or may be)
+  // in no document.
+  __device__ __forceinline__ void tiles(const Call& p, bool sees, int* range, int& t0, int& t1, int& holes) const {
+    if (threadIdx.x == 0) { range[0] = 0x7fffffff; range[1] = 0; range[2] = 0x7fffffff; range[3] = -1; range[4] = 0; range[5] = 0x7fffffff; }
     __syncthreads();
     const int most = wave_max_i(sees ? lim : 0);
     if ((threadIdx.x & 63) == 0) atomicMax(&range[1], most);
@@ -309,10 +323,10 @@ struct QueryBlock {
       t1 = range[4];
       t0 = min(range[0], t1);
       for (int t = threadIdx.x; t < t1; t += 256)
-        if (t >= t0 && (t < 256 ? sum0 : sum[t]).z) range[5] = 1;
+        if (t >= t0 && (t < 256 ? sum0 : sum[t]).z) { atomicMin(&range[5], t); break; }
       __syncthreads();
     }
-    holes = p.doc_q && (!p.sum_k || __builtin_amdgcn_readfirstlane(range[5]));
+    holes = p.doc_q && !p.sum_k ? 0 : __builtin_amdgcn_readfirstlane(range[5]);
     t0 = __builtin_amdgcn_readfirstlane(t0);
     t1 = __builtin_amdgcn_readfirstlane(t1);
   }
@@ -353,10 +367,9 @@ struct KeyRing {
   const T *kb, *vb;
   const int* kid;
   const int4* sum;
-  int len;
-  bool holes;
-  __device__ __forceinline__ void init(const Call& p, const QueryBlock& q, bool some_holes) {
-    holes = some_holes;
+  int len, holes;
+  __device__ __forceinline__ void init(const Call& p, const QueryBlock& q, int first_hole) {
+    holes = first_hole;
     k.init(p.ldk, p.d);
     v.init(p.ldv, p.d);
     kb = (const T*)p.k + (long)q.b * p.tk * p.ldk + q.kh * p.d;
@@ -369,8 +382,9 @@ struct KeyRing {
   __device__ __forceinline__ void load(const Call& p, Lds& lds, int t, int buf) const {
     const int r0 = t * 64, last = len - 1 - r0;
     const T *ka = kb + (long)r0 * p.ldk, *va = vb + (long)r0 * p.ldv;
-    // a key in no document: its row may hold anything (asked for each tile, the answer would be waited for in each)
-    if (holes && (!sum || sum[t].z)) {
+    // a key in no document: its row may hold anything (asked for each tile, the answer would be waited for in each; rows in none lie
+    // behind the last document, as a rule)
+    if (t >= holes && (!sum || sum[t].z)) {
       auto keep = [&](int r) __attribute__((always_inline)) { return kid[min(r0 + r, len - 1)] >= 0; };
       k.load_some(ka, lds.tiles[buf], last, keep);
       v.load_some(va, lds.tiles[buf] + TILE, last, keep);
@@ -386,6 +400,8 @@ struct KeyRing {
 constexpr int kMaxSplit = 64;
 bool shape_ok(const dc_attn_desc* d);
 int tile_splits(const dc_attn_desc* d);
+struct Lists { bool on; int items_q, items_k, entries_q, entries_k, most_q, most_k; };   // most: parts of a block
+Lists lists_of(const dc_attn_desc* d);
 int make_call(const dc_attn_desc* d, Call& c, bool backward);
 long long summary_bytes(const dc_attn_desc* d, bool backward);
 void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st);

@@ -56,6 +56,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   QueryBlock q;
   q.init(p, bk.nq);
+  if (q.idle) return;
   const long row = ((long)q.b * p.heads + q.h) * p.tq + (q.live ? q.qi : 0), trow = (long)q.b * p.tq + (q.live ? q.qi : 0);
   const float lse = p.lse[row];
   const bool sees = q.live && lse != -INFINITY;
@@ -82,10 +83,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   if (lane == 0 && q.part == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
   const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
   int t0, t1;
-  bool holes;
+  int holes;
   q.tiles(p, sees, range, t0, t1, holes);
-  if (bk.nq > 1) {
-    const int each = (t1 - t0 + bk.nq - 1) / bk.nq;
+  if (q.parts > 1) {
+    const int each = (t1 - t0 + q.parts - 1) / q.parts;
     t0 = min(t1, t0 + q.part * each);
     t1 = min(t1, t0 + each);
   }
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   if (!q.live) return;
   const float k = ds_scale(p) / f;
   T* out = (T*)p.dq + ((long)q.b * p.tq + q.qi) * p.lddq + q.h * p.d;
-  float* pq = bk.nq > 1 ? bk.part_q + ((((long)q.part * p.nb + q.b) * p.tq + q.qi) * p.heads + q.h) * DP : nullptr;
+  float* pq = q.parts > 1 ? bk.part_q + ((((long)q.part * p.nb + q.b) * p.tq + q.qi) * p.heads + q.h) * DP : nullptr;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -271,11 +272,12 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   const int lane = threadIdx.x & 63, hh = lane >> 5, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), second = PAIR ? wid & 1 : 0;
   // (the first keys of a causal call have the longest columns; 128 columns have one block to a CU, and what comes later fills the gaps)
   const int nkb = (p.tk + 127) / 128;
-  const Place place = p.order_k ? place_of(p.kvh, p.nb * nkb, bk.nk, true, !PAIR)
-                                : place_of(p.nb * p.kvh, nkb, bk.nk, gridDim.x <= kSpread, !PAIR);
-  const int item = p.order_k ? p.order_k[place.item] : place.item;
-  const int b = p.order_k ? item / nkb : place.unit / p.kvh, kh = place.unit % p.kvh;
-  const int part = place.part, k0 = (p.order_k ? item % nkb : item) * 128;
+  const Place place = p.list_k ? place_of(p.kvh, p.entries_k, 1, true, !PAIR)
+                               : place_of(p.nb * p.kvh, nkb, bk.nk, gridDim.x <= kSpread, !PAIR);
+  const int2 e = p.list_k ? entry_of(p.list_k, place.item) : make_int2(place.item, place.part | bk.nk << 8);
+  if (e.x < 0) return;
+  const int b = p.list_k ? e.x / nkb : place.unit / p.kvh, kh = place.unit % p.kvh;
+  const int part = e.y & 255, parts = e.y >> 8, k0 = (p.list_k ? e.x % nkb : e.x) * 128;
   const int len = length_of(p, b), pre = p.prefix ? p.prefix[b] : 0, shift = len - p.tq;
   const int key = k0 + (PAIR ? wid >> 1 : wid) * 32 + (lane & 31);
   const int mine = p.doc_q ? (key < len ? p.doc_k[(long)b * p.tk + key] : -1) : 0;
@@ -314,16 +316,16 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     t1 = __builtin_amdgcn_readfirstlane(range[1]);
   }
   const int nt = max(0, t1 - t0), steps = nt * p.grp;
-  // whether some row of the sweep sees no key (asked for each tile, the answer would be waited for in each)
-  if (threadIdx.x == 0) blind_rows = 0;
+  // the first tile with a row that sees no key (asked for each tile, the answer would be waited for in each)
+  if (threadIdx.x == 0) blind_rows = 0x7fffffff;
   __syncthreads();
   for (int i = threadIdx.x; i < steps; i += NT) {
     const int2* fl = bk.rows32 + ((long)b * p.heads + kh * p.grp + i / nt) * bk.n32 + (t0 + i % nt) * 2;
-    if (fl[0].x | fl[1].x) blind_rows = 1;
+    if (fl[0].x | fl[1].x) atomicMin(&blind_rows, t0 + i % nt);
   }
   __syncthreads();
-  const bool blind = __builtin_amdgcn_readfirstlane(blind_rows);
-  const int each = (steps + bk.nk - 1) / bk.nk, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
+  const int blind = __builtin_amdgcn_readfirstlane(blind_rows);
+  const int each = (steps + parts - 1) / parts, i0 = min(steps, part * each), i1 = min(steps, i0 + each);
 
   D qs, ds;
   qs.init(p.ldq, p.d);
@@ -334,7 +336,7 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h, at = head * p.tq + r0;
     const T *qa = (const T*)p.q + trow * p.ldq + h * p.d, *da = (const T*)p.dout + trow * p.lddo + h * p.d;
     const int2* fl = bk.rows32 + head * bk.n32 + r0 / 32;
-    if (blind && (fl[0].x | fl[1].x)) {   // a row that sees no key: it may hold anything
+    if (t_next >= blind && (fl[0].x | fl[1].x)) {   // a row that sees no key: it may hold anything
       auto keep = [&](int r) __attribute__((always_inline)) { return bk.nlse[at + min(r, last)] != -INFINITY; };
       qs.load_some(qa, tiles[buf], last, keep);
       ds.load_some(da, tiles[buf] + TILE, last, keep);
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   if (key >= p.tk) return;
   const long krow = (long)b * p.tk + key;
   auto leave = [&](const f32x16 (&acc)[DP / 32], float k, int which, T* out) __attribute__((always_inline)) {   // which: 0 dK, 1 dV
-    float* pk = bk.nk > 1 ? bk.part + ((((long)part * 2 + which) * p.nb * p.tk + krow) * p.kvh + kh) * DP : nullptr;
+    float* pk = parts > 1 ? bk.part + ((((long)part * 2 + which) * p.nb * p.tk + krow) * p.kvh + kh) * DP : nullptr;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -520,6 +522,8 @@ struct Parts {
   long rows, stride;   // stride: from a part to the next
   void* out;
   int ld;
+  const int* parts;    // of each block of 128 rows of a sequence of t, or NULL: n everywhere
+  int t;
 };
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void add_parts_kernel(Parts a, Parts b, Parts c, int d) {
@@ -527,17 +531,21 @@ __global__ __launch_bounds__(256) void add_parts_kernel(Parts a, Parts b, Parts 
   const long i = (long)blockIdx.x * 256 + threadIdx.x, rh = i / (DP / 4);
   const int col = (int)(i % (DP / 4)) * 4;
   if (rh >= p.rows * p.per || col >= d) return;
+  const long row = rh / p.per;
+  const int n = p.parts ? p.parts[row / p.t * ((p.t + 127) / 128) + row % p.t / 128] : p.n;
+  if (n == 1) return;   // it is there
   const float* src = p.part + rh * DP + col;
   f32x4 s = {};
 #pragma unroll 4
-  for (int k = 0; k < p.n; ++k) s += *reinterpret_cast<const f32x4*>(src + k * p.stride);
-  put4((T*)p.out + rh / p.per * p.ld + rh % p.per * d + col, s);
+  for (int k = 0; k < n; ++k) s += *reinterpret_cast<const f32x4*>(src + k * p.stride);
+  put4((T*)p.out + row * p.ld + rh % p.per * d + col, s);
 }
 
 // Splits of dkv_kernel's sweep, where its blocks do not fill the card: no shorter than 8 tiles each.  us of the whole backward with
 // 1, 2, 3, 4, 8: 6912 x 5 heads of 64 (270 blocks) 390, 354, 325, 328, 344; 4608 x 5 (180) 200, 166, 184, 166, 176; 8 x 1728 x 10 (1120)
 // 294, 312, 345, 365, 508; causal, heads of 128: 4096 x 32/8 (256) 691, 520, 553, 542, 617; 2 x 2500 x 16/4 (160) 401, 269, 254, 257, 282.
 int dkv_splits(const dc_attn_desc* d) {
+  if (const Lists l = lists_of(d); l.on) return l.most_k;
   const long blocks = (long)d->nb * d->kv_heads * ((d->tk + 127L) / 128);
   const long steps = (long)(d->heads / d->kv_heads) * ((d->tq + 63L) / 64);
   return (int)max(1L, min(min((d->d > 64 ? 600 : 900) / blocks, steps / 8), 8L));
@@ -560,16 +568,17 @@ long bwd_ws_bytes(const dc_attn_desc* d) {
 
 template <typename T, int DP, bool SHAPED>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
-  const dim3 grid((unsigned)((long)c.nb * c.heads * ((c.tq + 127) / 128) * bk.nq));
+  const long nqb = (long)c.nb * ((c.tq + 127) / 128), nkb = (long)c.nb * ((c.tk + 127) / 128);
+  const dim3 grid((unsigned)(c.heads * (c.list_q ? c.entries_q : nqb * bk.nq)));
   // two sweeps up to 16 tiles of keys (4 x 108 x 20 heads, forward and gradients: 31 us for 35)
   if (bk.nq == 1 && c.tk <= 1024) hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED, true>), grid, dim3(256), 0, st, c, bk);
   else hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED, false>), grid, dim3(256), 0, st, c, bk);
-  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)((long)c.nb * c.kvh * ((c.tk + 127) / 128) * bk.nk)),
+  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)(c.kvh * (c.list_k ? c.entries_k : nkb * bk.nk))),
                      dim3(DP == 64 ? 256 : 512), 0, st, c, bk);
   const long nk = (long)c.nb * c.tk * c.kvh, nq = (long)c.nb * c.tq * c.heads;
   const Parts none{};
-  const Parts dk{bk.part, bk.nk, c.kvh, (long)c.nb * c.tk, 2 * nk * DP, c.dk, c.lddk}, dv{bk.part + nk * DP, bk.nk, c.kvh,
-                 (long)c.nb * c.tk, 2 * nk * DP, c.dv, c.lddv}, dq{bk.part_q, bk.nq, c.heads, (long)c.nb * c.tq, nq * DP, c.dq, c.lddq};
+  const Parts dk{bk.part, bk.nk, c.kvh, (long)c.nb * c.tk, 2 * nk * DP, c.dk, c.lddk, c.parts_k, c.tk}, dv{bk.part + nk * DP, bk.nk, c.kvh,
+                 (long)c.nb * c.tk, 2 * nk * DP, c.dv, c.lddv, c.parts_k, c.tk}, dq{bk.part_q, bk.nq, c.heads, (long)c.nb * c.tq, nq * DP, c.dq, c.lddq, c.parts_q, c.tq};
   const long most = max(bk.nk > 1 ? nk : 0, bk.nq > 1 ? nq : 0);
   if (most)
     hipLaunchKernelGGL((add_parts_kernel<T, DP>), dim3((unsigned)((most * (DP / 4) + 255) / 256), bk.nk > 1 ? 3 : 1), dim3(256), 0,

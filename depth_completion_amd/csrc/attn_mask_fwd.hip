@@ -31,13 +31,16 @@ __global__ __launch_bounds__(256) void summary_kernel(const int* doc_k, int tk, 
   if (lane == 0) *to = make_int4(lo, hi, none, 0);
 }
 
-// The same tiles by one block, for calls of few blocks, and the orders in which these are taken: blocks of 128 rows by the number of the
-// other side's tiles that their documents meet (a prefix left out), the most first.  order_k: NULL in the forward.  Packed documents
-// in unlucky order cost what the longest CU has: 9001 x 5 heads with the longest document last 157 us unsorted, 91 with it first.
+// The same tiles by one block, for calls of few blocks, and the lists of what these take: blocks of 128 rows in parts of as many tiles
+// as give the card its fill, the longest first.  A block's tiles are those of the other side that its documents meet (a prefix left
+// out).  list_k is NULL in the forward.  What it costs (9 us for 9001 rows) buys the balance: us unsorted with even parts and so, forward
+// and with the gradients, 5 heads of 64, 9001 rows: the longest document first 91 88, 324 323, last 156 114, 518 377; 4 x 4700 111 104,
+// 397 365; 10 heads, 4700 67 59, 236 207.
 constexpr int kSorted = 1024;   // tiles, and blocks of either side
-__global__ __launch_bounds__(1024) void plan_kernel(Call p, int nk, int nq, int4* out, int* order_q, int* order_k) {
+__global__ __launch_bounds__(1024) void plan_kernel(Call p, int nk, int nq, Lists l, int4* out, int2* list_q, int* parts_q, int2* list_k,
+                                                    int* parts_k) {
   __shared__ int4 sum[kSorted];
-  __shared__ int cost[kSorted];
+  __shared__ int cost[kSorted], sums[16];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // a tile to a wave, eight on their way
   auto side = [&](const int* doc, int rows, int nt, int4* to, int4* copy) __attribute__((always_inline)) {
@@ -72,8 +75,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call p, int nk, int nq, int4
   if (nq) side(p.doc_q, p.tq, nq, out + p.nb * nk, sum + p.nb * nk);
   const int4* sum_q = nq ? sum + p.nb * nk : sum;
   const int nt_q = (p.tq + 63) / 64;
-  auto sort = [&](bool keys, int* order) __attribute__((always_inline)) {   // an item to a wave
+  auto fill = [&](bool keys, int2* list, int* parts) __attribute__((always_inline)) {   // a block of rows to a wave
     const int nt = keys ? nk : nt_q, blocks = (nt + 1) / 2, items = p.nb * blocks;
+    const int entries = keys ? l.entries_k : l.entries_q, most_parts = keys ? l.most_k : l.most_q;
     __syncthreads();
     int b = 0, w = wid;
     for (int i = wid; i < items; i += 16, w += 16) {
@@ -93,18 +97,48 @@ __global__ __launch_bounds__(1024) void plan_kernel(Call p, int nk, int nq, int4
       if (lane == 0) cost[i] = c;
     }
     __syncthreads();
+    // the least of 16 lengths of a part, from an even share to the longest block, whose parts fit the list: a length to a wave
+    int total = 0, longest = 0;
+    for (int i = lane; i < items; i += 64) {
+      total += cost[i];
+      longest = max(longest, cost[i]);
+    }
+    total = lanes_reduce(total, [](int a, int b) __attribute__((always_inline)) { return a + b; });
+    longest = wave_max_i(longest);
+    const float share = fmaxf((float)total / entries, keys ? fmaxf(1.0f, 8.0f / p.grp) : 8.0f);
+    auto length = [&](int k) __attribute__((always_inline)) { return share + fmaxf(longest - share, 0.0f) * (k / 15.0f); };
+    // (of the longest length the list holds all: no more than `even` parts each; its blocks are one part though the quotient is rounded)
+    const int even = entries / items;
+    auto parts_of = [&](int c, float len) __attribute__((always_inline)) {
+      return max(1, min(most_parts, max((int)ceilf(c * __builtin_amdgcn_rcpf(len) - 1e-3f), min(even, (c + 7) / 8))));
+    };
+    int sum_parts = 0;
+    for (int i = lane; i < items; i += 64) sum_parts += parts_of(cost[i], length(wid));
+    sum_parts = lanes_reduce(sum_parts, [](int a, int b) __attribute__((always_inline)) { return a + b; });
+    if (lane == 0) sums[wid] = sum_parts;
+    __syncthreads();
+    const int k = __ffsll(__ballot(sums[lane & 15] <= entries || lane >= 15)) - 1, filled = sums[k];
+    const float len = length(k);
+    for (int i = threadIdx.x; i < items; i += 1024) {
+      const int n = parts_of(cost[i], len);
+      parts[i] = n;
+      cost[i] = (cost[i] + n - 1) / n * 16 + n;
+    }
+    for (int i = filled + threadIdx.x; i < entries; i += 1024) list[i] = make_int2(-1, 0);
+    __syncthreads();
     for (int i = wid; i < items; i += 16) {
-      const int c = cost[i];
-      int rank = 0;
-      for (int j = 0; j < items; j += 64) {
-        const int o = cost[min(j + lane, items - 1)];
-        rank += __popcll(__ballot(j + lane < items && (o > c || (o == c && j + lane < i))));
+      const int c = cost[i], n = c & 15;
+      int at = 0;   // parts of the blocks before this one
+      for (int j = lane; j < items; j += 64) {
+        const int o = cost[j];
+        if (o >> 4 > c >> 4 || (o >> 4 == c >> 4 && j < i)) at += o & 15;
       }
-      if (lane == 0) order[rank] = i;
+      at = lanes_reduce(at, [](int a, int b) __attribute__((always_inline)) { return a + b; });
+      if (lane < n && at + lane < entries) list[at + lane] = make_int2(i, lane | n << 8);
     }
   };
-  sort(false, order_q);
-  if (order_k) sort(true, order_k);
+  fill(false, list_q, parts_q);
+  if (list_k) fill(true, list_k, parts_k);
 }
 
 // Running softmax of one lane's query over tiles of scores.  m is the reference of the weights 2^(x - m); it follows the row's
@@ -223,15 +257,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   QueryBlock q;
   q.init(p, sp.n);
+  if (q.idle) return;
   const T* qrow = (const T*)p.q + ((long)q.b * p.tq + q.qi) * p.ldq + q.h * p.d;
   v8 qf[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) qf[s] = load8_or_0(qrow + 16 * s + 8 * hh, q.live && 16 * s + 8 * hh < p.d);
   int t0, t1;
-  bool holes;
+  int holes;
   q.tiles(p, q.live, range, t0, t1, holes);
-  if (sp.n > 1) {
-    const int each = (t1 - t0 + sp.n - 1) / sp.n;
+  if (q.parts > 1) {
+    const int each = (t1 - t0 + q.parts - 1) / q.parts;
     t0 = min(t1, t0 + q.part * each);
     t1 = min(t1, t0 + each);
   }
@@ -338,7 +373,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   const float l = pair_sum(st.l);
   if (!q.live) return;
   const long row = ((long)q.b * p.heads + q.h) * p.tq + q.qi;
-  if (sp.n > 1) put_part<T, DP>(sp, st, l, row, q.part, hh);
+  if (q.parts > 1) put_part<T, DP>(sp, st, l, row, q.part, hh);
   else put_row<T, DP>(p, st, l, row, (long)q.b * p.tq + q.qi, q.h, hh);
 }
 
@@ -483,19 +518,22 @@ __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) 
   const long row = ((long)blockIdx.x * 256 + threadIdx.x) / (LANES * G);
   const int lane = threadIdx.x % LANES, col = lane * 4, grp = G == 1 ? 0 : threadIdx.x / LANES;
   if (row >= rows) return;
+  const long bh = row / p.tq, q = row % p.tq, b = bh / p.heads;
+  const int n = p.parts_q ? p.parts_q[b * ((p.tq + 127) / 128) + q / 128] : sp.n;
+  if (p.parts_q && n == 1) return;   // it is there
   const float2* ml = reinterpret_cast<const float2*>(sp.ml) + row * sp.n;
   float top = -INFINITY;
   if constexpr (G == 1) {
 #pragma unroll 4
-    for (int i = 0; i < sp.n; ++i) top = fmaxf(top, ml[i].x);
+    for (int i = 0; i < n; ++i) top = fmaxf(top, ml[i].x);
   } else {
-    top = wave_max((int)(threadIdx.x & 63) < sp.n ? ml[threadIdx.x & 63].x : -INFINITY);   // (at most 64 splits)
+    top = wave_max((int)(threadIdx.x & 63) < n ? ml[threadIdx.x & 63].x : -INFINITY);   // (at most 64 splits)
   }
   float l = 0.0f;
   f32x4 o = {};
   const float* src = sp.o + row * sp.n * DP + col;
 #pragma unroll 4
-  for (int i = grp; i < sp.n; i += G) {
+  for (int i = grp; i < n; i += G) {
     const float2 x = ml[i];
     // a split without weights left no O; one that saw NaN scores alone has m = -inf and l = NaN, which has to reach the result
     const float k = x.x == -INFINITY ? 0.0f : exp2_raw(x.x - top);
@@ -514,7 +552,6 @@ __global__ __launch_bounds__(256) void join_kernel(Call p, Split sp, long rows) 
       l += red[i][lane][4];
     }
   }
-  const long bh = row / p.tq, q = row % p.tq, b = bh / p.heads;
   const int h = (int)(bh % p.heads);
   const bool none = l == 0.0f;
   const float inv = 1.0f / l;
@@ -560,7 +597,7 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
     const long blocks = (long)c.nb * c.kvh * ((c.tq * c.grp + 31) / 32) * s.n;
     hipLaunchKernelGGL((token_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   } else {
-    const long blocks = (long)c.nb * c.heads * ((c.tq + 127) / 128) * s.n;
+    const long blocks = c.heads * (c.list_q ? (long)c.entries_q : (long)c.nb * ((c.tq + 127) / 128) * s.n);
     hipLaunchKernelGGL((fwd_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   }
   const long rows = (long)c.nb * c.heads * c.tq, threads = rows * (DP / 4);
@@ -580,11 +617,12 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
 // Splits of the keys of blocks of 128 rows: only where the card is not full, to 4/3 of what it holds (a few long blocks more than it
 // has CUs for would double the time), each split 16 tiles of 64 or more.  Forward, us with 1, 2, 4, 8 splits: 6912 x 5 heads of 64
 // (270 blocks) 147, 108, 100, 106; 4608 x 5 (180) 86, 59, 50, 56; 1728 x 10 (140 blocks of 27 tiles) 33, 33, 31, 34; 8 x 1728 x 10
-// (1120) 94, 106, 125, 194: the 32-bit parts cost their writing and reading.  With documents many of the blocks are short, and what the
-// card holds is enough: 9001 x 5 in five documents (355) 113, 91, 97 (3), 98 (4).
+// (1120) 94, 106, 125, 194: the 32-bit parts cost their writing and reading.  With documents (where no list
+// is made) many of the blocks are short, and what the card holds is enough.
 int tile_splits(const dc_attn_desc* d) {
   const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
   const long slots = 256 * (d->d > 64 ? 2 : 3);   // blocks that the card holds at once
+  if (const Lists l = lists_of(d); l.on) return l.most_q;
   if (3 * blocks >= 2 * slots) return 1;
   const long n = d->doc_q ? slots / blocks : (4 * slots / 3 + blocks - 1) / blocks;
   return (int)min(min(n, max(tiles / 16, 1L)), (long)kMaxSplit);
@@ -593,20 +631,32 @@ int tile_splits(const dc_attn_desc* d) {
 // Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.  us with and
 // without, 10 heads of 64, forward and gradients: 8 x 256 in 2 documents 47 38, 4 x 512 in 1 76 70, in 4 47 51, 4 x 1024 in 2 112 131.
 bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
-// Blocks are sorted where they are few (place_of) and one block can look at all tiles.
-bool sorted(const dc_attn_desc* d) {
-  const long nk = (d->tk + 63L) / 64, nq = (d->tq + 63L) / 64;
-  return summarised(d) && !few_rows(d->tq) && d->nb * (nk + nq) <= kSorted && (long)d->nb * d->heads * ((nq + 1) / 2) <= kSpread;
+// Lists where blocks are few (place_of) and one block can look at all tiles.  Entries: as many as the card holds (4/3 of it: 4 to 10 %
+// slower), or a block of rows each; a block has twice its even share of parts at most, as its documents may be the longest.
+Lists lists_of(const dc_attn_desc* d) {
+  const long nk = (d->tk + 63L) / 64, nq = (d->tq + 63L) / 64, bq = d->nb * ((nq + 1) / 2), bk = d->nb * ((nk + 1) / 2);
+  Lists l{};
+  l.on = summarised(d) && !few_rows(d->tq) && d->nb * (nk + nq) <= kSorted && bq * d->heads <= kSpread;
+  if (!l.on) return l;
+  l.items_q = (int)bq;
+  l.items_k = (int)bk;
+  const long slots = 256 * (d->d > 64 ? 2 : 3) / d->heads, slots_k = (d->d > 64 ? 600 : 900) / d->kv_heads;
+  l.most_q = (int)max(1L, min(min(8L, 2 * slots / bq), nk / 16));
+  l.most_k = (int)max(1L, min(min(8L, 2 * slots_k / bk), nq * (d->heads / d->kv_heads) / 16));
+  l.entries_q = (int)(l.most_q > 1 ? max(bq, slots) : bq);
+  l.entries_k = (int)(l.most_k > 1 ? max(bk, slots_k) : bk);
+  return l;
 }
 // the queries' tiles are the keys' where the documents are the same rows; the forward asks for them only to sort
 bool query_tiles(const dc_attn_desc* d, bool backward) {
-  return (backward || sorted(d)) && !(d->doc_q == d->doc_k && d->tq == d->tk);
+  return (backward || lists_of(d).on) && !(d->doc_q == d->doc_k && d->tq == d->tk);
 }
 
 long long summary_bytes(const dc_attn_desc* d, bool backward) {
   if (!summarised(d)) return 0;
   const long long sums = 16LL * d->nb * ((d->tk + 63L) / 64 + (query_tiles(d, backward) ? (d->tq + 63L) / 64 : 0));
-  return sums + (sorted(d) ? (4LL * d->nb * ((d->tk + 127L) / 128 + (d->tq + 127L) / 128) + 15) / 16 * 16 : 0);
+  const Lists l = lists_of(d);
+  return sums + (l.on ? (8LL * (l.entries_q + l.entries_k) + 4LL * (l.items_q + l.items_k) + 15) / 16 * 16 : 0);
 }
 
 void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st) {
@@ -615,11 +665,16 @@ void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, h
   int4* k = reinterpret_cast<int4*>(ws);
   c.sum_k = k;
   c.sum_q = nq ? k + (long)d->nb * nk : k;
-  if (sorted(d)) {
-    int* order = reinterpret_cast<int*>(k + (long)d->nb * (nk + nq));
-    c.order_q = order;
-    c.order_k = backward ? order + (long)d->nb * ((d->tq + 127) / 128) : nullptr;
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, c, nk, nq, k, order, const_cast<int*>(c.order_k));
+  if (const Lists l = lists_of(d); l.on) {
+    int2 *lq = reinterpret_cast<int2*>(k + (long)d->nb * (nk + nq)), *lk = backward ? lq + l.entries_q : nullptr;
+    int *pq = reinterpret_cast<int*>(lq + l.entries_q + l.entries_k), *pk = pq + l.items_q;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, c, nk, nq, l, k, lq, pq, lk, pk);
+    c.list_q = lq;
+    c.list_k = lk;
+    c.parts_q = pq;
+    c.parts_k = pk;
+    c.entries_q = l.entries_q;
+    c.entries_k = l.entries_k;
     return;
   }
   hipLaunchKernelGGL(summary_kernel, dim3((unsigned)((d->nb * (nk + nq) + 3) / 4)), dim3(256), 0, st, d->doc_k, d->tk, nk, d->doc_q,

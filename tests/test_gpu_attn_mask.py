@@ -193,6 +193,66 @@ def test_documents(ctx, kind, t, d, causal, dtype):
     check(ctx, c, dtype, tensors=(q, k, v, do))
 
 
+def runs(lengths, t, start=0):
+    """int32 [t]: documents of these lengths from number `start` on, rows in none behind them."""
+    ids = torch.full((t,), -1, dtype=torch.int32)
+    at = 0
+    for n, length in enumerate(lengths):
+        ids[at:at + length] = n + start
+        at += length
+    return ids.to(dev)
+
+
+@TYPES
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,t", [
+    (3, 3, 64, [60, 431, 90, 1000], 1700), (4, 1, 128, [1100, 70, 500], 1700), (1, 1, 64, [5, 2300, 1, 130], 2500),
+    (2, 1, 64, [40] * 30, 1201)])
+def test_documents_in_parts(ctx, heads, kv_heads, d, lengths, t, causal, dtype):
+    """Few blocks whose documents differ in length, so that some of them are split and some are not."""
+    ids = runs(lengths, t)
+    check(ctx, shape(1, t, t, heads, kv_heads, d, doc_q=ids, doc_k=ids, causal=causal), dtype, seed=21)
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+def test_documents_of_filled_lengths(ctx, prefix):
+    """Queries and keys of their own documents and counts, filled keys, a causal mask and a prefix, over two sequences."""
+    iq = torch.cat([runs([200, 300, 150], 700, 1), runs([700], 700, 2)])
+    ik = torch.cat([runs([100, 600, 500], 1500), runs([33, 67, 1000], 1500)])
+    c = shape(2, 700, 1500, 4, 2, 64, doc_q=iq, doc_k=ik, causal=True,
+              kv_len=torch.tensor([1400, 640], dtype=torch.int32, device=dev))
+    if prefix:
+        c["prefix"] = torch.tensor([900, 0], dtype=torch.int32, device=dev)
+    check(ctx, c, torch.bfloat16, seed=22)
+
+
+def test_documents_that_change_between_replays(ctx):
+    """A captured call takes its documents from where they lie when it runs."""
+    from depth_completion_amd import ops
+    t = 1300
+    ids = runs([700, 90, 400], t)
+    c = shape(1, t, t, 4, 2, 64, doc_q=ids, doc_k=ids)
+    q, k, v, do = inputs(c, torch.bfloat16, 23)
+    bufs = [torch.empty_like(q), torch.empty(1, 4, t, device=dev), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
+
+    def step(o, lse, dq, dk, dv):
+        ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+        ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+
+    step(*bufs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*bufs)
+    for lengths in ([700, 90, 400], [30, 1200], [1300], [], [64] * 20):
+        ids.copy_(runs(lengths, t))
+        graph.replay()
+        got = [b.clone() for b in bufs]
+        want = [torch.empty_like(b) for b in bufs]
+        step(*want)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), lengths
+
+
 def test_documents_across(ctx):
     """Queries and keys of different counts; a query document without keys and a key document without queries."""
     iq = torch.tensor([0] * 40 + [3] * 30 + [1] * 31, dtype=torch.int32, device=dev)
