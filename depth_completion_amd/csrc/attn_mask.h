@@ -399,7 +399,7 @@ struct KeyRing {
 // Host side: what both directions share (attn_mask_fwd.hip).
 constexpr int kMaxSplit = 64;
 bool shape_ok(const dc_attn_desc* d);
-int tile_splits(const dc_attn_desc* d);
+int tile_splits(const dc_attn_desc* d, bool backward);
 struct Lists { bool on; int items_q, items_k, entries_q, entries_k, most_q, most_k; };   // most: parts of a block
 Lists lists_of(const dc_attn_desc* d);
 int make_call(const dc_attn_desc* d, Call& c, bool backward);

@@ -559,7 +559,7 @@ long part_bytes(const dc_attn_desc* d) {
   return n > 1 ? 8L * n * d->nb * d->tk * d->kv_heads * (d->d > 64 ? 128 : 64) : 0;
 }
 long part_q_bytes(const dc_attn_desc* d) {
-  const int n = tile_splits(d);
+  const int n = tile_splits(d, true);
   return n > 1 ? 4L * n * d->nb * d->tq * d->heads * (d->d > 64 ? 128 : 64) : 0;
 }
 long bwd_ws_bytes(const dc_attn_desc* d) {
@@ -616,7 +616,7 @@ extern "C" int dc_attn_mask_bwd(const dc_attn_desc* d, void* scratch, long long 
   bk.ndel = reinterpret_cast<float*>(ws + rows_bytes(d));
   bk.rows32 = reinterpret_cast<int2*>(ws + 2 * rows_bytes(d));
   bk.n32 = (d->tq + 127) / 128 * 4;
-  bk.nq = tile_splits(d);
+  bk.nq = tile_splits(d, true);
   bk.nk = dkv_splits(d);
   bk.part = reinterpret_cast<float*>(ws + 2 * rows_bytes(d) + rows32_bytes(d));
   bk.part_q = reinterpret_cast<float*>(ws + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d));

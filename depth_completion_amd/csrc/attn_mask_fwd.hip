@@ -581,7 +581,7 @@ Split split_of(const dc_attn_desc* d) {
     s.tiles = (int)((steps + n - 1) / n);
     s.n = (int)((steps + s.tiles - 1) / s.tiles);
   } else {
-    s.n = tile_splits(d);
+    s.n = tile_splits(d, false);
   }
   return s;
 }
@@ -615,17 +615,20 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
 }  // namespace
 
 // Splits of the keys of blocks of 128 rows: only where the card is not full, to 4/3 of what it holds (a few long blocks more than it
-// has CUs for would double the time), each split 16 tiles of 64 or more.  Forward, us with 1, 2, 4, 8 splits: 6912 x 5 heads of 64
+// has CUs for would double the time), each split 8 tiles of 64 or
+// more, 3 where blocks are very few, 16 in the backward (whose short rows are not split).  Forward, us with 1, 2, 4, 8 splits: 6912 x 5 heads of 64
 // (270 blocks) 147, 108, 100, 106; 4608 x 5 (180) 86, 59, 50, 56; 1728 x 10 (140 blocks of 27 tiles) 33, 33, 31, 34; 8 x 1728 x 10
-// (1120) 94, 106, 125, 194: the 32-bit parts cost their writing and reading.  With documents (where no list
-// is made) many of the blocks are short, and what the card holds is enough.
-int tile_splits(const dc_attn_desc* d) {
+// (1120) 94, 106, 125, 194: the 32-bit parts cost their writing and reading.  With splits of 16, 8, 5 and 3
+// tiles: 92 x 829 keys, 3 heads of 128 (3 blocks) 25, 25, 19, 15; 100 x 1000, 20 of 64 (20) 20, 18, 16, 15; 1000 x 8 of 128 (64) 30, 26,
+// 25, 26; 432 x 20 (80) 12, 12, 12, 15; 1000 x 16 (128) 21, 23, 25, 27; 1728 x 10 (140) 34, 28, 30, 34.  With documents (where no list is
+// made) many of the blocks are short, and what the card holds is enough.
+int tile_splits(const dc_attn_desc* d, bool backward) {
   const long blocks = (long)d->nb * d->heads * ((d->tq + 127L) / 128), tiles = (d->tk + 63L) / 64;
   const long slots = 256 * (d->d > 64 ? 2 : 3);   // blocks that the card holds at once
   if (const Lists l = lists_of(d); l.on) return l.most_q;
   if (3 * blocks >= 2 * slots) return 1;
   const long n = d->doc_q ? slots / blocks : (4 * slots / 3 + blocks - 1) / blocks;
-  return (int)min(min(n, max(tiles / 16, 1L)), (long)kMaxSplit);
+  return (int)min(min(n, max(tiles / (backward ? 16 : blocks > 64 ? 8 : 3), 1L)), (long)kMaxSplit);
 }
 
 // Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.  us with and
