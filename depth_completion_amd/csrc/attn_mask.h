@@ -34,8 +34,8 @@ struct Call {
   float* lse;
   int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int nb, tq, tk, heads, kvh, grp, d;
-  float scale, mul;       // score scale; what turns a score into the exponent of 2: scale log2 e, or 1 where the scores are shaped
-  float cap2, icap;       // softcap log2 e, 2 log2 e scale / softcap (0: none)
+  float scale, mul;       // score scale; what turns a score into the exponent of 2: scale log2 e, or 1 where the scores are capped
+  float cap2, icap, bend; // softcap log2 e, 2 log2 e scale / softcap (0: none); what makes slopes fit scores: 1 / scale, log2 e with a cap
   const float* slopes;
   int causal;
   const int *prefix, *kv_len, *doc_q, *doc_k;

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
-  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
@@ -134,9 +134,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
             s[r] = cap_score(p, s[r], &g);
             if constexpr (!FIRST) dp[r] *= g;
           }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= p.scale * kLog2e;
         }
         if (p.slopes) {
           const float dist = (float)(q.pos - t * 64 - 4 * hh);
@@ -147,7 +144,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float pw = exp2_raw(SHAPED ? s[r] + nl : fmaf(s[r], p.mul, nl));
+        const float pw = exp2_raw(fmaf(s[r], p.mul, nl));
         s[r] = (is_half<T> && !FIRST ? pw * f : pw) * dp[r];
       }
       if (masked) {
@@ -405,12 +402,9 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
             s[r] = cap_score(p, s[r], &g);
             dp[r] *= g;
           }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= p.scale * kLog2e;
         }
         if (p.slopes) {
-          const float slope = p.slopes[kh * p.grp + hg] * kLog2e, dist = (float)(pos0 - key);
+          const float slope = p.slopes[kh * p.grp + hg] * p.bend, dist = (float)(pos0 - key);
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = fmaf(-slope, fabsf(dist + (float)((r & 3) + 8 * (r >> 2))), s[r]);
         }
@@ -419,7 +413,7 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float up = is_half<T> ? kPShift : 0.0f;
-        s[r] = exp2_raw(fmaf(s[r], SHAPED ? 1.0f : p.mul, nl[r >> 2][r & 3] + up));
+        s[r] = exp2_raw(fmaf(s[r], p.mul, nl[r >> 2][r & 3] + up));
         dp[r] *= is_half<T> ? s[r] * fs : s[r];
       }
       if (mixed || from_last > t * 64 + shift + rows) {

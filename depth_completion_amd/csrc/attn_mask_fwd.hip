@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   ring.init(p, q, holes);
   Row<T, DP> st;
   st.init();
-  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
@@ -306,11 +306,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
         for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb2][r] = cap_score(p, s[kb2][r], nullptr);
-      } else {
-#pragma unroll
-        for (int kb2 = 0; kb2 < 2; ++kb2)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb2][r] *= p.scale * kLog2e;
       }
       if (p.slopes) {
         const float dist = (float)(q.pos - t * 64 - 4 * hh);
@@ -336,7 +331,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
             if (t * 64 + key + e >= q.lim || (id && id4[e] != q.mine)) s[kb2][4 * g + e] = -INFINITY;
         }
     }
-    st.weigh(s, SHAPED ? 1.0f : p.mul);
+    st.weigh(s, p.mul);
     auto add = [&](auto C) __attribute__((always_inline)) {
       constexpr int c = decltype(C)::value;
       v8 f[DP / 32];
@@ -405,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
   const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
   T* vt = reinterpret_cast<T*>(smem) + wid * SUB;
-  const float slope = SHAPED && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+  const float slope = SHAPED && p.slopes ? p.slopes[h] * p.bend : 0.0f;
   TrAt va[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
@@ -455,9 +450,6 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
       if (p.cap2 != 0.0f) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[0][e] = cap_score(p, s[0][e], nullptr);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][e] *= p.scale * kLog2e;
       }
       if (p.slopes) {
         const float dist = (float)(pos - u * 32 - 4 * hh);
@@ -473,7 +465,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
         if (u * 32 + key >= lim || other) s[0][e] = -INFINITY;
       }
     }
-    st.weigh(s, SHAPED ? 1.0f : p.mul);
+    st.weigh(s, p.mul);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const v8 pf = acc_frag<T>(s[0], c);
@@ -696,7 +688,7 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   if (!shape_ok(d) || !d->q || !d->k || !d->v || !d->o || !d->lse || d->type < 0 || d->type > 1) return DC_ERR_ARG;
   if (d->d <= 0 || d->d > 128 || d->d % 8 || !(d->scale > 0.0f) || !(d->softcap >= 0.0f)) return DC_ERR_ARG;
   if (!(d->scale <= 1e30f) || !(d->softcap <= 1e30f) || (d->softcap > 0.0f && !(d->scale / d->softcap <= 1e30f))) return DC_ERR_ARG;
-  if (d->prefix && !d->causal) return DC_ERR_ARG;
+  if ((d->prefix && !d->causal) || (d->slopes && !(d->scale >= 1e-30f))) return DC_ERR_ARG;
   if (!d->doc_q != !d->doc_k) return DC_ERR_ARG;
   const long long hq = (long long)d->heads * d->d, hk = (long long)d->kv_heads * d->d;
   if (d->ldq < hq || d->ldo < hq || d->ldk < hk || d->ldv < hk) return DC_ERR_ARG;
@@ -717,7 +709,8 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   c.lddo = d->lddo; c.lddq = d->lddq; c.lddk = d->lddk; c.lddv = d->lddv;
   c.nb = d->nb; c.tq = d->tq; c.tk = d->tk; c.heads = d->heads; c.kvh = d->kv_heads; c.grp = d->heads / d->kv_heads; c.d = d->d;
   c.scale = d->scale;
-  c.mul = d->softcap > 0.0f || d->slopes ? 1.0f : d->scale * kLog2e;
+  c.mul = d->softcap > 0.0f ? 1.0f : d->scale * kLog2e;
+  c.bend = d->softcap > 0.0f ? kLog2e : 1.0f / d->scale;
   if (d->softcap > 0.0f) {
     c.cap2 = d->softcap * kLog2e;
     c.icap = 2.0f * kLog2e * d->scale / d->softcap;

@@ -524,6 +524,8 @@ def _attn_mask(ctx: Ctx, back, q, k, v, o, lse, nb, tq, tk, heads, kv_heads, d, 
     if not 0.0 < scale <= 1e30 or not 0.0 <= softcap <= 1e30 or softcap and scale > 1e30 * softcap:
         raise ValueError(f"attn_mask: scale {scale}, softcap {softcap} "
                          "(scale above 0, softcap 0 for none, both and scale / softcap at most 1e30)")
+    if slopes is not None and scale < 1e-30:
+        raise ValueError(f"attn_mask: slopes beside a scale of {scale} (1e-30 or more)")
     if prefix is not None and not causal:
         raise ValueError("attn_mask: a prefix opens a causal mask; without causal every key is seen already")
     if (doc_q is None) != (doc_k is None):

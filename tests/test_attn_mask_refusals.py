@@ -122,3 +122,10 @@ def test_fields_that_do_not_hold():
         with pytest.raises(ValueError, match="attn"):
             ops._pack(_lib.PACK_ATTN, "attn_mask", *bad)
     assert ops._pack(_lib.PACK_ATTN, "attn_mask", *fields) == bytes(_lib.AttnDesc())
+
+
+def test_slopes_beside_no_scale():
+    with pytest.raises(ValueError, match="slopes"):
+        call(slopes=torch.zeros(4), scale=1e-31)
+    d = descriptor(slopes=4096, scale=1e-31)
+    assert _lib.load().dc_attn_mask_fwd(C.byref(d), 4096, 1 << 30, None) == ARG
