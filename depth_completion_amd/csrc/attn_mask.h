@@ -1,5 +1,5 @@
 // Shared device helpers of the masked attention kernels (attn_mask_fwd.hip, attn_mask_bwd.hip): fragment types of the two
-// storage types, the LDS tile with its swizzle, staging through registers, and the description of a call.
+// storage types, the LDS tile with its swizzle and the loads into it, which block takes what, and the description of a call.
 #pragma once
 #include "common.h"
 #include "../../include/dcamd.h"
