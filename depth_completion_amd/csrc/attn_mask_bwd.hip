@@ -16,7 +16,7 @@ namespace dcm {
 namespace {
 
 struct Back {
-  float *nlse, *ndel;   // [nb heads][tq]: -lse log2 e (-inf: the row sees no key), -rowsum(dO o)
+  float *nlse, *ndel;   // [nb heads][32 n32]: -lse log2 e (-inf: the row sees no key, or lies behind the last), -rowsum(dO o)
   int2* rows32;         // [nb heads][n32]: of 32 rows, whether one sees no key, and the largest |dO| (its bits)
   int n32;
   int nq, nk;           // splits of dq_kernel's sweep over the keys, of dkv_kernel's over the queries
@@ -210,9 +210,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     del = pair_sum(exact);
     tile_barrier();
   }
-  if (q.live && hh == 0 && q.part == 0) {
-    bk.nlse[row] = nl;
-    bk.ndel[row] = -del;
+  // (rows behind the last too: what dkv_kernel reads there has to weigh nothing, whatever its scores become)
+  if (hh == 0 && q.part == 0) {
+    const long at = ((long)q.b * p.heads + q.h) * 32 * bk.n32 + q.qi;
+    bk.nlse[at] = nl;
+    bk.ndel[at] = -del;
   }
   sweep(std::false_type{});
   if (!q.live) return;
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
   int hg_next = nt ? i0 / nt : 0, t_next = nt ? t0 + i0 % nt : 0;
   auto load = [&](int buf) __attribute__((always_inline)) {   // the next (query head, tile) of the sweep
     const int h = kh * p.grp + hg_next, r0 = t_next * 64, last = p.tq - 1 - r0;
-    const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h, at = head * p.tq + r0;
+    const long trow = (long)b * p.tq + r0, head = (long)b * p.heads + h, at = head * 32 * bk.n32 + r0;
     const T *qa = (const T*)p.q + trow * p.ldq + h * p.d, *da = (const T*)p.dout + trow * p.lddo + h * p.d;
     const int2* fl = bk.rows32 + head * bk.n32 + r0 / 32;
     if (t_next >= blind && (fl[0].x | fl[1].x)) {   // a row that sees no key: it may hold anything
@@ -342,8 +344,8 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
       ds.load(da, tiles[buf] + TILE, last);
     }
     if (wid == 0) {
-      dma_words(bk.nlse + at, cn[buf], last);
-      dma_words(bk.ndel + at, cd[buf], last);
+      dma_words(bk.nlse + at, cn[buf], 63);
+      dma_words(bk.ndel + at, cd[buf], 63);
       if (p.doc_q) dma_words(p.doc_q + trow, ids[buf], last);
     }
     if (++t_next == t1) { t_next = t0; ++hg_next; }
@@ -546,7 +548,7 @@ int dkv_splits(const dc_attn_desc* d) {
 }
 long pad16(long bytes) { return (bytes + 15) / 16 * 16; }
 
-long rows_bytes(const dc_attn_desc* d) { return pad16(4L * d->nb * d->heads * d->tq); }
+long rows_bytes(const dc_attn_desc* d) { return 4L * d->nb * d->heads * ((d->tq + 127L) / 128 * 128); }
 long rows32_bytes(const dc_attn_desc* d) { return pad16(8L * d->nb * d->heads * ((d->tq + 127L) / 128 * 4)); }
 long part_bytes(const dc_attn_desc* d) {
   const int n = dkv_splits(d);

@@ -471,7 +471,7 @@ typedef struct dc_attn_desc {
   float* lse;                   /* [nb][heads][tq] natural log; read by the backward */
   int ldq, ldk, ldv, ldo;
   float scale, softcap;         /* scale > 0; softcap 0: none */
-  const float* slopes;          /* [heads] or NULL; constants, no gradient; with a scale of 1e-30 or more */
+  const float* slopes;          /* [heads] of either sign, or NULL; constants, no gradient; with a scale of 1e-30 or more */
   int causal;
   const int* prefix;            /* [nb] or NULL; with causal only */
   const int* kv_len;            /* [nb] or NULL */

@@ -418,3 +418,12 @@ def test_two_graphs_and_a_stream(ctx):
         for bufs, ref in zip(outs, want):
             assert all(torch.equal(a, b) for a, b in zip(bufs, ref))
         assert torch.equal(o3, want[0][0])
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tq,tk,causal", [(130, 200, False), (130, 200, True), (70, 90, False), (5, 300, True), (513, 1100, True)])
+def test_bias_that_grows_with_distance(ctx, tq, tk, causal, d, dtype):
+    """Slopes of either sign, and row counts that end inside a tile: what lies behind the last row weighs nothing, however far."""
+    slopes = torch.tensor([-0.05, 0.05, -2.0, 0.5], device=dev)
+    check(ctx, shape(2, tq, tk, 4, 2, d, slopes=slopes, causal=causal), dtype, seed=31)
