@@ -35,6 +35,7 @@ struct Call {
   int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int nb, tq, tk, heads, kvh, grp, d;
   float scale, mul;       // score scale; what turns a score into the exponent of 2: scale log2 e, or 1 where the scores are capped
+  float wide;             // 1 / softcap of a cap above kWideCap, else 0
   float cap2, icap, bend; // softcap log2 e, 2 log2 e scale / softcap (0: none); what makes slopes fit scores: 1 / scale, log2 e with a cap
   const float* slopes;
   int causal;
@@ -46,9 +47,20 @@ struct Call {
   int entries_q, entries_k;
 };
 
-// Scores of a call with a cap, in units of log2: cap2 tanh(scale s / cap), with tanh(x) = 1 - 2 r, r = 1 / (1 + e^2x): absolute error
-// of tanh below 2e-7, so the exponent is off by under 1e-5 at cap = 50.  slope: r - r^2, a quarter of 1 - tanh^2.
+// What the scores pass: nothing but their scale; a cap or a bias; a cap above kWideCap (and a bias).
+enum { PLAIN, SHAPED, WIDE };
+// Scores of a call with a cap, in units of log2: cap2 tanh(scale s / cap), with tanh(x) = 1 - 2 r, r = 1 / (1 + e^2x).  slope: r - r^2,
+// a quarter of 1 - tanh^2.  The difference leaves tanh an absolute error below 2e-7, and the cap multiplies it: a score is off by
+// under 1.3e-5 at a cap of 64, by 0.2 at 1e6.  Wider caps, whose scores lie far below them, take the function whose error is relative
+// (kernels of their own: as a branch beside the other form it takes dQ's at 64 columns past their 168 registers).
+constexpr float kWideCap = 64.0f;
+template <int FORM>
 __device__ __forceinline__ float cap_score(const Call& p, float s, float* slope) {
+  if constexpr (FORM == WIDE) {
+    const float t = tanhf(s * p.scale * p.wide);
+    if (slope) *slope = 0.25f * fmaf(-t, t, 1.0f);
+    return p.cap2 * t;
+  }
   const float r = __builtin_amdgcn_rcpf(1.0f + exp2_raw(s * p.icap));
   if (slope) *slope = fmaf(-r, r, r);
   return fmaf(-2.0f * p.cap2, r, p.cap2);

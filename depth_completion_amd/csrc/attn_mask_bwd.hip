@@ -46,7 +46,7 @@ __device__ __forceinline__ float near_sixteenth(float x) {
 // EXACT: rowsum(dO o) from the rounded o is off by a rounding of o, the same for all keys of the row.  Rows of few keys, whose gradients
 // are small differences, take it from a sweep of its own over P dP: of 750 gradients of random calls of 8 to 6000 keys the furthest
 // (12 keys) was off by 0.46 % of its norm without and 0.36 % with (2009 keys), 264 and 49 of them by more than one rounding and a half.
-template <typename T, int DP, bool SHAPED, bool EXACT>
+template <typename T, int DP, int FORM, bool EXACT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
-  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
+  const float slope = FORM != PLAIN && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
@@ -126,12 +126,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
       if constexpr (!FIRST)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] -= del;
-      if constexpr (SHAPED) {
+      if constexpr (FORM != PLAIN) {
         if (p.cap2 != 0.0f) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float g;
-            s[r] = cap_score(p, s[r], &g);
+            s[r] = cap_score<FORM>(p, s[r], &g);
             if constexpr (!FIRST) dp[r] *= g;
           }
         }
@@ -255,7 +255,7 @@ constexpr float kPShift = 14.0f;   // fp16: P in dV is 2^14 times as large
 // (2 KB each way), and a wave carries one sum, not two, which is what lets two waves share a SIMD (one wave with both took 416
 // registers and 24 % of the matrix units' time: 4097 x 32/8 heads causal 511 us for 398; at 64 columns, where both fit, pairs lose:
 // 8 x 4096 x 16 heads with dQ 2020 us for 2824).
-template <typename T, int DP, bool SHAPED>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
   constexpr bool PAIR = DP == 128;
@@ -396,12 +396,12 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
         s = mfma(*reinterpret_cast<const v8*>(qt + at * DP + qoff[c]), kf[c], s);
         dp = mfma(*reinterpret_cast<const v8*>(dt + at * DP + qoff[c]), vf[c], dp);
       }
-      if constexpr (SHAPED) {
+      if constexpr (FORM != PLAIN) {
         if (p.cap2 != 0.0f) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float g;
-            s[r] = cap_score(p, s[r], &g);
+            s[r] = cap_score<FORM>(p, s[r], &g);
             dp[r] *= g;
           }
         }
@@ -562,14 +562,14 @@ long bwd_ws_bytes(const dc_attn_desc* d) {
   return summary_bytes(d, true) + 2 * rows_bytes(d) + rows32_bytes(d) + part_bytes(d) + part_q_bytes(d);
 }
 
-template <typename T, int DP, bool SHAPED>
+template <typename T, int DP, int FORM>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
   const long nqb = (long)c.nb * ((c.tq + 127) / 128), nkb = (long)c.nb * ((c.tk + 127) / 128);
   const dim3 grid((unsigned)(c.heads * (c.list_q ? c.entries_q : nqb * bk.nq)));
   // two sweeps up to 16 tiles of keys (4 x 108 x 20 heads, forward and gradients: 31 us for 35)
-  if (bk.nq == 1 && c.tk <= 1024) hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED, true>), grid, dim3(256), 0, st, c, bk);
-  else hipLaunchKernelGGL((dq_kernel<T, DP, SHAPED, false>), grid, dim3(256), 0, st, c, bk);
-  hipLaunchKernelGGL((dkv_kernel<T, DP, SHAPED>), dim3((unsigned)(c.kvh * (c.list_k ? c.entries_k : nkb * bk.nk))),
+  if (bk.nq == 1 && c.tk <= 1024) hipLaunchKernelGGL((dq_kernel<T, DP, FORM, true>), grid, dim3(256), 0, st, c, bk);
+  else hipLaunchKernelGGL((dq_kernel<T, DP, FORM, false>), grid, dim3(256), 0, st, c, bk);
+  hipLaunchKernelGGL((dkv_kernel<T, DP, FORM>), dim3((unsigned)(c.kvh * (c.list_k ? c.entries_k : nkb * bk.nk))),
                      dim3(DP == 64 ? 256 : 512), 0, st, c, bk);
   const long nk = (long)c.nb * c.tk * c.kvh, nq = (long)c.nb * c.tq * c.heads;
   const Parts none{};
@@ -582,7 +582,9 @@ void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
 }
 template <typename T, int DP>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
-  c.cap2 != 0.0f || c.slopes ? launch_bwd<T, DP, true>(c, bk, st) : launch_bwd<T, DP, false>(c, bk, st);
+  if (c.wide != 0.0f) launch_bwd<T, DP, WIDE>(c, bk, st);
+  else if (c.cap2 != 0.0f || c.slopes) launch_bwd<T, DP, SHAPED>(c, bk, st);
+  else launch_bwd<T, DP, PLAIN>(c, bk, st);
 }
 
 }  // namespace

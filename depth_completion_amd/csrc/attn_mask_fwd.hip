@@ -247,7 +247,7 @@ __device__ __forceinline__ void put_part(const Split& sp, const Row<T, DP>& s, f
 // transposed reads carry no alias information, so the compiler waits for every load into LDS before them: sent any earlier, a tile
 // would be waited for at once.  128 columns hold two tiles alone (three would leave one block to a CU): there tile i + 1 is sent when
 // the step begins, and the reads are waited for in blocks of their own (tr_frags).
-template <typename T, int DP, bool SHAPED>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Split sp) {
   typedef typename Vec<T>::v8 v8;
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
   ring.init(p, q, holes);
   Row<T, DP> st;
   st.init();
-  const float slope = SHAPED && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
+  const float slope = FORM != PLAIN && p.slopes ? p.slopes[q.h] * p.bend : 0.0f;
   int koff[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) koff[s] = tile_at<DP>(lane & 31, 2 * s + hh);
@@ -300,12 +300,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) s[kb2] = mfma(*reinterpret_cast<const v8*>(kt + 32 * kb2 * DP + koff[c]), qf[c], s[kb2]);
     }
-    if constexpr (SHAPED) {
+    if constexpr (FORM != PLAIN) {
       if (p.cap2 != 0.0f) {
 #pragma unroll
         for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb2][r] = cap_score(p, s[kb2][r], nullptr);
+          for (int r = 0; r < 16; ++r) s[kb2][r] = cap_score<FORM>(p, s[kb2][r], nullptr);
       }
       if (p.slopes) {
         const float dist = (float)(q.pos - t * 64 - 4 * hh);
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void fwd_kernel(Call p, Spli
 }
 
 // One block: up to 32 of the rows (query, head of the group) of one key head, `sp.tiles` steps of 4 x 32 keys.
-template <typename T, int DP, bool SHAPED>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   typedef typename Vec<T>::v8 v8;
   constexpr int SUB = 32 * DP, NV = SUB / 8 / 64, CH = DP / 8, RED = (2 + DP / 2) * 64;
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
   const T* vb = (const T*)p.v + (long)b * p.tk * p.ldv + kh * p.d;
   const int* kid = p.doc_q ? p.doc_k + (long)b * p.tk : nullptr;
   T* vt = reinterpret_cast<T*>(smem) + wid * SUB;
-  const float slope = SHAPED && p.slopes ? p.slopes[h] * p.bend : 0.0f;
+  const float slope = FORM != PLAIN && p.slopes ? p.slopes[h] * p.bend : 0.0f;
   TrAt va[DP / 32];
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n) va[n] = tr_at<DP>(32 * n, lane);
@@ -446,10 +446,10 @@ __global__ __launch_bounds__(256, 2) void token_kernel(Call p, Split sp) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) s[0] = mfma(kf[c], qf[c], s[0]);   // qf is zero where the columns end
     if (u + 4 < u1) fetch(u + 4);
-    if constexpr (SHAPED) {
+    if constexpr (FORM != PLAIN) {
       if (p.cap2 != 0.0f) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][e] = cap_score(p, s[0][e], nullptr);
+        for (int e = 0; e < 16; ++e) s[0][e] = cap_score<FORM>(p, s[0][e], nullptr);
       }
       if (p.slopes) {
         const float dist = (float)(pos - u * 32 - 4 * hh);
@@ -583,14 +583,14 @@ long part_floats(const dc_attn_desc* d, const Split& s) {
   return (long)d->nb * d->heads * d->tq * s.n * ((d->d > 64 ? 128 : 64) + 2);
 }
 
-template <typename T, int DP, bool SHAPED>
+template <typename T, int DP, int FORM>
 void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
   if (few_rows(d->tq)) {
     const long blocks = (long)c.nb * c.kvh * ((c.tq * c.grp + 31) / 32) * s.n;
-    hipLaunchKernelGGL((token_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
+    hipLaunchKernelGGL((token_kernel<T, DP, FORM>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   } else {
     const long blocks = c.heads * (c.list_q ? (long)c.entries_q : (long)c.nb * ((c.tq + 127) / 128) * s.n);
-    hipLaunchKernelGGL((fwd_kernel<T, DP, SHAPED>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
+    hipLaunchKernelGGL((fwd_kernel<T, DP, FORM>), dim3((unsigned)blocks), dim3(256), 0, st, c, s);
   }
   const long rows = (long)c.nb * c.heads * c.tq, threads = rows * (DP / 4);
   if (s.n <= 1) return;
@@ -601,7 +601,9 @@ void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
 }
 template <typename T, int DP>
 void launch_fwd(const Call& c, const dc_attn_desc* d, Split s, hipStream_t st) {
-  c.cap2 != 0.0f || c.slopes ? launch_fwd<T, DP, true>(c, d, s, st) : launch_fwd<T, DP, false>(c, d, s, st);
+  if (c.wide != 0.0f) launch_fwd<T, DP, WIDE>(c, d, s, st);
+  else if (c.cap2 != 0.0f || c.slopes) launch_fwd<T, DP, SHAPED>(c, d, s, st);
+  else launch_fwd<T, DP, PLAIN>(c, d, s, st);
 }
 
 }  // namespace
@@ -714,6 +716,7 @@ int make_call(const dc_attn_desc* d, Call& c, bool backward) {
   if (d->softcap > 0.0f) {
     c.cap2 = d->softcap * kLog2e;
     c.icap = 2.0f * kLog2e * d->scale / d->softcap;
+    c.wide = d->softcap > kWideCap ? 1.0f / d->softcap : 0.0f;
   }
   c.slopes = d->slopes;
   c.causal = d->causal;

@@ -427,3 +427,13 @@ def test_bias_that_grows_with_distance(ctx, tq, tk, causal, d, dtype):
     """Slopes of either sign, and row counts that end inside a tile: what lies behind the last row weighs nothing, however far."""
     slopes = torch.tensor([-0.05, 0.05, -2.0, 0.5], device=dev)
     check(ctx, shape(2, tq, tk, 4, 2, d, slopes=slopes, causal=causal), dtype, seed=31)
+
+
+@TYPES
+@pytest.mark.parametrize("tq,d", [(4, 64), (130, 64), (33, 128), (129, 128)])
+@pytest.mark.parametrize("cap", [64.0, 65.0, 1e4, 1e6, 1e30])
+def test_wide_caps(ctx, cap, tq, d, dtype):
+    """A cap far above the scores leaves them as they are, one that they reach bends them."""
+    slopes = 2.0 ** -torch.arange(1.0, 3.0, device=dev)
+    check(ctx, shape(1, tq, 300, 2, 1, d, softcap=cap, slopes=slopes), dtype, qscale=4.0, seed=32)
+    check(ctx, shape(1, tq, 300, 2, 2, d, softcap=cap, scale=0.5, causal=True), dtype, qscale=8.0, seed=33)
