@@ -627,13 +627,16 @@ int tile_splits(const dc_attn_desc* d, bool backward) {
 
 // Short rows go without summaries: the kernels visit every tile, and look at the documents of every key that they load.  us with and
 // without, 10 heads of 64, forward and gradients: 8 x 256 in 2 documents 47 38, 4 x 512 in 1 76 70, in 4 47 51, 4 x 1024 in 2 112 131.
-bool summarised(const dc_attn_desc* d) { return d->doc_q && (d->tq > 512 || d->tk > 512); }
+// token_kernel does not ask for them.
+bool summarised(const dc_attn_desc* d, bool backward) {
+  return d->doc_q && (d->tq > 512 || d->tk > 512) && (backward || !few_rows(d->tq));
+}
 // Lists where blocks are few (place_of) and one block can look at all tiles.  Entries: as many as the card holds (4/3 of it: 4 to 10 %
 // slower), or a block of rows each; a block has twice its even share of parts at most, as its documents may be the longest.
 Lists lists_of(const dc_attn_desc* d) {
   const long nk = (d->tk + 63L) / 64, nq = (d->tq + 63L) / 64, bq = d->nb * ((nq + 1) / 2), bk = d->nb * ((nk + 1) / 2);
   Lists l{};
-  l.on = summarised(d) && !few_rows(d->tq) && d->nb * (nk + nq) <= kSorted && bq * d->heads <= kSpread;
+  l.on = summarised(d, false) && d->nb * (nk + nq) <= kSorted && bq * d->heads <= kSpread;
   if (!l.on) return l;
   l.items_q = (int)bq;
   l.items_k = (int)bk;
@@ -650,14 +653,14 @@ bool query_tiles(const dc_attn_desc* d, bool backward) {
 }
 
 long long summary_bytes(const dc_attn_desc* d, bool backward) {
-  if (!summarised(d)) return 0;
+  if (!summarised(d, backward)) return 0;
   const long long sums = 16LL * d->nb * ((d->tk + 63L) / 64 + (query_tiles(d, backward) ? (d->tq + 63L) / 64 : 0));
   const Lists l = lists_of(d);
   return sums + (l.on ? (8LL * (l.entries_q + l.entries_k) + 4LL * (l.items_q + l.items_k) + 15) / 16 * 16 : 0);
 }
 
 void launch_summaries(const dc_attn_desc* d, Call& c, bool backward, char* ws, hipStream_t st) {
-  if (!summarised(d)) return;
+  if (!summarised(d, backward)) return;
   const int nk = (d->tk + 63) / 64, nq = query_tiles(d, backward) ? (d->tq + 63) / 64 : 0;
   int4* k = reinterpret_cast<int4*>(ws);
   c.sum_k = k;

@@ -129,3 +129,12 @@ def test_slopes_beside_no_scale():
         call(slopes=torch.zeros(4), scale=1e-31)
     d = descriptor(slopes=4096, scale=1e-31)
     assert _lib.load().dc_attn_mask_fwd(C.byref(d), 4096, 1 << 30, None) == ARG
+
+
+def test_scratch_of_few_rows():
+    """Documents of few query rows are looked at as their keys are read: without split keys the forward needs no scratch."""
+    lib = _lib.load()
+    few = descriptor(nb=64, tq=64, tk=600, heads=8, kv_heads=8, doc_q=4096, doc_k=4096)
+    assert lib.dc_attn_mask_ws_bytes(C.byref(few), 0) == 0
+    few.tq = 65
+    assert lib.dc_attn_mask_ws_bytes(C.byref(few), 0) >= 64 * 10 * 16   # a summary of each tile of keys
