@@ -43,10 +43,14 @@ __device__ __forceinline__ float near_sixteenth(float x) {
   return ldexpf(1.0f, min(max(-4 - e, -100), 100));
 }
 
-// EXACT: rowsum(dO o) from the rounded o is off by a rounding of o, the same for all keys of the row.  Rows of few keys, whose gradients
+// rowsum(dO o) from the rounded o is off by a rounding of o, the same for all keys of the row.  Rows of few keys, whose gradients
 // are small differences, take it from a sweep of its own over P dP: of 750 gradients of random calls of 8 to 6000 keys the furthest
 // (12 keys) was off by 0.46 % of its norm without and 0.36 % with (2009 keys), 264 and 49 of them by more than one rounding and a half.
-template <typename T, int DP, int FORM, bool EXACT>
+// A block does so where all its rows together meet at most kExact tiles (4 x 108 x 20 heads, forward and gradients: 34 us, 31 without), whatever
+// the length of the call that they are part of and the parts that they are split in.  SHORT: no block of the call meets more (the
+// question itself costs 8 x 1024 x 16 heads, causal, 9 us of 165).
+constexpr int kExact = 16;
+template <typename T, int DP, int FORM, bool SHORT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back bk) {
   typedef typename Vec<T>::v8 v8;
   constexpr int S = DP == 64 ? 3 : 2, TILE = 64 * DP, OPS = 2 * Dma<T, DP>::N;
@@ -85,11 +89,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   int t0, t1;
   int holes;
   q.tiles(p, sees, range, t0, t1, holes);
-  if (q.parts > 1) {
-    const int each = (t1 - t0 + q.parts - 1) / q.parts;
-    t0 = min(t1, t0 + q.part * each);
-    t1 = min(t1, t0 + each);
-  }
+  const int each = (t1 - t0 + q.parts - 1) / q.parts, part0 = min(t1, t0 + q.part * each), part1 = min(t1, part0 + each);
 
   Ring ring;
   ring.init(p, q, holes);
@@ -205,11 +205,13 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
         if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{}, F);
     }
   };
-  if constexpr (EXACT) {
+  if (SHORT || t1 - t0 <= kExact) {
     sweep(std::true_type{});
     del = pair_sum(exact);
     tile_barrier();
   }
+  t0 = part0;
+  t1 = part1;
   // (rows behind the last too: what dkv_kernel reads there has to weigh nothing, whatever its scores become)
   if (hh == 0 && q.part == 0) {
     const long at = ((long)q.b * p.heads + q.h) * 32 * bk.n32 + q.qi;
@@ -566,8 +568,7 @@ template <typename T, int DP, int FORM>
 void launch_bwd(const Call& c, const Back& bk, hipStream_t st) {
   const long nqb = (long)c.nb * ((c.tq + 127) / 128), nkb = (long)c.nb * ((c.tk + 127) / 128);
   const dim3 grid((unsigned)(c.heads * (c.list_q ? c.entries_q : nqb * bk.nq)));
-  // two sweeps up to 16 tiles of keys (4 x 108 x 20 heads, forward and gradients: 31 us for 35)
-  if (bk.nq == 1 && c.tk <= 1024) hipLaunchKernelGGL((dq_kernel<T, DP, FORM, true>), grid, dim3(256), 0, st, c, bk);
+  if (c.tk <= kExact * 64) hipLaunchKernelGGL((dq_kernel<T, DP, FORM, true>), grid, dim3(256), 0, st, c, bk);
   else hipLaunchKernelGGL((dq_kernel<T, DP, FORM, false>), grid, dim3(256), 0, st, c, bk);
   hipLaunchKernelGGL((dkv_kernel<T, DP, FORM>), dim3((unsigned)(c.kvh * (c.list_k ? c.entries_k : nkb * bk.nk))),
                      dim3(DP == 64 ? 256 : 512), 0, st, c, bk);

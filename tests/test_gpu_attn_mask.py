@@ -437,3 +437,29 @@ def test_wide_caps(ctx, cap, tq, d, dtype):
     slopes = 2.0 ** -torch.arange(1.0, 3.0, device=dev)
     check(ctx, shape(1, tq, 300, 2, 1, d, softcap=cap, slopes=slopes), dtype, qscale=4.0, seed=32)
     check(ctx, shape(1, tq, 300, 2, 2, d, softcap=cap, scale=0.5, causal=True), dtype, qscale=8.0, seed=33)
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["documents", "causal"])
+def test_short_rows_in_long_calls(ctx, kind, d, dtype):
+    """Gradients of rows of few keys inside a call of many, each document (or the first rows of a causal call) against its own norm.
+    The values share an offset of 16, which P (dP - rowsum) takes out again: rowsum(dO o) from a rounded o is off by up to 2^-8 (fp16
+    2^-11) of it, many times the differences' own roundings."""
+    from depth_completion_amd import ops
+    lengths, t = [12, 500, 30, 300, 400], 1500
+    ids = runs(lengths, t) if kind == "documents" else None
+    c = shape(1, t, t, 2, 1, d, **(dict(doc_q=ids, doc_k=ids) if ids is not None else dict(causal=True)))
+    q, k, v, do = inputs(c, dtype, 41)
+    v = (16.0 + 0.25 * v.float()).to(dtype)
+    o, lse = torch.empty_like(q), torch.empty(1, 2, t, device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+    _, _, rq, rk, _, _ = definition(q, k, v, c, do)
+    at = 0
+    for n in lengths if ids is not None else [1024]:
+        rows = slice(at, at + n)
+        assert rel(dq[rows], rq[rows]) < 4 * U[dtype], (at, n)
+        assert ids is None or rel(dk[rows], rk[rows]) < 4 * U[dtype], (at, n)
+        at += n
