@@ -7,8 +7,11 @@
 // query heads of its group).  Both compute S and dP again: 7 products for 5, for no exchange of dQ between blocks.
 //
 // fp16: dS is scaled by a power of two before it is rounded, by the row's (dQ) or the key head's (dK) largest |dO| so that this
-// lies in [2^-4, 2^-3): gradients far below 1 keep their digits, and dS stays in range while |v| < 2000.  P in dV is held 2^14 times
-// as large for the same reason.  Both factors are taken out of the fp32 sums again.
+// lies in [2^-4, 2^-3): gradients far below 1 keep their digits.  P in dV is held 2^14 times as large for the same reason.  Both
+// factors are taken out of the fp32 sums again.  With values in the thousands dS could leave the type so.  dK, whose keys are there,
+// takes a smaller factor where |dP| <= d max |dO| max |v| or |rowsum(dO o)| asks for it; dQ, which meets its keys as it goes, looks
+// at its sums at the end (inf times anything left none of a row finite) and sweeps once more with 2^-6 of these rows' factors, which
+// holds for every finite v: |dP - rowsum| to 2 x 128 x 2^-9 x 65504 = 32752.
 #include "attn_mask.h"
 #include <type_traits>
 
@@ -17,13 +20,16 @@ namespace {
 
 struct Back {
   float *nlse, *ndel;   // [nb heads][32 n32]: -lse log2 e (-inf: the row sees no key, or lies behind the last), -rowsum(dO o)
-  int2* rows32;         // [nb heads][n32]: of 32 rows, whether one sees no key, and the largest |dO| (its bits)
+  int2* rows32;         // [nb heads][n32]: of 32 rows, whether one sees no key, and the largest |dO|, or kRoom |rowsum(dO o)| (its bits)
   int n32;
   int nq, nk;           // splits of dq_kernel's sweep over the keys, of dkv_kernel's over the queries
   float *part_q, *part; // [nq][nb tq][heads][DP]; [nk][2][nb tk][kvh][DP]
 };
 
 template <typename T> constexpr bool is_half = __is_same(T, half);
+constexpr float kLess = 0.015625f;   // 2^-6, for dS that left the type's range
+constexpr float kRoom = 7.62939453125e-06f;   // 2^-17: what is kept below 2^-3 when it is multiplied by this stays below 2^14 itself
+__device__ __forceinline__ bool left_range(float sum) { return !(fabsf(sum) < INFINITY); }
 
 // what dS as the kernels hold it lacks (cap_score gives a quarter of the slope)
 __device__ __forceinline__ float ds_scale(const Call& p) { return p.cap2 != 0.0f ? 4.0f * p.scale : p.scale; }
@@ -47,8 +53,8 @@ __device__ __forceinline__ float near_sixteenth(float x) {
 // are small differences, take it from a sweep of its own over P dP: of 750 gradients of random calls of 8 to 6000 keys the furthest
 // (12 keys) was off by 0.46 % of its norm without and 0.36 % with (2009 keys), 264 and 49 of them by more than one rounding and a half.
 // A block does so where all its rows together meet at most kExact tiles (4 x 108 x 20 heads, forward and gradients: 34 us, 31 without), whatever
-// the length of the call that they are part of and the parts that they are split in.  SHORT: no block of the call meets more (the
-// question itself costs 8 x 1024 x 16 heads, causal, 9 us of 165).
+// the length of the call that they are part of and the parts that they are split in.  SHORT: no block of the call meets more, and
+// none reads o (which costs 8 x 1024 x 16 heads, causal, 9 us of 165).
 constexpr int kExact = 16;
 template <typename T, int DP, int FORM, bool SHORT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back bk) {
@@ -64,7 +70,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   const long row = ((long)q.b * p.heads + q.h) * p.tq + (q.live ? q.qi : 0), trow = (long)q.b * p.tq + (q.live ? q.qi : 0);
   const float lse = p.lse[row];
   const bool sees = q.live && lse != -INFINITY;
-  v8 qf[DP / 16], df[DP / 16];
+  v8 qf[DP / 16], df[DP / 16], of[DP / 16];
   float del = 0.0f, most = 0.0f;
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
@@ -72,25 +78,25 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     const bool ok = sees && c < p.d;
     qf[s] = load8_or_0((const T*)p.q + trow * p.ldq + q.h * p.d + c, ok);
     df[s] = load8_or_0((const T*)p.dout + trow * p.lddo + q.h * p.d + c, ok);
-    const v8 of = load8_or_0((const T*)p.o + trow * p.ldo + q.h * p.d + c, ok);
+    of[s] = load8_or_0((const T*)p.o + trow * p.ldo + q.h * p.d + c, ok);
+  }
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      del = fmaf((float)df[s][j], (float)of[j], del);
+      del = fmaf((float)df[s][j], (float)of[s][j], del);
       most = fmaxf(most, fabsf((float)df[s][j]));
     }
-  }
   del = pair_sum(del);
   most = pair_max(most);
   const float nl = sees ? -lse * kLog2e : -INFINITY;
-  const float wave_most = wave_max(most);
-  const bool blind = __any(q.live && !sees);
-  if (lane == 0 && q.part == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
-  const float f = is_half<T> ? near_sixteenth(most) : 1.0f;
+  float f = is_half<T> ? near_sixteenth(most) : 1.0f;
   int t0, t1;
   int holes;
   q.tiles(p, sees, range, t0, t1, holes);
   const int each = (t1 - t0 + q.parts - 1) / q.parts, part0 = min(t1, t0 + q.part * each), part1 = min(t1, part0 + each);
 
+  if (is_half<T> && threadIdx.x == 0) range[0] = 0;   // whether the sums have been swept again
   Ring ring;
   ring.init(p, q, holes);
   f32x16 dq[DP / 32];
@@ -196,13 +202,28 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     if (S == 3 && t + 2 < t1) ring.load(p, lds, t + 2, (buf + 2) % 3);
   };
   auto sweep = [&](auto F) __attribute__((always_inline)) {
-    if (t0 < t1) ring.load(p, lds, t0, 0);
-    if (S == 3 && t0 + 1 < t1) ring.load(p, lds, t0 + 1, 1);
-    for (int t = t0; t < t1; t += S) {
-      step(t, std::integral_constant<int, 0>{}, F);
-      if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{}, F);
-      if constexpr (S == 3)
-        if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{}, F);
+    constexpr bool FIRST = decltype(F)::value;
+    for (;;) {
+      int t = t0;
+      if constexpr (is_half<T> && !FIRST) asm volatile("" : "+s"(t));   // (what the loads start from is not kept for a second time)
+      if (t < t1) ring.load(p, lds, t, 0);
+      if (S == 3 && t + 1 < t1) ring.load(p, lds, t + 1, 1);
+      for (; t < t1; t += S) {
+        step(t, std::integral_constant<int, 0>{}, F);
+        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{}, F);
+        if constexpr (S == 3)
+          if (t + 2 < t1) step(t + 2, std::integral_constant<int, 2>{}, F);
+      }
+      if constexpr (!is_half<T> || FIRST) break;
+      tile_barrier();
+      const bool twice = range[0], over = left_range(dq[0][0]);
+      tile_barrier();
+      if (over) range[0] = 1;
+      tile_barrier();
+      if (twice || !range[0]) break;
+      if (over) f *= kLess;
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) dq[n] = f32x16{};
     }
   };
   if (SHORT || t1 - t0 <= kExact) {
@@ -212,6 +233,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
   }
   t0 = part0;
   t1 = part1;
+  const float wave_most = is_half<T> ? wave_max(fmaxf(most, kRoom * fabsf(del))) : 0.0f;
+  const bool blind = __any(q.live && !sees);
+  if (lane == 0 && q.part == 0) bk.rows32[((long)q.b * p.heads + q.h) * bk.n32 + q.qi / 32] = make_int2(blind, __float_as_int(wave_most));
   // (rows behind the last too: what dkv_kernel reads there has to weigh nothing, whatever its scores become)
   if (hh == 0 && q.part == 0) {
     const long at = ((long)q.b * p.heads + q.h) * 32 * bk.n32 + q.qi;
@@ -237,8 +261,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void dq_kernel(Call p, Back 
     }
 }
 
-// the factor of dS in dK for a key head: by the largest |dO| of its query heads, the same in every block that needs it
-__device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int b, int kh, float* scratch) {
+// what the factor of dS in dK goes by for a key head: the largest of its query heads' rows32, the same in every block that asks
+__device__ __forceinline__ float head_most(const Call& p, const Back& bk, int b, int kh, float* scratch) {
   const int2* r = bk.rows32 + ((long)b * p.heads + kh * p.grp) * bk.n32;
   float most = 0.0f;
   for (int i = threadIdx.x; i < p.grp * bk.n32; i += blockDim.x) most = fmaxf(most, __int_as_float(r[i].y));
@@ -246,7 +270,7 @@ __device__ __forceinline__ float head_factor(const Call& p, const Back& bk, int 
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = most;
   __syncthreads();
   for (int i = 0; i < (int)blockDim.x / 64; ++i) most = fmaxf(most, scratch[i]);
-  return near_sixteenth(most);
+  return most;
 }
 
 constexpr float kPShift = 14.0f;   // fp16: P in dV is 2^14 times as large
@@ -290,7 +314,15 @@ __global__ __launch_bounds__(DP == 64 ? 256 : 512, 2) void dkv_kernel(Call p, Ba
     kf[s] = load8_or_0((const T*)p.k + ((long)b * p.tk + key) * p.ldk + kh * p.d + c, ok && c < p.d);
     vf[s] = load8_or_0((const T*)p.v + ((long)b * p.tk + key) * p.ldv + kh * p.d + c, ok && c < p.d);
   }
-  const float f = is_half<T> ? head_factor(p, bk, b, kh, scratch) : 1.0f;
+  float f = 1.0f;   // of the lane's key
+  if constexpr (is_half<T>) {
+    float v = 0.0f;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf((float)vf[s][j]));
+    f = near_sixteenth(head_most(p, bk, b, kh, scratch) * fmaxf(1.0f, kRoom * DP * pair_max(v)));
+  }
   // the lane's key is seen from position `from` on
   const int from = !ok ? 0x7fffffff : p.causal && key >= pre ? key : -0x7fffffff;
   const int from_last = __builtin_amdgcn_readfirstlane(wave_max_i(from)), from_first = __builtin_amdgcn_readfirstlane(wave_min_i(from));

@@ -463,3 +463,54 @@ def test_short_rows_in_long_calls(ctx, kind, d, dtype):
         assert rel(dq[rows], rq[rows]) < 4 * U[dtype], (at, n)
         assert ids is None or rel(dk[rows], rk[rows]) < 4 * U[dtype], (at, n)
         at += n
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tq,docs,kv_heads", [(4, False, 2), (70, False, 1), (200, True, 2)])
+def test_large_values_of_two_keys(ctx, tq, docs, kv_heads, d):
+    """fp16 values near the type's largest, weights near a half and a dout with their signs: P (dP - rowsum) passes the type's range,
+    the gradients, of small q and k, do not.  (q and k of 2^-10: no gradient is above 1.5 d 60000 2^-10 2 rows.)"""
+    ids = (torch.arange(tq, dtype=torch.int32, device=dev) // 2).repeat(2) if docs else None
+    c = shape(2, tq, tq if docs else 2, 2, kv_heads, d, **(dict(doc_q=ids, doc_k=ids) if docs else {}))
+    q, k, v, do = inputs(c, torch.float16, 51)
+    q, k = (q.float() * 2.0 ** -10).half(), (k.float() * 2.0 ** -10).half()
+    size = 40000.0 + 20000.0 * torch.rand(v.shape, generator=torch.Generator().manual_seed(1)).to(dev)
+    alternate = 1.0 - 2.0 * (torch.arange(v.shape[0], device=dev) % 2)[:, None]
+    v = (size * alternate).half()
+    do = (do.float() * 0.25 + 1.5).half()
+    if not docs:   # (all rows add up in the two keys' gradients)
+        do = (do.float() / tq).half()
+        q = q * 4
+    check(ctx, c, torch.float16, tensors=(q, k, v, do))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_values_among_many_keys(ctx, d):
+    """The same with two heavy keys among 1100 (more than the rows whose rowsum has a sweep of its own), and four rows whose dout
+    is large beside the others'.  The heavy keys are both 50 in each column, to 0.05, so their shares of dQ cancel but for a tenth:
+    dS of each is rounded, by u at most, and so is o in rowsum(dO o), by u of sum |dO o|, which is |rowsum| where dO and o have one sign
+    each, as in the rows that count.  Both bound dQ's error by u times the norm of P (|dP| + |rowsum|) |K|, `size`, beside its own
+    rounding."""
+    from depth_completion_amd import ops
+    t = 1100
+    c = shape(1, t, t, 2, 1, d, scale=0.04 / d)
+    q, k, v, do = inputs(c, torch.float16, 52)
+    signs = torch.sign(q[:1, :d].float())
+    q = (4.0 * signs.repeat(t, 2) + 0.2 * q.float()).half()
+    k = 0.05 * k.float()
+    k[:2] += 50.0 * signs
+    v = v.float()
+    v[0], v[1] = 60000.0, -30000.0
+    do = 0.01 * do.float()
+    do[::300] += 1.5
+    k, v, do = k.half(), v.half(), do.half()
+    o, lse = torch.empty_like(q), torch.empty(1, 2, t, device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+    ro, _, rq, rk, rv, size = definition(q, k, v, c, do)
+    u = U[torch.float16]
+    assert rel(o, ro) < 2 * u
+    for name, x, r in (("dq", dq, rq), ("dk", dk, rk), ("dv", dv, rv)):
+        off, norm = float((x.double().cpu() - r).norm()), float(r.norm())
+        assert off <= max(4 * u * norm, 2 * u * size[name] + u * norm if name == "dq" else 0.0), (name, off, norm, size[name])
