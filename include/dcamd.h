@@ -457,10 +457,13 @@ int dc_complete(dc_session* s, const void* imgs_u8, const float* sparses, int n,
  *   s = scale q_i . k_j;  softcap c > 0: s = c tanh(s / c);  slopes: s -= slopes[h] |pos(i) - j|
  *   key j counts where j < L, doc_q[i] == doc_k[j] >= 0 (documents given), and j <= pos(i) or j < prefix[b] (causal)
  *   o = softmax(s) v;  lse = log sum exp(s).  A row that sees no key: o = 0, lse = -inf, and its gradients are 0.
- * Rows of q / k / v / dout that no pair reaches (keys from L on, documents below 0, rows that see no key) may hold anything.
- * A visible key that is not finite may also reach other rows of its tile of 64 keys.  Sums and softmax statistics are fp32, the
- * weights P and dS are rounded to the type for the matrix units (dS of fp16 scaled by a power of two so that small gradients
- * keep their digits).  Gradients of shared key heads are summed over their query heads in a fixed order; no atomics.
+ * Rows of q / k / v / dout may hold anything where they are keys from L on, in a document below 0, or query rows that see no key.
+ * All other keys are read and have to be finite, those included whose document no query is in: one that is not may reach any row of
+ * a tile of 64 keys that it shares.  Sums and softmax statistics are fp32, the weights P and dS are rounded to the type for the
+ * matrix units (dS of fp16 scaled by a power of two so that small gradients keep their digits).  rowsum(dout o) in dS is taken from
+ * o as it was rounded; a block of 128 query rows that meets at most 16 tiles of 64 keys forms it again, as rowsum(P dP) in fp32,
+ * which leaves dq and dk their own rounding and that of dS.  Gradients of shared key heads are summed over their query heads in a
+ * fixed order; no atomics.
  * type: 0 bf16, 1 fp16.  d: a multiple of 8.  Pointers 16-byte aligned, ld* multiples of 8.  Inputs and outputs may not overlap.
  * nb heads tq and nb kv_heads tk below 2^30, nb heads (and kv_heads) times blocks of 128 rows below 2^23, ldk and ldv (in the
  * backward ldq and lddo too) at most 2^23. */
