@@ -514,3 +514,71 @@ def test_large_values_among_many_keys(ctx, d):
     for name, x, r in (("dq", dq, rq), ("dk", dk, rk), ("dv", dv, rv)):
         off, norm = float((x.double().cpu() - r).norm()), float(r.norm())
         assert off <= max(4 * u * norm, 2 * u * size[name] + u * norm if name == "dq" else 0.0), (name, off, norm, size[name])
+
+
+def near(ctx, c, dtype, seed, qscale=1.0):
+    """As check(), against what independent roundings leave: one is off by u at most and by u / sqrt(3) in the root mean square, k of
+    them by sqrt(k / 3) u.  k: o its own and P's, dV its own and P's, dQ and dK their own, dS's and that of o in rowsum(dO o)."""
+    from depth_completion_amd import ops
+    q, k, v, do = inputs(c, dtype, seed, qscale)
+    o, lse = torch.empty_like(q), torch.empty(c["nb"], c["heads"], c["tq"], device=dev)
+    ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+    ro, rl, rq, rk, rv, _ = definition(q, k, v, c, do)
+    seen = torch.isfinite(rl)
+    assert torch.equal(torch.isinf(lse.cpu()), ~seen)
+    assert float(((lse.cpu().double() - rl)[seen].abs() / rl[seen].abs().clamp_min(1.0)).max()) < (1e-5 if c.get("softcap") else 2e-6)
+    for name, x, r, n in (("o", o, ro, 2), ("dv", dv, rv, 2), ("dq", dq, rq, 3), ("dk", dk, rk, 3)):
+        assert rel(x, r) < math.sqrt(n / 3) * U[dtype], (name, rel(x, r), U[dtype])
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nb,tq,tk,heads,kv_heads,lengths,kv_len,cap,causal", [
+    (1, 1500, 1500, 2, 1, [700, 90, 600], None, 0.0, False),      # a bias inside documents, some blocks split
+    (2, 300, 300, 4, 2, [140, 130], None, 25.0, True),            # with a cap, short rows
+    (1, 1700, 1700, 2, 2, [1100, 500], None, 25.0, False),
+    (3, 200, 900, 4, 1, None, [900, 333, 640], 0.0, True),        # a bias over filled lengths
+    (1, 200, 5000, 2, 1, None, None, 0.0, True),                  # split keys, split sweeps
+    (1, 200, 5000, 2, 1, None, None, 25.0, False),
+    (2, 5, 3000, 4, 2, [1000, 1900], [3000, 2500], 0.0, True)])   # a few rows at the end of two caches
+def test_bias_with_other_masks(ctx, nb, tq, tk, heads, kv_heads, lengths, kv_len, cap, causal, d, dtype):
+    c = shape(nb, tq, tk, heads, kv_heads, d, softcap=cap, causal=causal,
+              slopes=torch.tensor([0.01, -0.002, 0.03, 0.001][:heads], device=dev))
+    if lengths:
+        ids = runs(lengths, tk)
+        c["doc_k"] = ids.repeat(nb)
+        c["doc_q"] = c["doc_k"] if tq == tk else ids[sum(lengths) - tq:sum(lengths)].repeat(nb)
+    if kv_len:
+        c["kv_len"] = torch.tensor(kv_len, dtype=torch.int32, device=dev)
+    near(ctx, c, dtype, 61)
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tk", [1024, 1025, 1088, 1153])
+def test_border_of_short_rows(ctx, tk, d, dtype):
+    """16 tiles of keys, where rowsum has a sweep of its own, and 17 and more, where it is taken from o."""
+    near(ctx, shape(1, 130, tk, 2, 1, d), dtype, 62)
+    near(ctx, shape(1, tk, tk, 2, 2, d, causal=True), dtype, 63)
+
+
+def test_same_bits_of_other_forms(ctx):
+    """As test_same_bits_every_time: listed documents in parts, short rows, fp16 sums that are swept again, wide caps."""
+    from depth_completion_amd import ops
+    ids = runs([900, 60, 700], 1700)
+    for c, dtype, big in ((shape(1, 1700, 1700, 3, 1, 64, doc_q=ids, doc_k=ids, softcap=30.0), torch.bfloat16, 1.0),
+                          (shape(2, 300, 300, 4, 2, 128, causal=True), torch.float16, 30000.0),
+                          (shape(1, 50, 700, 8, 2, 128, softcap=500.0), torch.float16, 1.0)):
+        q, k, v, do = inputs(c, dtype, 71)
+        v = (v.float().clamp(-2, 2) * big).to(dtype)
+        got = []
+        for _ in range(3):
+            o, lse = torch.empty_like(q), torch.empty(c["nb"], c["heads"], c["tq"], device=dev)
+            ops.attn_mask_fwd(ctx, q, k, v, o, lse, **c)
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            ops.attn_mask_bwd(ctx, q, k, v, o, lse, do, dq, dk, dv, **c)
+            got.append((o, lse, dq, dk, dv))
+        for other in got[1:]:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got[0], other))
